@@ -213,6 +213,37 @@ typedef struct HstuJaggedBwdArgs {
 HSTU_API int hstu_jagged_bwd_get_workspace_size(const HstuJaggedBwdArgs* args, uint64_t* workspace_bytes);
 HSTU_API int hstu_jagged_bwd(const HstuJaggedBwdArgs* args, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------- sliding window
+ * The forward and its gradients over a sliding window with sinks (no counterpart in the reference): the row at position
+ * p = i + (len_k - len_q) of its sequence sees the keys j <= p with  p - j < window  or  j < num_sink, everything else of
+ * the formula being the jagged operator's.  A target row (num_target and target_group_size > 0) counts its window from the
+ * end of the history, p = len_k - num_target: it sees the history keys that are left, and the targets of its own group up
+ * to itself.  A row that sees nothing (len_q > len_k) gives zeros.  Arithmetic and traffic follow the visible tiles, not
+ * len^2.
+ *   fwd        the jagged arguments, with mask_type HSTU_MASK_TRIL and without mask, attn_bias and num_context
+ *   window     >= 1, the row's own key among them; window >= max_seq_len_k is the jagged operator
+ *   num_sink   >= 0 */
+typedef struct HstuWindowArgs {
+  uint32_t struct_bytes;  /* sizeof(HstuWindowArgs) */
+  int32_t window;
+  int32_t num_sink;
+  uint32_t reserved;
+  HstuJaggedArgs fwd;
+} HstuWindowArgs;
+HSTU_API int hstu_window_fwd_get_workspace_size(const HstuWindowArgs* args, uint64_t* workspace_bytes);
+HSTU_API int hstu_window_fwd(const HstuWindowArgs* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* Gradients of hstu_window_fwd with respect to q, k and v (`bwd.fwd.out` is not read; grad_bias must be null). */
+typedef struct HstuWindowBwdArgs {
+  uint32_t struct_bytes;  /* sizeof(HstuWindowBwdArgs) */
+  int32_t window;
+  int32_t num_sink;
+  uint32_t reserved;
+  HstuJaggedBwdArgs bwd;
+} HstuWindowBwdArgs;
+HSTU_API int hstu_window_bwd_get_workspace_size(const HstuWindowBwdArgs* args, uint64_t* workspace_bytes);
+HSTU_API int hstu_window_bwd(const HstuWindowBwdArgs* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------------------ ln_mul
  * The step that consumes the attention output in an HSTU layer: out = (LayerNorm(x) * gamma + beta) * u over the
  * rows of fp32 [rows, cols] matrices, eps = 1e-5 (fixed by the reference's host code, ln_mul/op_host/ln_mul.cpp:73).

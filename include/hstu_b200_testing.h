@@ -22,6 +22,12 @@ HSTU_API int hstu_debug_tiles_host(int32_t len_q, int32_t len_k, int32_t num_con
                           int32_t target_group_size, int32_t mask_type, int32_t r0, int32_t rows, int32_t bn,
                           uint64_t* full_bits);
 
+/* The mask algebra of hstu_window, evaluated on the host: visible[len_q * len_k]; and for the q-tile of rows
+ * [r0, r0 + rows) on K tiles of width bn, tiles[3 * len_k], per key whether its tile is visited by the q-tile, is visited
+ * without a predicate, and is asked for by a pass over key tiles. */
+HSTU_API int hstu_debug_window_host(int32_t len_q, int32_t len_k, int32_t num_target, int32_t target_group_size, int32_t window,
+                           int32_t num_sink, int32_t r0, int32_t rows, int32_t bn, uint8_t* visible, uint8_t* tiles);
+
 /* out[i] = a[i] / b[i], fp32 device arrays, by the quotient of the fp32 kernels' SiLU and sigmoid (b >= 1). */
 HSTU_API int hstu_debug_divide(const void* a, const void* b, void* out, int64_t n, void* stream);
 

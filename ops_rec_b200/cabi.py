@@ -28,6 +28,8 @@ EXPORTS = (
     "hstu_jagged_bwd_get_workspace_size", "hstu_jagged_bwd", "ops_rec_ln_mul_f32", "ops_rec_in_linear_silu_fwd",
     "hstu_paged_fwd_get_workspace_size", "hstu_paged_fwd",
     "ops_rec_in_linear_silu_bwd_get_workspace_size", "ops_rec_in_linear_silu_bwd",
+    "hstu_window_fwd_get_workspace_size", "hstu_window_fwd", "hstu_window_bwd_get_workspace_size", "hstu_window_bwd",
+    "hstu_debug_window_host",
 )
 STATIC_SCRATCH_BYTES = 1 << 20
 E_SCRATCH_LIMIT = -6
@@ -63,6 +65,16 @@ class HstuJaggedBwdArgs(C.Structure):
         ("grad_out", C.c_void_p), ("grad_q", C.c_void_p), ("grad_k", C.c_void_p), ("grad_v", C.c_void_p),
         ("grad_bias", C.c_void_p),
     ]
+
+
+class HstuWindowArgs(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("window", C.c_int32), ("num_sink", C.c_int32), ("reserved", C.c_uint32),
+                ("fwd", HstuJaggedArgs)]
+
+
+class HstuWindowBwdArgs(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("window", C.c_int32), ("num_sink", C.c_int32), ("reserved", C.c_uint32),
+                ("bwd", HstuJaggedBwdArgs)]
 
 
 class OpsRecInLinearSiluArgs(C.Structure):
@@ -143,6 +155,15 @@ def load():
     lib.ops_rec_in_linear_silu_bwd_get_workspace_size.restype = C.c_int
     lib.ops_rec_in_linear_silu_bwd.argtypes = [LB, C.c_void_p, C.c_uint64, C.c_void_p]
     lib.ops_rec_in_linear_silu_bwd.restype = C.c_int
+    W, WB = C.POINTER(HstuWindowArgs), C.POINTER(HstuWindowBwdArgs)
+    lib.hstu_window_fwd_get_workspace_size.argtypes = [W, C.POINTER(C.c_uint64)]
+    lib.hstu_window_fwd.argtypes = [W, C.c_void_p, C.c_uint64, C.c_void_p]
+    lib.hstu_window_bwd_get_workspace_size.argtypes = [WB, C.POINTER(C.c_uint64)]
+    lib.hstu_window_bwd.argtypes = [WB, C.c_void_p, C.c_uint64, C.c_void_p]
+    lib.hstu_debug_window_host.argtypes = [C.c_int32] * 9 + [C.c_void_p] * 2
+    for name in ("hstu_window_fwd_get_workspace_size", "hstu_window_fwd", "hstu_window_bwd_get_workspace_size",
+                 "hstu_window_bwd", "hstu_debug_window_host"):
+        getattr(lib, name).restype = C.c_int
     lib.ops_rec_ln_mul_f32.argtypes = [C.c_void_p] * 5 + [C.c_int64, C.c_int64, C.c_void_p]
     lib.ops_rec_ln_mul_f32.restype = C.c_int
     lib.ops_rec_in_linear_silu_fwd.argtypes = [C.POINTER(OpsRecInLinearSiluArgs), C.c_void_p]
@@ -306,6 +327,64 @@ def hstu_jagged_backward(grad, q, k, v, mask=None, attn_bias=None, mask_type=0, 
             return (dq, dk, dv, dbias), st.value
     del keep
     return dq, dk, dv, dbias
+
+
+def hstu_window_forward(q, k, v, window, num_sink=0, max_seq_len=0, max_seq_len_k=0, silu_scale=0.0, seq_offset=None,
+                        seq_offset_k=None, num_target=None, target_group_size=0, alpha=1.0, *, flags=0, return_status=False):
+    """ops_rec::hstu_window through hstu_window_fwd on CUDA tensors; with return_status it synchronises and returns the
+    device status word too."""
+    import torch
+    if q.dim() != 3:
+        raise HstuError(-2, "The q should be 3D in jagged layout")
+    if not q.is_cuda:
+        raise HstuError(-2, "tensors must live on a CUDA device; there is no CPU implementation")
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    out = torch.empty(q.shape[0], q.shape[1], v.shape[2], dtype=q.dtype, device=q.device)
+    fwd, keep = make_args(q, k, v, out, seq_offset, seq_offset_k=seq_offset_k, max_seq_len=max_seq_len,
+                          max_seq_len_k=max_seq_len_k or None, silu_scale=silu_scale, num_target=num_target,
+                          target_group_size=target_group_size, alpha=alpha, flags=flags)
+    a = HstuWindowArgs(C.sizeof(HstuWindowArgs), int(window), int(num_sink), 0, fwd)
+    n = C.c_uint64(0)
+    check(load().hstu_window_fwd_get_workspace_size(C.byref(a), C.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    with torch.cuda.device(q.device):
+        check(load().hstu_window_fwd(C.byref(a), ws.data_ptr(), n.value, stream))
+        if return_status:
+            st = C.c_uint32(0)
+            check(load().hstu_jagged_fwd_status(ws.data_ptr(), stream, C.byref(st)))
+            return out, st.value
+    del keep
+    return out
+
+
+def hstu_window_backward(grad, q, k, v, window, num_sink=0, max_seq_len=0, max_seq_len_k=0, silu_scale=0.0, seq_offset=None,
+                         seq_offset_k=None, num_target=None, target_group_size=0, alpha=1.0, *, flags=0, return_status=False):
+    """Gradients (dq, dk, dv) through hstu_window_bwd on CUDA tensors."""
+    import torch
+    if q.dim() != 3:
+        raise HstuError(-2, "The q should be 3D in jagged layout")
+    if not q.is_cuda:
+        raise HstuError(-2, "tensors must live on a CUDA device; there is no CPU implementation")
+    grad, q, k, v = grad.contiguous(), q.contiguous(), k.contiguous(), v.contiguous()
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    fwd, keep = make_args(q, k, v, None, seq_offset, seq_offset_k=seq_offset_k, max_seq_len=max_seq_len,
+                          max_seq_len_k=max_seq_len_k or None, silu_scale=silu_scale, num_target=num_target,
+                          target_group_size=target_group_size, alpha=alpha, flags=flags)
+    b = HstuJaggedBwdArgs(C.sizeof(HstuJaggedBwdArgs), 0, fwd, grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None)
+    a = HstuWindowBwdArgs(C.sizeof(HstuWindowBwdArgs), int(window), int(num_sink), 0, b)
+    n = C.c_uint64(0)
+    check(load().hstu_window_bwd_get_workspace_size(C.byref(a), C.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    with torch.cuda.device(q.device):
+        check(load().hstu_window_bwd(C.byref(a), ws.data_ptr(), n.value, stream))
+        if return_status:
+            st = C.c_uint32(0)
+            check(load().hstu_jagged_fwd_status(ws.data_ptr(), stream, C.byref(st)))
+            return (dq, dk, dv), st.value
+    del keep
+    return dq, dk, dv
 
 
 def hstu_paged_forward(q, k, v, kv_cache, mask=None, attn_bias=None, mask_type=0, max_seq_len=0, max_seq_len_k=0,
@@ -498,6 +577,16 @@ def debug_mask(len_q, len_k, ctx, tgt, group, mask_type=0):
     out = np.zeros((len_q, len_k), dtype=np.uint8)
     check(load().hstu_debug_mask_host(len_q, len_k, ctx, tgt, group, mask_type, out.ctypes.data))
     return out.astype(bool)
+
+
+def debug_window(len_q, len_k, tgt, group, window, sink, r0, rows, bn):
+    """(visible [len_q, len_k], times each key is visited, keys visited without a predicate, keys of tiles that may be seen) of
+    the q-tile of rows [r0, r0 + rows) on K tiles of width bn, from the device's own mask algebra compiled for the host."""
+    out = np.zeros((len_q, len_k), dtype=np.uint8)
+    tiles = np.zeros((3, len_k), dtype=np.uint8)
+    check(load().hstu_debug_window_host(len_q, len_k, tgt, group, window, sink, r0, rows, bn, out.ctypes.data,
+                                        tiles.ctypes.data))
+    return out.astype(bool), tiles[0], tiles[1].astype(bool), tiles[2].astype(bool)
 
 
 def debug_tiles(len_q, len_k, ctx, tgt, group, mask_type, r0, rows, bn):

@@ -196,7 +196,7 @@ int hstu_jagged_fwd_kernel_kind(const HstuJaggedArgs* args) {
   return wants_tc(args, p) ? 1 : 0;
 }
 
-// `paged` (hstu_paged only): parameters that carry the page table, for the pre-pass's consistency check.
+// `paged` (hstu_paged, hstu_window): parameters that carry what HstuJaggedArgs has no place for - the page table, the window.
 static int jagged_fwd_impl(const HstuJaggedArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v,
                            const hstu::KParams* paged);
 
@@ -238,6 +238,8 @@ static int jagged_fwd_impl(const HstuJaggedArgs* args, void* workspace, uint64_t
     p.paged_split = paged->paged_split;
     p.k_new = paged->k_new;
     p.v_new = paged->v_new;
+    p.window = paged->window;
+    p.sink = paged->sink;
   }
   const bool tc = wants_tc(args, p);
   cudaError_t e = hstu::launch_prepass(p, tc, stream);
@@ -251,6 +253,48 @@ static int jagged_fwd_impl(const HstuJaggedArgs* args, void* workspace, uint64_t
   }
   if (e != cudaSuccess) return fail(HSTU_E_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   return HSTU_OK;
+}
+
+// -------------------------------------------------------------------------------------------------- window
+namespace {
+// A window or a number of sinks beyond any sequence (2^24 keys) is every key, and leaves room for sums in 32 bits.
+constexpr int kMostWindow = 1 << 24;
+
+int validate_window(const HstuJaggedArgs* a, int window, int num_sink) {
+  if (window < 1) return fail(HSTU_E_PARAM, "window expect at least 1, but value is %d", window);
+  if (num_sink < 0) return fail(HSTU_E_PARAM, "num_sink expect at least 0, but value is %d", num_sink);
+  if (a->mask_type != HSTU_MASK_TRIL || a->mask) return fail(HSTU_E_PARAM, "a window takes no mask: maskType must be 0");
+  if (a->attn_bias) return fail(HSTU_E_PARAM, "a window takes no attn_bias");
+  if (a->num_context) return fail(HSTU_E_PARAM, "a window takes no num_context (num_sink keeps the first keys visible)");
+  return HSTU_OK;
+}
+int validate_window_fwd(const HstuWindowArgs* a) {
+  if (!a) return fail(HSTU_E_NULL, "args is null");
+  if (a->struct_bytes != sizeof(HstuWindowArgs))
+    return fail(HSTU_E_PARAM, "struct_bytes is %u, this library expects %zu", a->struct_bytes, sizeof(HstuWindowArgs));
+  const int rc = validate_window(&a->fwd, a->window, a->num_sink);
+  return rc ? rc : validate(&a->fwd);
+}
+void set_window(hstu::KParams* p, int window, int num_sink) {
+  p->window = window < kMostWindow ? window : kMostWindow;
+  p->sink = num_sink < kMostWindow ? num_sink : kMostWindow;
+}
+}  // namespace
+
+int hstu_window_fwd_get_workspace_size(const HstuWindowArgs* args, uint64_t* workspace_bytes) {
+  g_err[0] = 0;
+  const int rc = validate_window_fwd(args);
+  return rc ? rc : hstu_jagged_fwd_get_workspace_size(&args->fwd, workspace_bytes);
+}
+
+int hstu_window_fwd(const HstuWindowArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v) {
+  g_err[0] = 0;
+  const int rc = validate_window_fwd(args);
+  if (rc) return rc;
+  hstu::KParams p;
+  memset(&p, 0, sizeof(p));
+  set_window(&p, args->window, args->num_sink);
+  return jagged_fwd_impl(&args->fwd, workspace, workspace_bytes, stream_v, &p);
 }
 
 // --------------------------------------------------------------------------------------------------- paged
@@ -398,8 +442,37 @@ int hstu_jagged_bwd_get_workspace_size(const HstuJaggedBwdArgs* args, uint64_t* 
   return HSTU_OK;
 }
 
+static int jagged_bwd_impl(const HstuJaggedBwdArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v,
+                           int window, int num_sink);
+
 int hstu_jagged_bwd(const HstuJaggedBwdArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v) {
   g_err[0] = 0;
+  return jagged_bwd_impl(args, workspace, workspace_bytes, stream_v, 0, 0);
+}
+
+static int validate_window_bwd(const HstuWindowBwdArgs* a) {
+  if (!a) return fail(HSTU_E_NULL, "args is null");
+  if (a->struct_bytes != sizeof(HstuWindowBwdArgs))
+    return fail(HSTU_E_PARAM, "struct_bytes is %u, this library expects %zu", a->struct_bytes, sizeof(HstuWindowBwdArgs));
+  if (a->bwd.grad_bias) return fail(HSTU_E_PARAM, "a window takes no attn_bias: grad_bias must be null");
+  const int rc = validate_window(&a->bwd.fwd, a->window, a->num_sink);
+  return rc ? rc : validate_bwd(&a->bwd);
+}
+
+int hstu_window_bwd_get_workspace_size(const HstuWindowBwdArgs* args, uint64_t* workspace_bytes) {
+  g_err[0] = 0;
+  const int rc = validate_window_bwd(args);
+  return rc ? rc : hstu_jagged_bwd_get_workspace_size(&args->bwd, workspace_bytes);
+}
+
+int hstu_window_bwd(const HstuWindowBwdArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v) {
+  g_err[0] = 0;
+  const int rc = validate_window_bwd(args);
+  return rc ? rc : jagged_bwd_impl(&args->bwd, workspace, workspace_bytes, stream_v, args->window, args->num_sink);
+}
+
+static int jagged_bwd_impl(const HstuJaggedBwdArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v,
+                           int window, int num_sink) {
   int rc = validate_bwd(args);
   if (rc) return rc;
   const HstuJaggedArgs* f = &args->fwd;
@@ -422,6 +495,7 @@ int hstu_jagged_bwd(const HstuJaggedBwdArgs* args, void* workspace, uint64_t wor
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   hstu::BwdParams bp;
   bp.f = to_params(f, workspace, ws_need);
+  set_window(&bp.f, window, num_sink);
   bp.dout = args->grad_out;
   bp.dq = args->grad_q;
   bp.dk = args->grad_k;
@@ -651,6 +725,34 @@ int hstu_debug_mask_host(int32_t len_q, int32_t len_k, int32_t num_context, int3
     const hstu::RowBounds rb = hstu::row_bounds(s, i, mask_type, target_group_size);
     for (int j = 0; j < len_k; ++j) out[static_cast<size_t>(i) * len_k + j] = hstu::allowed(rb, j) ? 1 : 0;
   }
+  return HSTU_OK;
+}
+
+int hstu_debug_window_host(int32_t len_q, int32_t len_k, int32_t num_target, int32_t target_group_size, int32_t window,
+                           int32_t num_sink, int32_t r0, int32_t rows, int32_t bn, uint8_t* visible, uint8_t* tiles) {
+  g_err[0] = 0;
+  if (!visible || !tiles || len_q < 0 || len_k < 0 || rows < 1 || bn < 1 || window < 1 || num_sink < 0)
+    return fail(HSTU_E_PARAM, "hstu_debug_window_host: bad arguments");
+  hstu::KParams p;
+  memset(&p, 0, sizeof(p));
+  p.group = target_group_size;
+  set_window(&p, window, num_sink);
+  hstu::SeqInfo s = {0, 0, len_q, len_k, 0, num_target};
+  using Mask = hstu::MaskOf<true>;
+  for (int i = 0; i < len_q; ++i) {
+    const hstu::WinBounds rb = Mask::bounds(p, s, i);
+    for (int j = 0; j < len_k; ++j) visible[static_cast<size_t>(i) * len_k + j] = hstu::allowed(rb, j) ? 1 : 0;
+  }
+  memset(tiles, 0, static_cast<size_t>(3) * len_k);
+  const hstu::KeyTiles t = Mask::tiles(p, s, r0, rows, bn);
+  for (int n = 0; n < t.n; ++n) {
+    const int c0 = hstu::key_of_tile(t, n, bn);
+    for (int j = c0; j < c0 + bn && j < len_k; ++j) {
+      ++tiles[j];   // (2 and more: visited twice)
+      tiles[len_k + j] = Mask::full(p, s, r0, rows, c0, bn) ? 1 : 0;
+    }
+  }
+  for (int j = 0; j < len_k; ++j) tiles[2 * static_cast<size_t>(len_k) + j] = Mask::sees(p, s, r0, rows, j / bn * bn, bn) ? 1 : 0;
   return HSTU_OK;
 }
 

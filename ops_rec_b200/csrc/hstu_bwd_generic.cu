@@ -79,8 +79,9 @@ __device__ __forceinline__ void score_grad(const KParams& p, int b, int h, int i
   *dbias_out = db;
 }
 
-template <typename T>
+template <typename T, bool kWin>
 __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dq_kernel(const BwdParams bp) {
+  using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
   const KParams& p = bp.f;
   const int bh = blockIdx.x;
@@ -94,8 +95,9 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dq_kernel(const BwdParams b
   T* dbias = static_cast<T*>(bp.dbias);
   const long long brow0 = (static_cast<long long>(b) * p.hq + h) * p.maxq;  // first bias row of (b, h)
 
-  const int ntiles = kv_tiles_for_rows(s, r0, BT, p.mask_type, BT);
-  if (dbias) {
+  const KeyTiles tiles = Mask::tiles(p, s, r0, BT, BT);
+  const int ntiles = tiles.n;
+  if (dbias) {   // (never with a window)
     // zeros of this CTA's d_bias rows: everything right of the visited tiles (all columns when none is visited)
     const int first = ntiles * BT;
     const int width = p.maxk - first;
@@ -104,6 +106,12 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dq_kernel(const BwdParams b
         const int r = idx / width, c = idx - r * width;
         if (r0 + r < p.maxq) dbias[(brow0 + r0 + r) * p.maxk + first + c] = cvt_f<T>(0.f);
       }
+    }
+  }
+  if (ntiles == 0) {   // no row of the tile sees anything: their gradients are zeros
+    for (int idx = tid; idx < BT * p.dqk; idx += BTHREADS) {
+      const int r = idx / p.dqk, d = idx - r * p.dqk;
+      if (r0 + r < s.lq) static_cast<T*>(bp.dq)[((s.q0 + r0 + r) * p.hq + h) * p.dqk + d] = cvt_f<T>(0.f);
     }
   }
   if (ntiles == 0) return;
@@ -120,14 +128,14 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dq_kernel(const BwdParams b
   load_tile<T>(Gs, ldv, static_cast<const T*>(bp.dout), s.q0, r0, s.lq, p.hq, h, dv);
 
   const int i = r0 + ty;
-  const RowBounds rb = row_bounds(s, i < s.lq ? i : s.lq - 1, p.mask_type, p.group);
+  const typename Mask::Bounds rb = Mask::bounds(p, s, i < s.lq ? i : s.lq - 1);
   float acc[BMAXC];
 #pragma unroll
   for (int c = 0; c < BMAXC; ++c) acc[c] = 0.f;
   const int ncol = (dq + BT - 1) / BT;
 
   for (int t = 0; t < ntiles; ++t) {
-    const int c0 = t * BT;
+    const int c0 = kWin ? key_of_tile(tiles, t, BT) : t * BT;
     __syncthreads();  // the previous tile's Ks / Vs / Ds are consumed (and, for t == 0, Qs / Gs are filled)
     load_tile<T>(Ks, ldq, static_cast<const T*>(p.k), s.k0, c0, s.lk, p.hk, hk, dq);
     load_tile<T>(Vs, ldv, static_cast<const T*>(p.v), s.k0, c0, s.lk, p.hk, hk, dv);
@@ -163,8 +171,9 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dq_kernel(const BwdParams b
   }
 }
 
-template <typename T>
+template <typename T, bool kWin>
 __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dkv_kernel(const BwdParams bp) {
+  using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
   const KParams& p = bp.f;
   const int bh = blockIdx.x;
@@ -192,19 +201,18 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dkv_kernel(const BwdParams 
 #pragma unroll
   for (int c = 0; c < BMAXC; ++c) acc_k[c] = acc_v[c] = 0.f;
   const int ncol_k = (dq + BT - 1) / BT, ncol_v = (dv + BT - 1) / BT;
-  const int ktile = c0 / BT;
   const int j = c0 + tx;
 
   for (int hh = 0; hh < p.gqa_ratio; ++hh) {
     const int h = hk * p.gqa_ratio + hh;
     for (int r0 = 0; r0 < s.lq; r0 += BT) {
-      if (kv_tiles_for_rows(s, r0, BT, p.mask_type, BT) <= ktile) continue;  // no row of this q-tile sees these keys
+      if (!Mask::sees(p, s, r0, BT, c0, BT)) continue;  // no row of this q-tile sees these keys
       __syncthreads();  // the previous Qs / Gs / Ps / Ds are consumed (and, first time, Ks / Vs are filled)
       load_tile<T>(Qs, ldq, static_cast<const T*>(p.q), s.q0, r0, s.lq, p.hq, h, dq);
       load_tile<T>(Gs, ldv, static_cast<const T*>(bp.dout), s.q0, r0, s.lq, p.hq, h, dv);
       __syncthreads();
       const int i = r0 + ty;
-      const RowBounds rb = row_bounds(s, i < s.lq ? i : s.lq - 1, p.mask_type, p.group);
+      const typename Mask::Bounds rb = Mask::bounds(p, s, i < s.lq ? i : s.lq - 1);
       float sc = 0.f, dp = 0.f;
       for (int d = 0; d < dq; ++d) sc = fmaf(Qs[ty * ldq + d], Ks[tx * ldq + d], sc);
       for (int d = 0; d < dv; ++d) dp = fmaf(Gs[ty * ldv + d], Vs[tx * ldv + d], dp);
@@ -243,8 +251,9 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dkv_kernel(const BwdParams 
 // Rows of the streamed tile: 64, or 32 at width 128 (two CTAs on an SM instead of one).
 template <int kDim> constexpr int kStream = kDim > 64 ? 32 : 64;
 
-template <typename T, int kDim>
+template <typename T, int kDim, bool kWin>
 __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const BwdParams bp) {
+  using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
   constexpr int kN = kStream<kDim>, kCols = kN / 16, kPer = simt::OutCols<kDim>::kPer;
   constexpr int ld = kDim + 4, ldp = kN + 4;
@@ -259,8 +268,10 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const 
   const long long brow0 = (static_cast<long long>(b) * p.hq + h) * p.maxq;
   const int seen = kv_tiles_for_rows(s, r0, simt::kRows, p.mask_type, 32) * 32;
   const int end = seen < s.lk ? seen : s.lk;
-  const int ntiles = (end + kN - 1) / kN;
-  if (dbias) {
+  const KeyTiles tiles = Mask::tiles(p, s, r0, simt::kRows, kN);
+  const int ntiles = kWin ? tiles.n : (end + kN - 1) / kN;
+  auto key_of = [&](int t) { return kWin ? key_of_tile(tiles, t, kN) : t * kN; };
+  if (dbias) {   // (never with a window)
     // zeros of this CTA's d_bias rows: everything right of the visited tiles (all columns when none is visited)
     const int lane = threadIdx.x & 31;
     for (int r = threadIdx.x >> 5; r < simt::kRows && r0 + r < p.maxq; r += simt::kThreads / 32)
@@ -275,12 +286,11 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const 
     float* Ds = Vs + kN * ld;             // [32][ldp]  dS
     const T* k = static_cast<const T*>(p.k);
     const T* v = static_cast<const T*>(p.v);
-    RowBounds rb[4];
+    typename Mask::Bounds rb[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = r0 + 4 * ty + r;
-      rb[r] = row_bounds(s, i, p.mask_type, p.group);
-      if (i >= s.lq) rb[r].lim1 = 0, rb[r].lo2 = 1, rb[r].hi2 = 0;   // (a row past the end sees nothing)
+      rb[r] = i < s.lq ? Mask::bounds(p, s, i) : Mask::none();   // (a row past the end sees nothing)
     }
     float acc[4][kPer];
 #pragma unroll
@@ -290,12 +300,12 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const 
     if (ntiles > 0) {
       simt::load_rows<T, simt::kRows, kDim>(Qs, ld, static_cast<const T*>(p.q), s.q0, r0, s.lq, p.hq, h, dq);
       simt::load_rows<T, simt::kRows, kDim>(Gs, ld, static_cast<const T*>(bp.dout), s.q0, r0, s.lq, p.hq, h, dv);
-      simt::load_rows<T, kN, kDim>(Ks, ld, k, s.k0, 0, s.lk, p.hk, hk, dq);
-      simt::load_rows<T, kN, kDim>(Vs, ld, v, s.k0, 0, s.lk, p.hk, hk, dv);
+      simt::load_rows<T, kN, kDim>(Ks, ld, k, s.k0, key_of(0), s.lk, p.hk, hk, dq);
+      simt::load_rows<T, kN, kDim>(Vs, ld, v, s.k0, key_of(0), s.lk, p.hk, hk, dv);
       simt::cp_async_commit();
     }
     for (int t = 0; t < ntiles; ++t) {
-      const int c0 = t * kN;
+      const int c0 = key_of(t), c1 = key_of(t + 1);
       float bv[4][kCols];
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -320,11 +330,11 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const 
           if (dbias && i < p.maxq && j < p.maxk) dbias[(brow0 + i) * p.maxk + j] = cvt_f<T>(db);
         }
       __syncthreads();   // Ds is there; V_t is consumed
-      if (t + 1 < ntiles) simt::load_rows<T, kN, kDim>(Vs, ld, v, s.k0, c0 + kN, s.lk, p.hk, hk, dv);
+      if (t + 1 < ntiles) simt::load_rows<T, kN, kDim>(Vs, ld, v, s.k0, c1, s.lk, p.hk, hk, dv);
       const int left = (end - c0 + 3) & ~3;   // (rows of K between lk and the next multiple of four are zeros)
       simt::outer_tile<kDim>(Ds + 4 * ty * ldp, ldp, Ks, ld, left < kN ? left : kN, tx, acc);
       __syncthreads();   // K_t and Ds are consumed
-      if (t + 1 < ntiles) simt::load_rows<T, kN, kDim>(Ks, ld, k, s.k0, c0 + kN, s.lk, p.hk, hk, dq);
+      if (t + 1 < ntiles) simt::load_rows<T, kN, kDim>(Ks, ld, k, s.k0, c1, s.lk, p.hk, hk, dq);
       simt::cp_async_commit();
     }
     simt::cp_async_wait<0>();
@@ -337,8 +347,9 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const 
   asm volatile("griddepcontrol.wait;" ::: "memory");   // (the pre-pass: nothing here reads what it wrote)
 }
 
-template <typename T, int kDim>
+template <typename T, int kDim, bool kWin>
 __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const BwdParams bp) {
+  using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
   constexpr int kN = kStream<kDim>, kCols = kN / 16, kPer = simt::OutCols<kDim>::kPer;
   constexpr int ld = kDim + 4, ldp = kN + 4;
@@ -358,9 +369,9 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
     const T* q = static_cast<const T*>(p.q);
     const T* g = static_cast<const T*>(bp.dout);
     // Query tiles that see a key of this tile, one after the other: u = (query head of the group) * per_head + tile.
-    const int per_head = (s.lq + kN - 1) / kN, count = per_head * p.gqa_ratio, ktile = c0 / simt::kRows;
+    const int per_head = (s.lq + kN - 1) / kN, count = per_head * p.gqa_ratio;
     auto next = [&](int u) {
-      while (u < count && kv_tiles_for_rows(s, (u % per_head) * kN, kN, p.mask_type, simt::kRows) <= ktile) ++u;
+      while (u < count && !Mask::sees(p, s, (u % per_head) * kN, kN, c0, simt::kRows)) ++u;
       return u;
     };
     float acc_k[4][kPer], acc_v[4][kPer];
@@ -381,13 +392,12 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
       const int h = hk * p.gqa_ratio + u / per_head, r0 = (u % per_head) * kN;
       const int un = next(u + 1);
       const int hn = hk * p.gqa_ratio + un / per_head, rn = (un % per_head) * kN;
-      RowBounds rb[kCols];
+      typename Mask::Bounds rb[kCols];
       float bv[4][kCols];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         const int i = r0 + tx + 16 * c;
-        rb[c] = row_bounds(s, i, p.mask_type, p.group);
-        if (i >= s.lq) rb[c].lim1 = 0, rb[c].lo2 = 1, rb[c].hi2 = 0;
+        rb[c] = i < s.lq ? Mask::bounds(p, s, i) : Mask::none();
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = c0 + 4 * ty + r;
@@ -433,21 +443,26 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-template <typename T, int kDim>
-cudaError_t launch_simt_bwd(const BwdParams& bp, cudaStream_t stream) {
+template <typename T, int kDim, bool kWin>
+cudaError_t launch_simt_bwd_of(const BwdParams& bp, cudaStream_t stream) {
   const KParams& p = bp.f;
   constexpr int kN = kStream<kDim>;
   constexpr int tiles = 2 * (simt::kRows + kN) * (kDim + 4), part = simt::kRows * (kN + 4);
   constexpr int smem_q = 4 * (tiles + part), smem_kv = 4 * (tiles + 2 * part);
-  cudaError_t e = cudaFuncSetAttribute(hstu_simt_bwd_dq_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q);
+  cudaError_t e = cudaFuncSetAttribute(hstu_simt_bwd_dq_kernel<T, kDim, kWin>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q);
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(hstu_simt_bwd_dkv_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_kv);
+    e = cudaFuncSetAttribute(hstu_simt_bwd_dkv_kernel<T, kDim, kWin>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_kv);
   if (e != cudaSuccess) return e;
   const dim3 grid_q(static_cast<unsigned>(p.batch) * p.hq, (p.maxq + simt::kRows - 1) / simt::kRows, 1);
-  e = simt::launch(hstu_simt_bwd_dq_kernel<T, kDim>, grid_q, smem_q, stream, bp);
+  e = simt::launch(hstu_simt_bwd_dq_kernel<T, kDim, kWin>, grid_q, smem_q, stream, bp);
   if (e != cudaSuccess) return e;
   const dim3 grid_k(static_cast<unsigned>(p.batch) * p.hk, (p.maxk + simt::kRows - 1) / simt::kRows, 1);
-  return simt::launch(hstu_simt_bwd_dkv_kernel<T, kDim>, grid_k, smem_kv, stream, bp);
+  return simt::launch(hstu_simt_bwd_dkv_kernel<T, kDim, kWin>, grid_k, smem_kv, stream, bp);
+}
+
+template <typename T, int kDim>
+cudaError_t launch_simt_bwd(const BwdParams& bp, cudaStream_t stream) {
+  return bp.f.window ? launch_simt_bwd_of<T, kDim, true>(bp, stream) : launch_simt_bwd_of<T, kDim, false>(bp, stream);
 }
 
 // The register-tiled kernels wherever their loads are possible.  (16 sequences of 50-500 rows, 2 heads of 64, fp32, forward
@@ -471,18 +486,18 @@ cudaError_t launch_bwd_t(const BwdParams& bp, int dtype, cudaStream_t stream) {
   const size_t tile = static_cast<size_t>(BT) * (p.dqk + 1) + static_cast<size_t>(BT) * (p.dv + 1);
   const size_t smem_q = sizeof(float) * (2 * tile + BT * BT);
   const size_t smem_kv = sizeof(float) * (2 * tile + 2 * BT * BT);
-  cudaError_t e = cudaFuncSetAttribute(hstu_bwd_dq_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem_q));
+  auto kern_q = p.window ? hstu_bwd_dq_kernel<T, true> : hstu_bwd_dq_kernel<T, false>;
+  auto kern_kv = p.window ? hstu_bwd_dkv_kernel<T, true> : hstu_bwd_dkv_kernel<T, false>;
+  cudaError_t e = cudaFuncSetAttribute(kern_q, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_q));
   if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(hstu_bwd_dkv_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             static_cast<int>(smem_kv));
+    e = cudaFuncSetAttribute(kern_kv, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_kv));
   if (e != cudaSuccess) return e;
   dim3 grid_q(static_cast<unsigned>(p.batch) * p.hq, (p.maxq + BT - 1) / BT, 1);
-  hstu_bwd_dq_kernel<T><<<grid_q, BTHREADS, smem_q, stream>>>(bp);
+  kern_q<<<grid_q, BTHREADS, smem_q, stream>>>(bp);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   dim3 grid_k(static_cast<unsigned>(p.batch) * p.hk, (p.maxk + BT - 1) / BT, 1);
-  hstu_bwd_dkv_kernel<T><<<grid_k, BTHREADS, smem_kv, stream>>>(bp);
+  kern_kv<<<grid_k, BTHREADS, smem_kv, stream>>>(bp);
   return cudaGetLastError();
 }
 

@@ -116,16 +116,15 @@ struct BwdWaiter {
 // The steps of one CTA, in the order every role walks them.  f(stream_head, stream_row0, query_head):
 //   dQ pass:    stream = K/V tiles of kv head hk, rows stream_row0 = j * 128 (keys);   query_head = h
 //   dK/dV pass: stream = Q/dO tiles of query head h, rows stream_row0 = r0 (queries);  query_head = h
-template <bool kDKV, typename F>
+template <bool kDKV, bool kWin, typename F>
 __device__ __forceinline__ void for_each_step(const KParams& p, const SeqInfo& s, int tile0, int head, F&& f) {
   if (!kDKV) {
-    const int n = kv_tiles_for_rows(s, tile0, kTileM, p.mask_type, kTileN);
-    for (int j = 0; j < n; ++j) f(head / p.gqa_ratio, j * kTileN, head);
+    const KeyTiles t = MaskOf<kWin>::tiles(p, s, tile0, kTileM, kTileN);
+    for (int j = 0; j < t.n; ++j) f(head / p.gqa_ratio, kWin ? key_of_tile(t, j, kTileN) : j * kTileN, head);
   } else {
-    const int ktile = tile0 / kTileN;
     for (int hh = 0; hh < p.gqa_ratio; ++hh)
       for (int r0 = 0; r0 < s.lq; r0 += kTileM)
-        if (kv_tiles_for_rows(s, r0, kTileM, p.mask_type, kTileN) > ktile) f(head * p.gqa_ratio + hh, r0, head * p.gqa_ratio + hh);
+        if (MaskOf<kWin>::sees(p, s, r0, kTileM, tile0, kTileN)) f(head * p.gqa_ratio + hh, r0, head * p.gqa_ratio + hh);
   }
 }
 
@@ -135,6 +134,10 @@ __device__ __forceinline__ uint32_t low_bits(int n) {  // n lowest bits set, n c
 }
 __device__ __forceinline__ uint32_t visible_bits(const RowBounds& rb, int j0) {
   return low_bits(rb.lim1 - j0) | (low_bits(rb.hi2 + 1 - j0) & ~low_bits(rb.lo2 - j0));
+}
+__device__ __forceinline__ uint32_t visible_bits(const WinBounds& rb, int j0) {
+  return low_bits(rb.lim1 - j0) | (low_bits(rb.hi2 + 1 - j0) & ~low_bits(rb.lo2 - j0)) |
+         (low_bits(rb.hi3 + 1 - j0) & ~low_bits(rb.lo3 - j0));
 }
 
 // Two neighbouring elements, the part that needs the scores only (vector_score.h:175-197), on the packed f32x2 pipe:
@@ -182,7 +185,7 @@ static_assert(sizeof(BwdBars) <= 512, "barrier block too large");
 
 // kStaged (a bias that TMA can tile): a kernel of its own - the same code merely present in the bias-free kernel cost that
 // one 4 %.
-template <int D, typename T, bool kDKV, bool kStaged>
+template <int D, typename T, bool kDKV, bool kStaged, bool kWin>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1,
                    const __grid_constant__ CUtensorMap tm_a2, const __grid_constant__ CUtensorMap tm_b1,
@@ -329,7 +332,7 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
           if (hf < halves1) ptx::tma_load_3d(sm_a + hf * kHalfBytes, &tm_a1, afull, hf * 64, a_head, static_cast<int>(a_row));
           if (hf < halves2) ptx::tma_load_3d(sm_a + kTileBytes + hf * kHalfBytes, &tm_a2, afull, hf * 64, a_head, static_cast<int>(a_row));
         }
-        for_each_step<kDKV>(p, s, tile0, head, [&](int sh, int srow0, int qh) {
+        for_each_step<kDKV, kWin>(p, s, tile0, head, [&](int sh, int srow0, int qh) {
           const int row = static_cast<int>(b_row0) + srow0;
           const uint32_t s1 = cnt % kRing1, s2 = cnt % kRing2;
           const uint32_t full1 = ptx::smem_u32(&bars->b1_full[s1]), full2 = ptx::smem_u32(&bars->b2_full[s2]);
@@ -494,7 +497,7 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
         }
       };
       w.wait(ptx::smem_u32(&bars->a_full), tiles_done & 1u);
-      for_each_step<kDKV>(p, s, tile0, head, [&](int, int srow0, int) {
+      for_each_step<kDKV, kWin>(p, s, tile0, head, [&](int, int srow0, int) {
         // Products of one thread run in order, so one that overwrites a buffer may be issued right behind the one that read
         // it.  dK/dV pass: dV of the last step (reads P in T1), the scores of this one (T1), dK of the last (dS in T2), dP
         // of this one (T2) - the scores, on which most of the element-wise stage depends, do not wait for dS.  dQ pass: the
@@ -556,7 +559,7 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int mine = tile0 + row;                 // this thread's query row (dQ pass) / key (dK/dV pass)
     const bool mine_ok = mine < len;
-    const RowBounds rb_mine = row_bounds(s, (mine_ok || kDKV) ? mine : s.lq - 1, p.mask_type, p.group);  // dQ pass
+    const typename MaskOf<kWin>::Bounds rb_mine = MaskOf<kWin>::bounds(p, s, (mine_ok || kDKV) ? mine : s.lq - 1);  // dQ pass
     T* dbias = static_cast<T*>(bp.dbias);
     const bool dbias_vec = dbias && (p.maxk % 8 == 0) && (reinterpret_cast<uintptr_t>(bp.dbias) & 15u) == 0;
     const bool bias_vec = p.bias && (p.maxk % 8 == 0) && (p.bias_bstride % 8 == 0) &&
@@ -567,15 +570,19 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
     // own position on (the transpose of row_bounds(); no mask: every query).
     const bool grouped = p.mask_type == HSTU_MASK_TRIL && s.tgt > 0 && p.group > 0;
     const int hq_end = grouped ? s.lq - s.tgt : s.lq;
-    int c_lo = 0, ctx_hi = 0, t_lo = 0, t_hi = 0;
+    int c_lo = 0, c_hi = hq_end, ctx_hi = 0, t_lo = 0, t_hi = 0;
     if (kDKV && p.mask_type == HSTU_MASK_TRIL) {
       const int hist = s.lk - s.tgt;
       c_lo = mine - (s.lk - s.lq);
       if (s.ctx > 0 && mine < hist) ctx_hi = s.ctx < hq_end ? s.ctx : hq_end;
+      // with a window: the `window` rows from the key's own on, and every target if the window still holds the key at the
+      // end of the history; a sink is seen by all of them
+      const bool lasting = !kWin || mine < p.sink;
+      if (!lasting && c_hi - c_lo > p.window) c_hi = c_lo + p.window;
       if (grouped) {
         if (mine < hist) {
           t_lo = hq_end;
-          t_hi = s.lq;
+          t_hi = lasting || hist - mine < p.window ? s.lq : hq_end;
         } else {
           const int tj = mine - hist;
           const int gend = (tj / p.group + 1) * p.group;
@@ -591,10 +598,10 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
       ptx::fence_proxy_async();
       ptx::mbar_arrive(ptx::smem_u32(&bars->bias_free));
     };
-    for_each_step<kDKV>(p, s, tile0, head, [&](int, int srow0, int qh) {
+    for_each_step<kDKV, kWin>(p, s, tile0, head, [&](int, int srow0, int qh) {
       // rows of the score tile are queries, columns keys - in the dK/dV pass the tile is held transposed
       const int q_first = kDKV ? srow0 : tile0, k_first = kDKV ? tile0 : srow0;
-      const bool full = tile_is_full(s, q_first, kTileM, k_first, kTileN, p.mask_type, p.group) &&
+      const bool full = MaskOf<kWin>::full(p, s, q_first, kTileM, k_first, kTileN) &&
                         (!kDKV || q_first + kTileM <= s.lq);
       const long long bias_bh = static_cast<long long>(b) * p.bias_bstride + static_cast<long long>(qh) * p.maxq * p.maxk;
       const uint32_t col_t1 = tmem + lane_base + ((cnt & 1u) ? kColT1b : kColT1) + 64 * grp;
@@ -611,7 +618,7 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
         } else if (mine >= s.lk) {
           bits[ch] = 0u;
         } else {
-          bits[ch] = (low_bits(hq_end - i0) & ~low_bits(c_lo - i0)) | low_bits(ctx_hi - i0) |
+          bits[ch] = (low_bits((kWin ? c_hi : hq_end) - i0) & ~low_bits(c_lo - i0)) | low_bits(ctx_hi - i0) |
                      (low_bits(t_hi - i0) & ~low_bits(t_lo - i0));
         }
       }
@@ -875,7 +882,9 @@ cudaError_t launch_bwd_tc_t(const BwdParams& bp, int dtype, int num_sms, cudaStr
       cfg.numAttrs = (!kDKV || overlap) ? 1 : 0;
       return cudaLaunchKernelEx(&cfg, kern, bp, a1, a2, b1, b2, mb);
     };
-    return bias_staged ? go(hstu_bwd_tc_kernel<D, T, kDKV, true>, BwdRings<D, true, kDKV>::kSmem) : go(hstu_bwd_tc_kernel<D, T, kDKV, false>, BwdRings<D, false, kDKV>::kSmem);
+    if (p.window) return go(hstu_bwd_tc_kernel<D, T, kDKV, false, true>, BwdRings<D, false, kDKV>::kSmem);
+    return bias_staged ? go(hstu_bwd_tc_kernel<D, T, kDKV, true, false>, BwdRings<D, true, kDKV>::kSmem)
+                       : go(hstu_bwd_tc_kernel<D, T, kDKV, false, false>, BwdRings<D, false, kDKV>::kSmem);
   };
   cudaError_t e = cudaSuccess;
   overlap = p.total_q > 0;   // (a dQ pass is launched in front of the dK/dV pass)

@@ -83,6 +83,8 @@ struct KParams {
   int bwd_all_q_tiles;
   int bwd_by_steps;   // order the lists by the tiles' step counts (few tiles per CTA) instead of sequence by sequence
   int fwd_by_steps;   // the same for the forward's work list: all sequences' last q-pairs first, then the ones before
+  // hstu_window and hstu_paged_8bit (0 otherwise): keys a row sees up to its own position, and the first keys that stay visible
+  int window, sink;
 };
 
 // Backward call: the forward's parameters plus the gradient tensors.
@@ -295,6 +297,128 @@ HSTU_HD bool tile_is_full(const SeqInfo& s, int r0, int rows, int c0, int bn, in
   }
   return c0 + bn <= lim;
 }
+
+// ------------------------------------------------------------------------------------------------ sliding window
+// The mask of hstu_window: row i at position p = i + (len_k - len_q) sees the keys j <= p with p - j < window or j < sink.
+// With targets and groups a target row counts its window from the end of the history (as if p were len_k - num_target): it
+// sees the history keys that are left, and the targets of its own group up to itself.  num_context is not part of it.
+// Three intervals per row:  allowed(j)  <=>  j < lim1  ||  (lo2 <= j && j <= hi2)  ||  (lo3 <= j && j <= hi3).
+struct WinBounds {
+  int lim1, lo2, hi2, lo3, hi3;
+};
+
+// The position a row counts its window from.
+HSTU_HD int win_anchor(const SeqInfo& s, int i, int group) {
+  return s.tgt > 0 && group > 0 && i >= s.lq - s.tgt ? s.lk - s.tgt : i + (s.lk - s.lq);
+}
+
+HSTU_HD WinBounds win_bounds(const SeqInfo& s, int i, int group, int window, int sink) {
+  WinBounds r;
+  const int at = win_anchor(s, i, group);
+  const bool target = s.tgt > 0 && group > 0 && i >= s.lq - s.tgt;
+  int end = target ? at : at + 1;   // one past the last key the window holds
+  if (end > s.lk) end = s.lk;
+  if (end < 0) end = 0;
+  r.lim1 = sink < end ? sink : end;
+  r.lo2 = at - window + 1;
+  r.hi2 = end - 1;
+  r.lo3 = 1;
+  r.hi3 = 0;
+  if (target) {
+    const int ti = i - (s.lq - s.tgt);
+    r.lo3 = at + (ti / group) * group;
+    r.hi3 = at + ti;
+    if (r.hi3 > s.lk - 1) r.hi3 = s.lk - 1;
+  }
+  return r;
+}
+
+HSTU_HD bool allowed(const WinBounds& r, int j) {
+  return j < r.lim1 || (j >= r.lo2 && j <= r.hi2) || (j >= r.lo3 && j <= r.hi3);
+}
+
+// The K tiles of width bn a q-tile of rows [r0, r0 + rows) visits: the first n_first start at keys 0, bn, 2 bn .. (the sinks),
+// the others at start2, start2 + bn, .. (start2 a multiple of bn), n in all.  Without a window n_first == n.
+struct KeyTiles {
+  int n_first, start2, n;
+};
+HSTU_HD int key_of_tile(const KeyTiles& t, int j, int bn) {
+  return j < t.n_first ? j * bn : t.start2 + (j - t.n_first) * bn;
+}
+// Keys any row of the q-tile sees: [0, first) and [lo, end); nothing when end == 0.
+struct KeySpan {
+  int first, lo, end;
+};
+HSTU_HD KeySpan win_span(const SeqInfo& s, int r0, int rows, int group, int window, int sink) {
+  KeySpan k = {0, 0, 0};
+  if (r0 >= s.lq || s.lk <= 0) return k;
+  int r1 = r0 + rows - 1;
+  if (r1 > s.lq - 1) r1 = s.lq - 1;
+  int end = r1 + (s.lk - s.lq) + 1;   // (a target row's own key: the same formula)
+  if (end > s.lk) end = s.lk;
+  if (end <= 0) return k;
+  k.end = end;
+  k.first = sink < end ? sink : end;
+  k.lo = win_anchor(s, r0, group) - window + 1;   // (anchors grow with the row)
+  if (k.lo < 0) k.lo = 0;
+  return k;
+}
+HSTU_HD KeyTiles win_tiles(const SeqInfo& s, int r0, int rows, int group, int window, int sink, int bn) {
+  const KeySpan k = win_span(s, r0, rows, group, window, sink);
+  KeyTiles t;
+  t.n_first = (k.first + bn - 1) / bn;
+  t.start2 = k.lo / bn * bn;
+  if (t.n_first * bn >= t.start2) {   // no gap
+    t.n = t.n_first = (k.end + bn - 1) / bn;
+    t.start2 = t.n * bn;
+  } else {
+    t.n = t.n_first + (k.end - t.start2 + bn - 1) / bn;
+  }
+  return t;
+}
+// Whether a row of the q-tile may see a key of [c0, c0 + bn) (never false when one does).
+HSTU_HD bool win_sees(const SeqInfo& s, int r0, int rows, int group, int window, int sink, int c0, int bn) {
+  const KeySpan k = win_span(s, r0, rows, group, window, sink);
+  return c0 < k.end && (c0 < k.first || c0 + bn > k.lo);
+}
+// tile_is_full's question.
+HSTU_HD bool win_tile_is_full(const SeqInfo& s, int r0, int rows, int c0, int bn, int group, int window, int sink) {
+  int r1 = r0 + rows - 1;
+  if (r1 > s.lq - 1) r1 = s.lq - 1;
+  if (!tile_is_full(s, r0, rows, c0, bn, HSTU_MASK_TRIL, group)) return false;
+  return c0 > win_anchor(s, r1, group) - window || c0 + bn <= sink;
+}
+
+// The mask of a kernel instantiation: the composite mask (kWin = false) or the windowed one.
+template <bool kWin> struct MaskOf {
+  using Bounds = RowBounds;
+  static HSTU_HD Bounds bounds(const KParams& p, const SeqInfo& s, int i) { return row_bounds(s, i, p.mask_type, p.group); }
+  static HSTU_HD Bounds none() { return {0, 1, 0}; }
+  static HSTU_HD KeyTiles tiles(const KParams& p, const SeqInfo& s, int r0, int rows, int bn) {
+    const int n = kv_tiles_for_rows(s, r0, rows, p.mask_type, bn);
+    return {n, n * bn, n};
+  }
+  static HSTU_HD bool sees(const KParams& p, const SeqInfo& s, int r0, int rows, int c0, int bn) {
+    return kv_tiles_for_rows(s, r0, rows, p.mask_type, bn) > c0 / bn;
+  }
+  static HSTU_HD bool full(const KParams& p, const SeqInfo& s, int r0, int rows, int c0, int bn) {
+    return tile_is_full(s, r0, rows, c0, bn, p.mask_type, p.group);
+  }
+};
+template <> struct MaskOf<true> {
+  using Bounds = WinBounds;
+  static HSTU_HD Bounds bounds(const KParams& p, const SeqInfo& s, int i) { return win_bounds(s, i, p.group, p.window, p.sink); }
+  static HSTU_HD Bounds none() { return {0, 1, 0, 1, 0}; }
+  static HSTU_HD KeyTiles tiles(const KParams& p, const SeqInfo& s, int r0, int rows, int bn) {
+    return win_tiles(s, r0, rows, p.group, p.window, p.sink, bn);
+  }
+  static HSTU_HD bool sees(const KParams& p, const SeqInfo& s, int r0, int rows, int c0, int bn) {
+    return win_sees(s, r0, rows, p.group, p.window, p.sink, c0, bn);
+  }
+  static HSTU_HD bool full(const KParams& p, const SeqInfo& s, int r0, int rows, int c0, int bn) {
+    return win_tile_is_full(s, r0, rows, c0, bn, p.group, p.window, p.sink);
+  }
+};
 
 // Number of work items (q-pairs) of a sequence.
 HSTU_HD int pairs_of(int lq) { return (lq + kPairM - 1) / kPairM; }

@@ -34,8 +34,9 @@ constexpr int kFwdKeys = 64;   // keys per tile of the register-tiled kernel
 
 // See hstu_simt.cuh for the tile shape and what bounds it.  K_t is read by the scores only and V_t by the output only,
 // so each is fetched again while the other's products run.
-template <typename T, int kDim>
+template <typename T, int kDim, bool kWin>
 __global__ void __launch_bounds__(simt::kThreads) hstu_simt_fwd_kernel(const KParams p) {
+  using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
   constexpr int kCols = kFwdKeys / 16;
   constexpr int kPer = simt::OutCols<kDim>::kPer;
@@ -56,29 +57,30 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_fwd_kernel(const KPa
     const T* bias = static_cast<const T*>(p.bias);
     const T* cmask = static_cast<const T*>(p.mask);
     const bool alpha_first = (p.flags & HSTU_FLAG_ALPHA_BEFORE_BIAS) != 0;
-    RowBounds rb[4];
+    typename Mask::Bounds rb[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = r0 + 4 * ty + r;
-      rb[r] = row_bounds(s, i, p.mask_type, p.group);
-      if (i >= s.lq) rb[r].lim1 = 0, rb[r].lo2 = 1, rb[r].hi2 = 0;   // (a row past the end sees nothing)
+      rb[r] = i < s.lq ? Mask::bounds(p, s, i) : Mask::none();   // (a row past the end sees nothing)
     }
     // keys any row of the q-tile sees, rounded up to the q-tile's height
     const int seen = kv_tiles_for_rows(s, r0, simt::kRows, p.mask_type, 32) * 32;
     const int end = seen < s.lk ? seen : s.lk;
-    const int ntiles = (end + kFwdKeys - 1) / kFwdKeys;
+    const KeyTiles tiles = Mask::tiles(p, s, r0, simt::kRows, kFwdKeys);
+    const int ntiles = kWin ? tiles.n : (end + kFwdKeys - 1) / kFwdKeys;
+    auto key_of = [&](int t) { return kWin ? key_of_tile(tiles, t, kFwdKeys) : t * kFwdKeys; };
     float acc[4][kPer];
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int c = 0; c < kPer; ++c) acc[r][c] = 0.f;
     simt::load_rows<T, simt::kRows, kDim>(Qs, ldq, static_cast<const T*>(p.q), s.q0, r0, s.lq, p.hq, h, dq);
-    if (ntiles > 0) simt::load_rows<T, kFwdKeys, kDim>(Ks, ldq, k, s.k0, 0, s.lk, p.hk, hk, dq);
+    if (ntiles > 0) simt::load_rows<T, kFwdKeys, kDim>(Ks, ldq, k, s.k0, key_of(0), s.lk, p.hk, hk, dq);
     simt::cp_async_commit();
-    if (ntiles > 0) simt::load_rows<T, kFwdKeys, kDim>(Vs, kDim, v, s.k0, 0, s.lk, p.hk, hk, dv);
+    if (ntiles > 0) simt::load_rows<T, kFwdKeys, kDim>(Vs, kDim, v, s.k0, key_of(0), s.lk, p.hk, hk, dv);
     simt::cp_async_commit();
     for (int t = 0; t < ntiles; ++t) {
-      const int c0 = t * kFwdKeys;
+      const int c0 = key_of(t), c1 = key_of(t + 1);
       float bv[4][kCols];
       if (bias) {   // (in flight while the scores are computed)
 #pragma unroll
@@ -113,12 +115,12 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_fwd_kernel(const KPa
         }
       simt::cp_async_wait<0>();   // V_t
       __syncthreads();            // Ps and V_t are there; K_t is consumed
-      if (t + 1 < ntiles) simt::load_rows<T, kFwdKeys, kDim>(Ks, ldq, k, s.k0, c0 + kFwdKeys, s.lk, p.hk, hk, dq);
+      if (t + 1 < ntiles) simt::load_rows<T, kFwdKeys, kDim>(Ks, ldq, k, s.k0, c1, s.lk, p.hk, hk, dq);
       simt::cp_async_commit();
       const int left = (end - c0 + 3) & ~3;   // (rows of V between lk and the next multiple of four are zeros)
       simt::outer_tile<kDim>(Ps + 4 * ty * ldp, ldp, Vs, kDim, left < kFwdKeys ? left : kFwdKeys, tx, acc);
       __syncthreads();            // V_t and Ps are consumed
-      if (t + 1 < ntiles) simt::load_rows<T, kFwdKeys, kDim>(Vs, kDim, v, s.k0, c0 + kFwdKeys, s.lk, p.hk, hk, dv);
+      if (t + 1 < ntiles) simt::load_rows<T, kFwdKeys, kDim>(Vs, kDim, v, s.k0, c1, s.lk, p.hk, hk, dv);
       simt::cp_async_commit();
     }
     simt::cp_async_wait<0>();
@@ -133,8 +135,9 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_fwd_kernel(const KPa
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-template <typename T>
+template <typename T, bool kWin>
 __global__ void __launch_bounds__(GTHREADS) hstu_generic_kernel(const KParams p) {
+  using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
   const int bh = blockIdx.x;
   const int b = bh / p.hq;
@@ -167,9 +170,9 @@ __global__ void __launch_bounds__(GTHREADS) hstu_generic_kernel(const KParams p)
     Qs[r * ldq + d] = row < s.lq ? to_f<T>(q[((s.q0 + row) * p.hq + h) * dq + d]) : 0.f;
   }
 
-  RowBounds rb[GROWS];
+  typename Mask::Bounds rb[GROWS];
 #pragma unroll
-  for (int r = 0; r < GROWS; ++r) rb[r] = row_bounds(s, r0 + ty * GROWS + r, p.mask_type, p.group);
+  for (int r = 0; r < GROWS; ++r) rb[r] = Mask::bounds(p, s, r0 + ty * GROWS + r);
 
   float acc[GROWS][GMAXC];
 #pragma unroll
@@ -177,12 +180,13 @@ __global__ void __launch_bounds__(GTHREADS) hstu_generic_kernel(const KParams p)
 #pragma unroll
     for (int c = 0; c < GMAXC; ++c) acc[r][c] = 0.f;
 
-  const int ntiles = kv_tiles_for_rows(s, r0, GM, p.mask_type, GN);
+  const KeyTiles tiles = Mask::tiles(p, s, r0, GM, GN);
+  const int ntiles = tiles.n;
   const int ncol = (dv + 31) >> 5;
   const bool alpha_first = (p.flags & HSTU_FLAG_ALPHA_BEFORE_BIAS) != 0;
 
   for (int t = 0; t < ntiles; ++t) {
-    const int c0 = t * GN;
+    const int c0 = kWin ? key_of_tile(tiles, t, GN) : t * GN;
     __syncthreads();  // previous tile's Ks/Vs/Ps fully consumed (also orders the Qs fill on t == 0)
     for (int idx = tid; idx < GN * dq; idx += GTHREADS) {
       const int r = idx / dq, d = idx - r * dq;
@@ -266,13 +270,18 @@ size_t generic_smem_bytes(const KParams& p) {
   return sizeof(float) * (static_cast<size_t>(GM + GN) * (p.dqk + 1) + static_cast<size_t>(GN) * p.dv + GM * GN);
 }
 
-template <typename T, int kDim>
-cudaError_t launch_simt(const KParams& p, cudaStream_t stream) {
+template <typename T, int kDim, bool kWin>
+cudaError_t launch_simt_of(const KParams& p, cudaStream_t stream) {
   constexpr int smem = 4 * (simt::kRows * (kDim + 4) + kFwdKeys * (kDim + 4) + kFwdKeys * kDim + simt::kRows * (kFwdKeys + 4));
-  cudaError_t e = cudaFuncSetAttribute(hstu_simt_fwd_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = cudaFuncSetAttribute(hstu_simt_fwd_kernel<T, kDim, kWin>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>(p.batch) * p.hq, (p.maxq + simt::kRows - 1) / simt::kRows, 1);
-  return simt::launch(hstu_simt_fwd_kernel<T, kDim>, grid, smem, stream, p);
+  return simt::launch(hstu_simt_fwd_kernel<T, kDim, kWin>, grid, smem, stream, p);
+}
+
+template <typename T, int kDim>
+cudaError_t launch_simt(const KParams& p, cudaStream_t stream) {
+  return p.window ? launch_simt_of<T, kDim, true>(p, stream) : launch_simt_of<T, kDim, false>(p, stream);
 }
 
 // The register-tiled kernel wherever its loads are possible.  (4 sequences of at most 128 rows, 2 heads of 32, fp32: a call
@@ -296,11 +305,11 @@ cudaError_t launch_t(const KParams& p, int dtype, cudaStream_t stream) {
     }
   }
   const size_t smem = generic_smem_bytes(p);
-  cudaError_t e = cudaFuncSetAttribute(hstu_generic_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
+  auto kern = p.window ? hstu_generic_kernel<T, true> : hstu_generic_kernel<T, false>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   dim3 grid(static_cast<unsigned>(p.batch) * p.hq, (p.maxq + GM - 1) / GM, 1);
-  hstu_generic_kernel<T><<<grid, GTHREADS, smem, stream>>>(p);
+  kern<<<grid, GTHREADS, smem, stream>>>(p);
   return cudaGetLastError();
 }
 

@@ -63,9 +63,18 @@ struct ShTile {
   // The keys of a sequence are one segment, or - hstu_paged - two: the cached keys [0, split) and the targets
   // [split, lk).  A tile lies in one segment: tiles j < n_first start at key 64 j, the others at split + 64 (j - n_first).
   int split, n_first;
+  // With a window (kWin) the tiles in front of the split are those of the sinks, j < n_sink, and those of the window, which
+  // start at key start2 + 64 (j - n_sink); without one n_sink == n_first.
+  int n_sink, start2;
   int pages;            // hstu_paged: pages of the sequence,
   long long first_slot; //   and the first of them in page_ids
 };
+
+// The first key of tile j, and the end of the segment it lies in.
+template <bool kWin> __device__ __forceinline__ int first_key(int j, int n_sink, int start2, int n_first, int split) {
+  if (kWin && j >= n_sink && j < n_first) return start2 + (j - n_sink) * kShKeys;
+  return j < n_first ? j * kShKeys : split + (j - n_first) * kShKeys;
+}
 
 struct ShBars {
   uint64_t q_full, q_free, s_full, p_full, o_full, o_free, done;
@@ -79,8 +88,8 @@ struct ShBars {
 static_assert(sizeof(ShBars) <= 1024, "barrier block too large");
 
 // This thread's 64 scores -> P, in place.  kMasked: the mask or the segment's end (`left` keys away) cuts through the tile.
-template <typename T, bool kBias, bool kMasked>
-__device__ __forceinline__ void short_p(uint32_t t_s, uint32_t bias_row, uint32_t bias_swz, const RowBounds& rb, int c0,
+template <typename T, bool kBias, bool kMasked, typename Bounds>
+__device__ __forceinline__ void short_p(uint32_t t_s, uint32_t bias_row, uint32_t bias_swz, const Bounds& rb, int c0,
                                         int left, float c_in, float scale) {
 #pragma unroll
   for (int ch = 0; ch < 2; ++ch) {
@@ -114,12 +123,13 @@ __device__ __forceinline__ void short_p(uint32_t t_s, uint32_t bias_row, uint32_
   }
 }
 
-template <int D, typename T, bool kBias>
+template <int D, typename T, bool kBias, bool kWin>
 __global__ void __launch_bounds__(kShThreads, ShCfg<D, kBias>::kPerSm)
 hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_bias,
                   const __grid_constant__ CUtensorMap tm_cache) {
   using C = ShCfg<D, kBias>;
+  using Mask = MaskOf<kWin>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = ptx::smem_u32(smem_raw);
   const uint32_t sm_q = (raw + 1023u) & ~1023u;
@@ -256,7 +266,16 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
         const int seen = kv_tiles_for_rows(t.s, t.r0, kTileM, p.mask_type, 1);   // keys [0, seen) are visited
         t.split = p.paged_split ? t.s.lk - t.s.tgt : t.s.lk;
         t.n_first = ((seen < t.split ? seen : t.split) + kShKeys - 1) / kShKeys;
-        t.n = t.n_first + (seen > t.split ? (seen - t.split + kShKeys - 1) / kShKeys : 0);
+        const int n_rest = seen > t.split ? (seen - t.split + kShKeys - 1) / kShKeys : 0;
+        if (kWin) {
+          const KeySpan k = win_span(t.s, t.r0, kTileM, p.group, p.window, p.sink);
+          const int end = k.end < t.split ? k.end : t.split;   // of the keys in front of the split
+          t.n_sink = (k.first + kShKeys - 1) / kShKeys;
+          t.start2 = k.lo / kShKeys * kShKeys;
+          if (t.n_sink * kShKeys >= t.start2) t.n_sink = t.n_first;   // no gap
+          else t.n_first = t.n_sink + (end > t.start2 ? (end - t.start2 + kShKeys - 1) / kShKeys : 0);
+        }
+        t.n = t.n_first + n_rest;
         t.valid = 1;
         return t;
       };
@@ -291,16 +310,17 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
           long long pid = 0;
           for (int j = 0; j < t.n; ++j) {
             const bool from_cache = p.paged_split && j < t.n_first;
-            int row = static_cast<int>(t.s.k0) + j * kShKeys, in_page = 0;
+            const int key = first_key<kWin>(j, t.n_sink, t.start2, t.n_first, t.split);
+            int row = static_cast<int>(t.s.k0) + key, in_page = 0;
             if (from_cache) {
-              in_page = (j * kShKeys) % p.page_size;
+              in_page = key % p.page_size;
               if (in_page == 0) {
                 pid = pid_next;   // (an id outside the cache reads as zeros: the coordinate lies past the tensor)
                 if (pid < 0 || pid >= p.num_pages) pid = p.num_pages;
                 pid_next = page(t, (j * kShKeys) / p.page_size + 1);
               }
             } else if (p.paged_split) {
-              row = static_cast<int>(t.s.q0) + t.s.lq - t.s.tgt + (j - t.n_first) * kShKeys;
+              row = static_cast<int>(t.s.q0) + t.s.lq - t.s.tgt + (key - t.split);
             }
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
@@ -361,6 +381,7 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
         if (w.aborted()) break;
         const int n = bars->item[slot].n, valid = bars->item[slot].valid, lk = bars->item[slot].s.lk;
         const int split = bars->item[slot].split, n_first = bars->item[slot].n_first;
+        const int n_sink = bars->item[slot].n_sink, start2 = bars->item[slot].start2;
         ptx::mbar_arrive(ptx::smem_u32(&bars->item_free[slot]));
         if (!valid) break;
         if (n == 0) continue;
@@ -403,7 +424,7 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
           ptx::tc_fence_after();
           const uint64_t vbase = kDescV | static_cast<uint64_t>((sm_ring + st * C::kKvBytes) >> 4);
           // (16-key products wholly behind the segment's end are left out)
-          const int keys = j < n_first ? split - j * kShKeys : lk - split - (j - n_first) * kShKeys;
+          const int keys = (j < n_first ? split : lk) - first_key<kWin>(j, n_sink, start2, n_first, split);
 #pragma unroll
           for (int ks = 0; ks < kShKeys / 16; ++ks)
             ptx::mma_ts_if(ks * 16 < keys ? 1u : 0u, tmem + kShColO, tmem + ks * 8,
@@ -443,15 +464,17 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
       if (stopped()) break;
       const ShTile& in = bars->item[slot];
       const int valid = in.valid, n = in.n, r0 = in.r0, lq = in.s.lq, lk = in.s.lk;
-      const int split = in.split, n_first = in.n_first;
+      const int split = in.split, n_first = in.n_first, n_sink = in.n_sink, start2 = in.start2;
       const int i_row = r0 + row;
       const bool row_ok = i_row < lq;
-      RowBounds rb = {0, 1, 0};
+      typename Mask::Bounds rb = Mask::none();
+      SeqInfo seq = {};   // (kWin)
       T* orow = nullptr;
       int full_end = 0;   // tiles that end at or before this key are visible to every row of the Q tile (tile_is_full's rule)
       if (valid) {
         const SeqInfo s = in.s;
-        if (lq > 0) rb = row_bounds(s, row_ok ? i_row : lq - 1, p.mask_type, p.group);
+        if (lq > 0) rb = Mask::bounds(p, s, row_ok ? i_row : lq - 1);
+        if (kWin) seq = s;
         orow = static_cast<T*>(p.out) + ((s.q0 + i_row) * p.hq + in.h) * p.dv;
         full_end = lk;
         if (p.mask_type == HSTU_MASK_TRIL) {
@@ -465,7 +488,7 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
       if (!valid) break;
       bool ok = true;
       for (int j = 0; j < n; ++j) {
-        const int c0 = j < n_first ? j * kShKeys : split + (j - n_first) * kShKeys;
+        const int c0 = first_key<kWin>(j, n_sink, start2, n_first, split);
         const int rem = (j < n_first ? split : lk) - c0;
         const uint32_t bb = bias_pos % C::kBiasBufs;
         if (kBias) w.wait(ptx::smem_u32(&bars->bias_full[bb]), (bias_pos / C::kBiasBufs) & 1u);
@@ -487,7 +510,7 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
         ++s_uses;
         ptx::tc_fence_after();
         const uint32_t brow = sm_bias + bb * C::kBiasBytes + row * 128, bswz = row & 7;
-        if (c0 + kShKeys <= full_end && rem >= kShKeys)
+        if ((kWin ? Mask::full(p, seq, r0, kTileM, c0, kShKeys) : c0 + kShKeys <= full_end) && rem >= kShKeys)
           short_p<T, kBias, false>(t_s, brow, bswz, rb, c0, rem, c_in, p.scale);
         else
           short_p<T, kBias, true>(t_s, brow, bswz, rb, c0, rem, c_in, p.scale);
@@ -542,11 +565,11 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
   }
 }
 
-template <int D, typename T, bool kBias>
+template <int D, typename T, bool kBias, bool kWin>
 cudaError_t launch_inst(const KParams& p, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                         const CUtensorMap& mb, const CUtensorMap& mc, int num_sms, cudaStream_t stream) {
   using C = ShCfg<D, kBias>;
-  auto kern = hstu_short_kernel<D, T, kBias>;
+  auto kern = hstu_short_kernel<D, T, kBias, kWin>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes);
   if (e != cudaSuccess) return e;
   const long long want = 2 * p.item_capacity, most = static_cast<long long>(num_sms) * C::kPerSm;
@@ -602,6 +625,7 @@ static bool short_rule(const KParams& p, long long mean_k, bool in_place) {
 }
 bool short_preferred(const KParams& p) {
   if (p.paged_split) return true;                     // (decided by short_paged_split)
+  if (p.window) return true;                          // (the only tensor-core kernel that knows windows)
   if (p.batch <= 0 || p.paged_direct) return false;   // (cache pages beside staging tensors: hstu_tc.cu)
   return short_rule(p, p.total_k / p.batch, false);
 }
@@ -631,8 +655,9 @@ cudaError_t launch_short(const KParams& p, int dtype, const CUtensorMap& mq, con
       !make_kv_tile_map(&mc, p.kv_cache, p.num_pages * 2 * p.page_size, p.hk, p.dqk, dtype, kShKeys))
     return cudaErrorNotSupported;
 #define HSTU_SHORT_CASE(DD, TT)                                                     \
-  return p.bias ? launch_inst<DD, TT, true>(p, mq, mk, mv, mbs, mc, num_sms, stream) \
-                : launch_inst<DD, TT, false>(p, mq, mk, mv, mbs, mc, num_sms, stream)
+  return p.window ? launch_inst<DD, TT, false, true>(p, mq, mk, mv, mbs, mc, num_sms, stream)  \
+         : p.bias ? launch_inst<DD, TT, true, false>(p, mq, mk, mv, mbs, mc, num_sms, stream) \
+                  : launch_inst<DD, TT, false, false>(p, mq, mk, mv, mbs, mc, num_sms, stream)
   const bool wide = p.dqk > 64 || p.dv > 64;
   if (dtype == HSTU_DTYPE_BF16) {
     if (!tanh_silu(p)) {

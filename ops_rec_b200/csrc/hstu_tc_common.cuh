@@ -120,6 +120,10 @@ __device__ __forceinline__ uint32_t low_bits(int n) {  // n lowest bits set, n c
 __device__ __forceinline__ uint32_t visible_bits(const RowBounds& rb, int j0) {
   return low_bits(rb.lim1 - j0) | (low_bits(rb.hi2 + 1 - j0) & ~low_bits(rb.lo2 - j0));
 }
+__device__ __forceinline__ uint32_t visible_bits(const WinBounds& rb, int j0) {
+  return low_bits(rb.lim1 - j0) | (low_bits(rb.hi2 + 1 - j0) & ~low_bits(rb.lo2 - j0)) |
+         (low_bits(rb.hi3 + 1 - j0) & ~low_bits(rb.lo3 - j0));
+}
 
 // Zeroes `pieces` 16-byte pieces from shared-memory address `first` on, in each of `boxes` regions `box_bytes` apart
 // (the rows of a V tile behind a sequence end); called by the 128 threads of a P/O group, `tid` = 0..127.

@@ -686,6 +686,161 @@ at::Tensor hstu_jagged_delta_autograd(const at::Tensor& q, const at::Tensor& k, 
                          seq_offset_k, num_context, num_target, target_group_size, alpha, deterministic);
 }
 
+// hstu_window: the jagged forward over a sliding window with sinks, its gradients and its autograd formula.  max_seq_len_k 0
+// means max_seq_len, an absent seq_offset_k the offsets of q (one operator for both forms of hstu_jagged).
+struct WindowCall {
+  Prepared pr;
+  int32_t window, num_sink;
+};
+
+WindowCall prepare_window(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t num_sink,
+                          int64_t max_q, int64_t max_k, double silu_scale, const OptTensor& seq_offset,
+                          const OptTensor& seq_offset_k, const OptTensor& num_target, OptInt group, OptDouble alpha,
+                          bool deterministic) {
+  TORCH_CHECK(seq_offset.has_value() && seq_offset->defined(), "hstu_window: seq_offset is required");
+  TORCH_CHECK(window >= 1, "hstu_window: window expect at least 1, but value is ", window);
+  TORCH_CHECK(num_sink >= 0, "hstu_window: num_sink expect at least 0, but value is ", num_sink);
+  TORCH_CHECK(group.value_or(0) >= 0 && group.value_or(0) <= INT32_MAX, "target_group_size must be >= 0");
+  const at::Tensor& off_k = seq_offset_k.has_value() && seq_offset_k->defined() ? *seq_offset_k : *seq_offset;
+  WindowCall c;
+  c.pr = prepare(q, k, v, c10::nullopt, c10::nullopt, HSTU_MASK_TRIL, max_q, max_k ? max_k : max_q, silu_scale, *seq_offset, off_k,
+                 c10::nullopt, num_target, group, alpha, deterministic);
+  // (beyond any sequence is beyond any sequence)
+  c.window = static_cast<int32_t>(std::min<int64_t>(window, INT32_MAX));
+  c.num_sink = static_cast<int32_t>(std::min<int64_t>(num_sink, INT32_MAX));
+  return c;
+}
+
+at::Tensor hstu_window(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t num_sink,
+                       int64_t max_q, int64_t max_k, double silu_scale, const OptTensor& seq_offset,
+                       const OptTensor& seq_offset_k, const OptTensor& num_target, OptInt group, OptDouble alpha,
+                       bool deterministic) {
+  c10::cuda::CUDAGuard guard(q.device());
+  WindowCall c = prepare_window(q, k, v, window, num_sink, max_q, max_k, silu_scale, seq_offset, seq_offset_k, num_target, group,
+                                alpha, deterministic);
+  auto out = at::empty({c.pr.q.size(0), c.pr.q.size(1), c.pr.v.size(2)}, c.pr.q.options());
+  HstuWindowArgs a;
+  memset(&a, 0, sizeof(a));
+  a.struct_bytes = sizeof(a);
+  a.window = c.window;
+  a.num_sink = c.num_sink;
+  a.fwd = c.pr.a;
+  a.fwd.out = out.data_ptr();
+  uint64_t ws_bytes = 0;
+  int rc = hstu_window_fwd_get_workspace_size(&a, &ws_bytes);
+  TORCH_CHECK(rc == 0, "hstu_window: ", hstu_last_error());
+  auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, c.pr.q.options().dtype(at::kByte));
+  rc = hstu_window_fwd(&a, ws.data_ptr(), ws_bytes, at::cuda::getCurrentCUDAStream().stream());
+  TORCH_CHECK(rc == 0, "hstu_window: ", hstu_last_error());
+  return out;
+}
+
+using Grads3 = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+
+Grads3 hstu_window_backward(const at::Tensor& grad, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
+                            int64_t num_sink, int64_t max_q, int64_t max_k, double silu_scale, const OptTensor& seq_offset,
+                            const OptTensor& seq_offset_k, const OptTensor& num_target, OptInt group, OptDouble alpha) {
+  TORCH_CHECK(grad.dim() == 3 && grad.is_cuda() && grad.scalar_type() == q.scalar_type(),
+              "grad must be a 3D CUDA tensor of q's dtype");
+  check_same_device(grad, q, "grad");
+  c10::cuda::CUDAGuard guard(q.device());
+  WindowCall c = prepare_window(q, k, v, window, num_sink, max_q, max_k, silu_scale, seq_offset, seq_offset_k, num_target, group,
+                                alpha, false);
+  TORCH_CHECK(grad.size(0) == c.pr.q.size(0) && grad.size(1) == c.pr.q.size(1) && grad.size(2) == c.pr.v.size(2),
+              "grad must be [total_q, heads_q, dim_v]");
+  auto g = grad.contiguous();
+  auto gq = at::empty_like(c.pr.q), gk = at::empty_like(c.pr.k), gv = at::empty_like(c.pr.v);
+  HstuWindowBwdArgs b;
+  memset(&b, 0, sizeof(b));
+  b.struct_bytes = sizeof(b);
+  b.window = c.window;
+  b.num_sink = c.num_sink;
+  b.bwd.struct_bytes = sizeof(b.bwd);
+  b.bwd.fwd = c.pr.a;
+  b.bwd.grad_out = g.data_ptr();
+  b.bwd.grad_q = gq.data_ptr();
+  b.bwd.grad_k = gk.data_ptr();
+  b.bwd.grad_v = gv.data_ptr();
+  uint64_t ws_bytes = 0;
+  int rc = hstu_window_bwd_get_workspace_size(&b, &ws_bytes);
+  TORCH_CHECK(rc == 0, "hstu_window_backward: ", hstu_last_error());
+  auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, c.pr.q.options().dtype(at::kByte));
+  rc = hstu_window_bwd(&b, ws.data_ptr(), ws_bytes, at::cuda::getCurrentCUDAStream().stream());
+  TORCH_CHECK(rc == 0, "hstu_window_backward: ", hstu_last_error());
+  return std::make_tuple(gq, gk, gv);
+}
+
+at::Tensor hstu_window_meta(const at::Tensor& q, const at::Tensor&, const at::Tensor& v, int64_t, int64_t, int64_t, int64_t, double,
+                            const OptTensor&, const OptTensor&, const OptTensor&, OptInt, OptDouble, bool) {
+  return meta_out(q, v);
+}
+
+Grads3 hstu_window_backward_meta(const at::Tensor&, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t,
+                                 int64_t, int64_t, int64_t, double, const OptTensor&, const OptTensor&, const OptTensor&, OptInt,
+                                 OptDouble) {
+  auto m = [](const at::Tensor& t) { return at::empty_like(t, t.options().device(c10::kMeta)); };
+  return std::make_tuple(m(q), m(k), m(v));
+}
+
+struct HstuWindowFunction : public torch::autograd::Function<HstuWindowFunction> {
+  static constexpr bool is_traceable = true;
+
+  static at::Tensor call(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t num_sink,
+                         int64_t max_q, int64_t max_k, double silu_scale, const OptTensor& seq_offset,
+                         const OptTensor& seq_offset_k, const OptTensor& num_target, OptInt group, OptDouble alpha,
+                         bool deterministic) {
+    at::AutoDispatchBelowAutograd guard;
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("ops_rec::hstu_window", "").typed<decltype(hstu_window)>();
+    return op.call(q, k, v, window, num_sink, max_q, max_k, silu_scale, seq_offset, seq_offset_k, num_target, group, alpha,
+                   deterministic);
+  }
+
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            int64_t window, int64_t num_sink, int64_t max_q, int64_t max_k, double silu_scale,
+                            const OptTensor& seq_offset, const OptTensor& seq_offset_k, const OptTensor& num_target, OptInt group,
+                            OptDouble alpha, bool deterministic) {
+    auto t = [](const OptTensor& o) { return o.has_value() ? *o : at::Tensor(); };
+    at::Tensor out = call(q, k, v, window, num_sink, max_q, max_k, silu_scale, seq_offset, seq_offset_k, num_target, group, alpha,
+                          deterministic);
+    ctx->save_for_backward({q, k, v, t(seq_offset), t(seq_offset_k), t(num_target)});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["num_sink"] = num_sink;
+    ctx->saved_data["max_q"] = max_q;
+    ctx->saved_data["max_k"] = max_k;
+    ctx->saved_data["silu_scale"] = silu_scale;
+    ctx->saved_data["group"] = group;
+    ctx->saved_data["alpha"] = alpha;
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    auto opt = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("ops_rec::hstu_window_backward", "")
+                               .typed<decltype(hstu_window_backward)>();
+    const Grads3 g = op.call(grads[0], saved[0], saved[1], saved[2], ctx->saved_data["window"].toInt(),
+                             ctx->saved_data["num_sink"].toInt(), ctx->saved_data["max_q"].toInt(), ctx->saved_data["max_k"].toInt(),
+                             ctx->saved_data["silu_scale"].toDouble(), opt(saved[3]), opt(saved[4]), opt(saved[5]),
+                             ctx->saved_data["group"].toOptional<int64_t>(), ctx->saved_data["alpha"].toOptional<double>());
+    torch::autograd::variable_list out(14);   // one per argument of forward
+    out[0] = std::get<0>(g);
+    out[1] = std::get<1>(g);
+    out[2] = std::get<2>(g);
+    return out;
+  }
+};
+
+at::Tensor hstu_window_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t num_sink,
+                                int64_t max_q, int64_t max_k, double silu_scale, const OptTensor& seq_offset,
+                                const OptTensor& seq_offset_k, const OptTensor& num_target, OptInt group, OptDouble alpha,
+                                bool deterministic) {
+  if (!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return HstuWindowFunction::call(q, k, v, window, num_sink, max_q, max_k, silu_scale, seq_offset, seq_offset_k, num_target,
+                                    group, alpha, deterministic);
+  return HstuWindowFunction::apply(q, k, v, window, num_sink, max_q, max_k, silu_scale, seq_offset, seq_offset_k, num_target, group,
+                                   alpha, deterministic);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(ops_rec, m) {
@@ -719,6 +874,12 @@ TORCH_LIBRARY_FRAGMENT(ops_rec, m) {
         " Tensor seq_offset_k=None, Tensor seq_offset_t=None, Tensor page_offsets=None, Tensor page_ids=None,"
         " Tensor last_page_len=None, Tensor num_target=None, int target_group_size=0, float? alpha=1.0,"
         " bool deterministic=False) -> Tensor");
+  m.def("hstu_window(Tensor q, Tensor k, Tensor v, int window, int num_sink=0, int max_seq_len=0, int max_seq_len_k=0, "
+        "float silu_scale=0.0, Tensor? seq_offset=None, Tensor? seq_offset_k=None, Tensor? num_target=None, "
+        "int? target_group_size=0, float? alpha=1.0, bool deterministic=False) -> Tensor");
+  m.def("hstu_window_backward(Tensor grad, Tensor q, Tensor k, Tensor v, int window, int num_sink=0, int max_seq_len=0, "
+        "int max_seq_len_k=0, float silu_scale=0.0, Tensor? seq_offset=None, Tensor? seq_offset_k=None, "
+        "Tensor? num_target=None, int? target_group_size=0, float? alpha=1.0) -> (Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(ops_rec, CUDA, m) {
@@ -731,11 +892,14 @@ TORCH_LIBRARY_IMPL(ops_rec, CUDA, m) {
   m.impl("hstu_dense", TORCH_FN(hstu_dense));
   m.impl("hstu_paged", TORCH_FN(hstu_paged));
   m.impl("in_linear_silu_backward", TORCH_FN(in_linear_silu_bwd));
+  m.impl("hstu_window", TORCH_FN(hstu_window));
+  m.impl("hstu_window_backward", TORCH_FN(hstu_window_backward));
 }
 
 TORCH_LIBRARY_IMPL(ops_rec, Autograd, m) {
   m.impl("hstu_jagged.equal", TORCH_FN(hstu_jagged_equal_autograd));
   m.impl("hstu_jagged.delta", TORCH_FN(hstu_jagged_delta_autograd));
+  m.impl("hstu_window", TORCH_FN(hstu_window_autograd));
 }
 
 TORCH_LIBRARY_IMPL(ops_rec, Meta, m) {
@@ -748,4 +912,6 @@ TORCH_LIBRARY_IMPL(ops_rec, Meta, m) {
   m.impl("hstu_dense", TORCH_FN(hstu_dense_meta));
   m.impl("hstu_paged", TORCH_FN(hstu_paged_meta));
   m.impl("in_linear_silu_backward", TORCH_FN(in_linear_silu_bwd_meta));
+  m.impl("hstu_window", TORCH_FN(hstu_window_meta));
+  m.impl("hstu_window_backward", TORCH_FN(hstu_window_backward_meta));
 }
