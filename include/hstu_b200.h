@@ -244,6 +244,65 @@ typedef struct HstuWindowBwdArgs {
 HSTU_API int hstu_window_bwd_get_workspace_size(const HstuWindowBwdArgs* args, uint64_t* workspace_bytes);
 HSTU_API int hstu_window_bwd(const HstuWindowBwdArgs* args, void* workspace, uint64_t workspace_bytes, void* stream);
 
+/* -------------------------------------------------------------------------------------------------- 8-bit cache
+ * A paged cache whose rows are held in 8 bits (no counterpart in the reference): the layout of hstu_paged's with one byte per
+ * element, kv_cache [num_pages, 2, page_size, heads_k, dim], and beside it kv_scale, fp32
+ * [num_pages, 2, page_size / block, heads_k]: value = number * scale of its block of `block` rows and its head. */
+enum { HSTU_HELD_E4M3 = 0 /* 8-bit floating point, 4 exponent and 3 fraction bits */, HSTU_HELD_INT8 = 1 };
+
+/* Writes new rows into such a cache.  The page table describes the cache AFTER the call, as the attention behind it reads it:
+ * sequence b has (pages - 1) * page_size + last_page_len[b] cached rows, the last len - num_target[b] of which are the first
+ * len - num_target[b] rows of its segment [seq_offset[b], seq_offset[b + 1]) of k and v.
+ *   scale of a block and head = the smallest power of two, 2^-100 at least, with amax <= 448 scale (int8: 127 scale) over its
+ *     finite new values; not smaller than the scale it has, if it holds rows already: those are rounded anew to the new scale
+ *   number = round to nearest even of value / scale, +-448 (+-127) for infinities; NaN stays NaN (int8: 0)
+ * Nothing else is touched: not the rows behind a sequence's last one, not the scales of other blocks.  A sequence whose table
+ * does not fit its rows, or names a page outside the cache, writes nothing (for a page outside: the blocks of that page) and
+ * sets bits in `status`.  A page that new rows go to belongs to one sequence; whole pages may be shared.
+ * Asynchronous on `stream`; no workspace. */
+typedef struct HstuCacheAppendArgs {
+  uint32_t struct_bytes;  /* sizeof(HstuCacheAppendArgs) */
+  int32_t dtype;          /* HSTU_DTYPE_*, of k and v */
+  int32_t held;           /* HSTU_HELD_* */
+  int32_t page_size;
+  int32_t block;          /* rows per scale; divides page_size */
+  int32_t heads_k;
+  int32_t dim;            /* [1, 512] */
+  int32_t index_bytes;    /* 4 or 8 */
+  int32_t batch;
+  int32_t reserved;
+  int64_t total;          /* rows of k and v, [total, heads_k, dim] contiguous */
+  int64_t num_pages;
+  int64_t num_page_ids;
+  const void* k;
+  const void* v;
+  void* kv_cache;
+  void* kv_scale;
+  const void* seq_offset;     /* [batch + 1] */
+  const void* num_target;     /* [batch] or null */
+  const void* page_offsets;   /* [batch + 1] */
+  const void* page_ids;       /* [num_page_ids] */
+  const void* last_page_len;  /* [batch] */
+  void* status;               /* optional device uint32, as in OpsRecInLinearSiluArgs: HSTU_ST_* bits are or-ed into it */
+} HstuCacheAppendArgs;
+HSTU_API int hstu_cache_append(const HstuCacheAppendArgs* args, void* stream);
+
+/* hstu_paged over such a cache: the arguments of hstu_paged_fwd without mask, attn_bias and num_context (mask_type
+ * HSTU_MASK_TRIL), paged.kv_cache in 8 bits.  window 0: every key up to the row's own; else the window and sinks of
+ * hstu_window_fwd.  q, k, v, out in bf16, fp16 or fp32. */
+typedef struct HstuPaged8Args {
+  uint32_t struct_bytes;  /* sizeof(HstuPaged8Args) */
+  int32_t held;           /* HSTU_HELD_* */
+  int32_t block;          /* rows per scale; divides paged.page_size */
+  int32_t window;         /* 0: none */
+  int32_t num_sink;
+  uint32_t reserved;
+  const void* kv_scale;
+  HstuPagedArgs paged;
+} HstuPaged8Args;
+HSTU_API int hstu_paged_8bit_fwd_get_workspace_size(const HstuPaged8Args* args, uint64_t* workspace_bytes);
+HSTU_API int hstu_paged_8bit_fwd(const HstuPaged8Args* args, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------------------------------------------ ln_mul
  * The step that consumes the attention output in an HSTU layer: out = (LayerNorm(x) * gamma + beta) * u over the
  * rows of fp32 [rows, cols] matrices, eps = 1e-5 (fixed by the reference's host code, ln_mul/op_host/ln_mul.cpp:73).

@@ -16,6 +16,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libhstu_b200.so")
 
 DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2
+HELD_E4M3, HELD_INT8 = 0, 1
 MASK_TRIL, MASK_TRIU, MASK_NONE, MASK_CUSTOM = 0, 1, 2, 3
 FLAG_DETERMINISTIC, FLAG_ALPHA_BEFORE_BIAS, FLAG_FORCE_GENERIC = 1, 2, 4
 ST_BAD_OFFSETS, ST_LEN_GT_MAX, ST_BAD_CTX_TARGET, ST_BAD_PAGES, ST_PIPE_TIMEOUT = 1, 2, 4, 8, 256
@@ -29,7 +30,7 @@ EXPORTS = (
     "hstu_paged_fwd_get_workspace_size", "hstu_paged_fwd",
     "ops_rec_in_linear_silu_bwd_get_workspace_size", "ops_rec_in_linear_silu_bwd",
     "hstu_window_fwd_get_workspace_size", "hstu_window_fwd", "hstu_window_bwd_get_workspace_size", "hstu_window_bwd",
-    "hstu_debug_window_host",
+    "hstu_debug_window_host", "hstu_cache_append", "hstu_paged_8bit_fwd_get_workspace_size", "hstu_paged_8bit_fwd",
 )
 STATIC_SCRATCH_BYTES = 1 << 20
 E_SCRATCH_LIMIT = -6
@@ -75,6 +76,21 @@ class HstuWindowArgs(C.Structure):
 class HstuWindowBwdArgs(C.Structure):
     _fields_ = [("struct_bytes", C.c_uint32), ("window", C.c_int32), ("num_sink", C.c_int32), ("reserved", C.c_uint32),
                 ("bwd", HstuJaggedBwdArgs)]
+
+
+class HstuCacheAppendArgs(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_uint32), ("dtype", C.c_int32), ("held", C.c_int32), ("page_size", C.c_int32), ("block", C.c_int32),
+        ("heads_k", C.c_int32), ("dim", C.c_int32), ("index_bytes", C.c_int32), ("batch", C.c_int32), ("reserved", C.c_int32),
+        ("total", C.c_int64), ("num_pages", C.c_int64), ("num_page_ids", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("kv_cache", C.c_void_p), ("kv_scale", C.c_void_p), ("seq_offset", C.c_void_p), ("num_target", C.c_void_p),
+        ("page_offsets", C.c_void_p), ("page_ids", C.c_void_p), ("last_page_len", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class HstuPaged8Args(C.Structure):
+    _fields_ = [("struct_bytes", C.c_uint32), ("held", C.c_int32), ("block", C.c_int32), ("window", C.c_int32),
+                ("num_sink", C.c_int32), ("reserved", C.c_uint32), ("kv_scale", C.c_void_p), ("paged", HstuPagedArgs)]
 
 
 class OpsRecInLinearSiluArgs(C.Structure):
@@ -160,9 +176,14 @@ def load():
     lib.hstu_window_fwd.argtypes = [W, C.c_void_p, C.c_uint64, C.c_void_p]
     lib.hstu_window_bwd_get_workspace_size.argtypes = [WB, C.POINTER(C.c_uint64)]
     lib.hstu_window_bwd.argtypes = [WB, C.c_void_p, C.c_uint64, C.c_void_p]
+    lib.hstu_cache_append.argtypes = [C.POINTER(HstuCacheAppendArgs), C.c_void_p]
+    P8 = C.POINTER(HstuPaged8Args)
+    lib.hstu_paged_8bit_fwd_get_workspace_size.argtypes = [P8, C.POINTER(C.c_uint64)]
+    lib.hstu_paged_8bit_fwd.argtypes = [P8, C.c_void_p, C.c_uint64, C.c_void_p]
     lib.hstu_debug_window_host.argtypes = [C.c_int32] * 9 + [C.c_void_p] * 2
     for name in ("hstu_window_fwd_get_workspace_size", "hstu_window_fwd", "hstu_window_bwd_get_workspace_size",
-                 "hstu_window_bwd", "hstu_debug_window_host"):
+                 "hstu_window_bwd", "hstu_debug_window_host", "hstu_cache_append",
+                 "hstu_paged_8bit_fwd_get_workspace_size", "hstu_paged_8bit_fwd"):
         getattr(lib, name).restype = C.c_int
     lib.ops_rec_ln_mul_f32.argtypes = [C.c_void_p] * 5 + [C.c_int64, C.c_int64, C.c_void_p]
     lib.ops_rec_ln_mul_f32.restype = C.c_int
@@ -429,6 +450,92 @@ def hstu_paged_forward(q, k, v, kv_cache, mask=None, attn_bias=None, mask_type=0
     stream = torch.cuda.current_stream(q.device).cuda_stream
     with torch.cuda.device(q.device):
         check(load().hstu_paged_fwd(C.byref(a), ws.data_ptr(), n.value, stream))
+        if return_status:
+            st = C.c_uint32(0)
+            check(load().hstu_jagged_fwd_status(ws.data_ptr(), stream, C.byref(st)))
+            return out, st.value
+    del keep, conv
+    return out
+
+
+def _held_code(kv_cache):
+    import torch
+    code = {torch.float8_e4m3fn: HELD_E4M3, torch.int8: HELD_INT8}.get(kv_cache.dtype)
+    if code is None:
+        raise HstuError(-2, f"kv_cache must be float8_e4m3fn or int8, but is {kv_cache.dtype}")
+    return code
+
+
+def _check_held(kv_cache, kv_scale, heads_k, dim):
+    import torch
+    if kv_cache.dim() != 5 or kv_cache.shape[1] != 2 or tuple(kv_cache.shape[3:]) != (heads_k, dim):
+        raise HstuError(-2, "kv_cache must be [pages, 2, page_size, heads_k, dim]")
+    n = kv_scale.shape[2] if kv_scale.dim() == 4 else 0
+    if (kv_scale.dtype != torch.float32 or n < 1 or kv_cache.shape[2] % n != 0 or
+            tuple(kv_scale.shape) != (kv_cache.shape[0], 2, n, heads_k)):
+        raise HstuError(-2, "kv_scale must be [pages, 2, page_size / block, heads_k] in float32")
+    if not (kv_cache.is_contiguous() and kv_scale.is_contiguous()):
+        raise HstuError(-2, "kv_cache and kv_scale must be contiguous")
+    return kv_cache.shape[2] // n
+
+
+def hstu_cache_append(k, v, kv_cache, kv_scale, seq_offset, page_offsets, page_ids, last_page_len, num_target=None, *,
+                      return_status=False):
+    """ops_rec::hstu_cache_append through the C ABI on CUDA tensors; kv_cache and kv_scale are written in place."""
+    import torch
+    if k.dim() != 3 or v.shape != k.shape:
+        raise HstuError(-2, "k and v must be [tokens, heads_k, dim] and of one shape")
+    if not k.is_cuda:
+        raise HstuError(-2, "tensors must live on a CUDA device; there is no CPU implementation")
+    for t in (v, kv_cache, kv_scale, seq_offset, page_offsets, page_ids, last_page_len, num_target):
+        if t is not None and t.device != k.device:
+            raise ValueError(f"a tensor is on {t.device} but k is on {k.device}")
+    k, v, it = k.contiguous(), v.contiguous(), seq_offset.dtype
+    idx = [t.to(it).contiguous() if t is not None else None for t in (seq_offset, num_target, page_offsets, page_ids, last_page_len)]
+    status = torch.zeros(1, dtype=torch.int32, device=k.device) if return_status else None
+    ptr = lambda t: t.data_ptr() if t is not None else None   # noqa: E731
+    a = HstuCacheAppendArgs(C.sizeof(HstuCacheAppendArgs), _dtype_code(k.dtype), _held_code(kv_cache), kv_cache.shape[2],
+                            _check_held(kv_cache, kv_scale, k.shape[1], k.shape[2]), k.shape[1], k.shape[2],
+                            seq_offset.element_size(), seq_offset.shape[0] - 1, 0, k.shape[0], kv_cache.shape[0], page_ids.numel(),
+                            ptr(k), ptr(v), ptr(kv_cache), ptr(kv_scale), *(ptr(t) for t in idx), ptr(status))
+    with torch.cuda.device(k.device):
+        check(load().hstu_cache_append(C.byref(a), torch.cuda.current_stream(k.device).cuda_stream))
+    return int(status) & 0xffffffff if return_status else None
+
+
+def hstu_paged_8bit_forward(q, k, v, kv_cache, kv_scale, max_seq_len=0, max_seq_len_k=0, silu_scale=0.0, seq_offset=None,
+                            seq_offset_k=None, page_offsets=None, page_ids=None, last_page_len=None, num_target=None,
+                            target_group_size=0, alpha=1.0, window=0, num_sink=0, *, flags=0, return_status=False,
+                            workspace_fill=None):
+    """ops_rec::hstu_paged_8bit through hstu_paged_8bit_fwd on CUDA tensors."""
+    import torch
+    if q.dim() != 3:
+        raise HstuError(-2, "The q should be 3D in jagged layout")
+    if not q.is_cuda:
+        raise HstuError(-2, "tensors must live on a CUDA device; there is no CPU implementation")
+    block = _check_held(kv_cache, kv_scale, k.shape[1], k.shape[2])
+    for t in (kv_cache, kv_scale, page_offsets, page_ids, last_page_len):
+        if t.device != q.device:
+            raise ValueError(f"a page-table tensor is on {t.device} but q is on {q.device}")
+    q, k, v, it = q.contiguous(), k.contiguous(), v.contiguous(), seq_offset.dtype
+    seq_offset_k, page_offsets, page_ids, last_page_len = conv = [
+        t.to(it).contiguous() for t in (seq_offset_k, page_offsets, page_ids, last_page_len)]
+    out = torch.empty(q.shape[0], q.shape[1], v.shape[2], dtype=q.dtype, device=q.device)
+    base, keep = make_args(q, k, v, out, seq_offset, seq_offset_k=seq_offset_k, max_seq_len=max_seq_len,
+                           max_seq_len_k=max_seq_len_k or None, silu_scale=silu_scale, num_target=num_target,
+                           target_group_size=target_group_size, alpha=alpha, flags=flags)
+    p = HstuPagedArgs(C.sizeof(HstuPagedArgs), kv_cache.shape[2], base, kv_cache.data_ptr(), page_offsets.data_ptr(),
+                      page_ids.data_ptr(), last_page_len.data_ptr(), None, kv_cache.shape[0], page_ids.numel())
+    a = HstuPaged8Args(C.sizeof(HstuPaged8Args), _held_code(kv_cache), block, int(window), int(num_sink), 0, kv_scale.data_ptr(), p)
+    n = C.c_uint64(0)
+    check(load().hstu_paged_8bit_fwd_get_workspace_size(C.byref(a), C.byref(n)))
+    # (workspace_fill: tests fill the workspace with a byte pattern first - nothing the call reads may be uninitialised)
+    ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
+    if workspace_fill is not None:
+        ws.fill_(workspace_fill)
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    with torch.cuda.device(q.device):
+        check(load().hstu_paged_8bit_fwd(C.byref(a), ws.data_ptr(), n.value, stream))
         if return_status:
             st = C.c_uint32(0)
             check(load().hstu_jagged_fwd_status(ws.data_ptr(), stream, C.byref(st)))

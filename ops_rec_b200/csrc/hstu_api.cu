@@ -36,7 +36,8 @@ cudaError_t launch_in_linear_silu_bwd(const LinSiluParams& shape, const void* x,
                                       cudaStream_t stream);
 cudaError_t launch_paged_gather(const KParams& p, const void* kv_cache, const void* k_in, const void* v_in,
                                 void* k_out, void* v_out, long long capacity, long long num_pages,
-                                long long num_page_ids, int esize, cudaStream_t stream);
+                                long long num_page_ids, int dtype, cudaStream_t stream);
+cudaError_t launch_append(const HstuCacheAppendArgs& a, cudaStream_t stream);
 }  // namespace hstu
 
 namespace {
@@ -393,9 +394,121 @@ int hstu_paged_fwd(const HstuPagedArgs* args, void* workspace, uint64_t workspac
   p.paged_direct = !p.paged_split && tc && args->page_size == hstu::kTileN && args->num_pages <= 0x7fffffll ? 1 : 0;
   if (!p.paged_split) {
     const cudaError_t e = hstu::launch_paged_gather(p, args->kv_cache, b->k, b->v, k_stage, v_stage, pl.capacity,
-                                                    args->num_pages, args->num_page_ids, pl.esize, stream);
+                                                    args->num_pages, args->num_page_ids, pl.fwd.dtype, stream);
     if (e != cudaSuccess) return fail(HSTU_E_CUDA, "gather launch: %s", cudaGetErrorString(e));
   }
+  return jagged_fwd_impl(&pl.fwd, workspace, pl.fwd_bytes, stream_v, &p);
+}
+
+// ---------------------------------------------------------------------------------------------- 8-bit cache
+static int validate_held(int held, int block, int page_size) {
+  if (held != HSTU_HELD_E4M3 && held != HSTU_HELD_INT8) return fail(HSTU_E_PARAM, "the cache must hold e4m3 or int8 numbers");
+  if (page_size < 1) return fail(HSTU_E_PARAM, "page_size must be positive, but value is %d", page_size);
+  if (block < 1 || page_size % block != 0)
+    return fail(HSTU_E_PARAM, "kv_scale: a page of %d rows must hold whole blocks, but a block has %d", page_size, block);
+  return HSTU_OK;
+}
+
+int hstu_cache_append(const HstuCacheAppendArgs* a, void* stream_v) {
+  g_err[0] = 0;
+  if (!a) return fail(HSTU_E_NULL, "args is null");
+  if (a->struct_bytes != sizeof(HstuCacheAppendArgs))
+    return fail(HSTU_E_PARAM, "struct_bytes is %u, this library expects %zu", a->struct_bytes, sizeof(HstuCacheAppendArgs));
+  if (a->dtype != HSTU_DTYPE_BF16 && a->dtype != HSTU_DTYPE_FP16 && a->dtype != HSTU_DTYPE_FP32)
+    return fail(HSTU_E_PARAM, "hstu_cache_append: k and v must be bf16, fp16 or fp32");
+  int rc = validate_held(a->held, a->block, a->page_size);
+  if (rc) return rc;
+  if (a->batch < 1) return fail(HSTU_E_PARAM, "seq_offset params error should have at least two element.");
+  if (a->index_bytes != 4 && a->index_bytes != 8) return fail(HSTU_E_PARAM, "seq_offset must be int32 or int64");
+  if (a->heads_k < 1 || a->heads_k > kMaxHeads)
+    return fail(HSTU_E_PARAM, "head count expect in [1, %d], but value is %d", kMaxHeads, a->heads_k);
+  if (a->dim < 1 || a->dim > kMaxDim) return fail(HSTU_E_PARAM, "k/v head dim expect in [1, 512], but value is %d", a->dim);
+  if (a->num_pages < 1 || a->num_page_ids < 1) return fail(HSTU_E_PARAM, "kv_cache / page_ids must not be empty");
+  if (a->total < 0 || a->total > 0x7fffff00ll || a->batch > 0xffffff)
+    return fail(HSTU_E_PARAM, "hstu_cache_append: %lld rows of %d sequences are too many", (long long)a->total, a->batch);
+  const long long esize = a->dtype == HSTU_DTYPE_FP32 ? 4 : 2;
+  if ((reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v)) % esize ||
+      ((reinterpret_cast<uintptr_t>(a->kv_scale) | reinterpret_cast<uintptr_t>(a->status)) & 3u))
+    return fail(HSTU_E_PARAM, "hstu_cache_append: a pointer is not aligned to its elements");
+  if (a->total == 0) return HSTU_OK;
+  if (!a->k || !a->v || !a->kv_cache || !a->kv_scale || !a->seq_offset || !a->page_offsets || !a->page_ids || !a->last_page_len)
+    return fail(HSTU_E_NULL, "hstu_cache_append: null pointer");
+  const long long units = (a->total / a->block + 2ll * a->batch) * 2 * a->heads_k;
+  if (units > 0x7fffffffll) return fail(HSTU_E_PARAM, "hstu_cache_append: %lld rows in blocks of %d are too many", (long long)a->total, a->block);
+  DeviceInfo dev;
+  rc = device_info(&dev);
+  if (rc) return rc;
+  if (dev.major != 10) return fail(HSTU_E_ARCH, "this library is built for sm_100a only; device has compute capability %d.x", dev.major);
+  const cudaError_t e = hstu::launch_append(*a, static_cast<cudaStream_t>(stream_v));
+  if (e != cudaSuccess) return fail(HSTU_E_CUDA, "hstu_cache_append launch: %s", cudaGetErrorString(e));
+  return HSTU_OK;
+}
+
+namespace {
+// hstu_paged's plan for a cache in 8 bits, whose staging tensors are in the call's type.
+int plan_paged8(const HstuPaged8Args* a, PagedPlan* pl) {
+  if (!a) return fail(HSTU_E_NULL, "args is null");
+  if (a->struct_bytes != sizeof(HstuPaged8Args))
+    return fail(HSTU_E_PARAM, "struct_bytes is %u, this library expects %zu", a->struct_bytes, sizeof(HstuPaged8Args));
+  int rc = validate_held(a->held, a->block, a->paged.page_size);
+  if (rc) return rc;
+  // (window 0 is none: what else a window asks of a call holds here in any case)
+  rc = a->window < 0 ? fail(HSTU_E_PARAM, "window expect at least 0, but value is %d", a->window)
+                     : validate_window(&a->paged.base, a->window ? a->window : 1, a->num_sink);
+  if (rc) return rc;
+  return plan_paged(&a->paged, pl);
+}
+}  // namespace
+
+int hstu_paged_8bit_fwd_get_workspace_size(const HstuPaged8Args* args, uint64_t* workspace_bytes) {
+  g_err[0] = 0;
+  if (!workspace_bytes) return fail(HSTU_E_NULL, "workspace_bytes is null");
+  PagedPlan pl;
+  const int rc = plan_paged8(args, &pl);
+  if (rc) return rc;
+  *workspace_bytes = pl.fwd_bytes + 2 * pl.stage_bytes;
+  return HSTU_OK;
+}
+
+int hstu_paged_8bit_fwd(const HstuPaged8Args* args, void* workspace, uint64_t workspace_bytes, void* stream_v) {
+  g_err[0] = 0;
+  PagedPlan pl;
+  int rc = plan_paged8(args, &pl);
+  if (rc) return rc;
+  const HstuPagedArgs* a = &args->paged;
+  const HstuJaggedArgs* b = &a->base;
+  if (!b->seq_offset_q || !b->seq_offset_k) return fail(HSTU_E_NULL, "seq_offset / seq_offset_k is null");
+  if (!a->kv_cache || !args->kv_scale || !a->page_offsets || !a->page_ids || !a->last_page_len)
+    return fail(HSTU_E_NULL, "kv_cache / kv_scale / page_offsets / page_ids / last_page_len is null");
+  if (reinterpret_cast<uintptr_t>(args->kv_scale) & 3u) return fail(HSTU_E_PARAM, "kv_scale must be 4-byte aligned");
+  if (b->total_q > 0 && (!b->q || !b->out || !b->k || !b->v)) return fail(HSTU_E_NULL, "q / k / v / out is null");
+  const uint64_t need = pl.fwd_bytes + 2 * pl.stage_bytes;
+  if (!workspace) return fail(HSTU_E_WORKSPACE, "workspace is null (%llu bytes needed)", (unsigned long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSTU_E_WORKSPACE, "workspace must be 256-byte aligned");
+  if (workspace_bytes < need)
+    return fail(HSTU_E_WORKSPACE, "workspace has %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
+                (unsigned long long)need);
+  char* base = static_cast<char*>(workspace);
+  pl.fwd.q = b->q;
+  pl.fwd.out = b->out;
+  pl.fwd.k = base + pl.fwd_bytes;
+  pl.fwd.v = base + pl.fwd_bytes + pl.stage_bytes;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  hstu::KParams p = to_params(&pl.fwd, nullptr, 0);
+  set_window(&p, args->window, args->num_sink);
+  p.page_offsets = a->page_offsets;
+  p.page_ids = a->page_ids;
+  p.last_page_len = a->last_page_len;
+  p.page_size = a->page_size;
+  p.num_pages = a->num_pages;
+  p.num_page_ids = a->num_page_ids;
+  p.kv_cache = a->kv_cache;
+  p.kv_scale = static_cast<const float*>(args->kv_scale);
+  p.held = args->held;
+  p.scale_block = args->block;
+  const cudaError_t e = hstu::launch_paged_gather(p, a->kv_cache, b->k, b->v, base + pl.fwd_bytes, base + pl.fwd_bytes + pl.stage_bytes,
+                                                  pl.capacity, a->num_pages, a->num_page_ids, pl.fwd.dtype, stream);
+  if (e != cudaSuccess) return fail(HSTU_E_CUDA, "gather launch: %s", cudaGetErrorString(e));
   return jagged_fwd_impl(&pl.fwd, workspace, pl.fwd_bytes, stream_v, &p);
 }
 

@@ -85,6 +85,9 @@ struct KParams {
   int fwd_by_steps;   // the same for the forward's work list: all sequences' last q-pairs first, then the ones before
   // hstu_window and hstu_paged_8bit (0 otherwise): keys a row sees up to its own position, and the first keys that stay visible
   int window, sink;
+  // hstu_paged_8bit: kv_cache holds 8-bit numbers (HSTU_HELD_*), with a scale per scale_block rows and head
+  const float* kv_scale;      // [num_pages, 2, page_size / scale_block, hk], null for a cache in the call's type
+  int held, scale_block;
 };
 
 // Backward call: the forward's parameters plus the gradient tensors.

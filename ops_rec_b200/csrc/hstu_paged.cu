@@ -14,7 +14,13 @@
 // Inconsistent page tables are flagged by the scheduling pre-pass (HSTU_ST_BAD_PAGES); this pass only makes them
 // harmless: a row whose source does not exist (a page slot outside the sequence's range, a page id outside the cache)
 // becomes zeros, and nothing outside the tensors is ever addressed.
-#include "hstu_common.cuh"
+//
+// hstu_paged_8bit calls that no kernel reads in place (fp32 queries, wide or odd heads) come through here too: the same pass,
+// with the cached rows turned into the call's type, number * scale rounded once, on the way.
+#include <type_traits>
+
+#include "hstu_held.cuh"
+#include "hstu_simt.cuh"
 
 namespace hstu {
 
@@ -38,7 +44,13 @@ struct GatherParams {
   int index_bytes, batch, page_size;
   int row_bytes;                // heads_k * dim * element size
   int skip_full_pages;          // the attention kernel reads whole pages from the cache: stage only the rest
+  // a cache of 8-bit rows
+  const float* scale;           // [pages, 2, page_size / block, heads_k]
+  int block, heads, dim;
 };
+
+// What a row of the cache is made of, and the type it is staged in: bytes that are copied, or 8-bit numbers.
+struct AsIs {};
 
 // One CTA per kGatherRows consecutive rows of a staging tensor (grid.y = 0: keys, 1: values).
 //   phase 1  one thread per row finds the row's source: its sequence by bisection over seq_offset_k, then either a row
@@ -46,8 +58,11 @@ struct GatherParams {
 //            tile's worth (a tile that runs past the end of the data multiplies those rows by P = 0, which must not
 //            meet the NaN bit patterns uninitialised memory may hold), the rest of the capacity is never read
 //   phase 2  all threads copy: a warp takes four rows at a time and issues their loads before the first store
-template <typename V>
+// V: the piece that is copied at once; with 8-bit rows kN elements of type T at a time.
+template <typename V, typename H, typename T, int kN>
 __global__ void __launch_bounds__(kGatherThreads) hstu_paged_gather_kernel(const GatherParams p) {
+  constexpr bool kHeld = !std::is_same<H, AsIs>::value;
+  __shared__ const float* s_scale[kHeld ? kGatherRows : 1];   // of the row's block, null for a row of k / v
   __shared__ const unsigned char* s_src[kGatherRows];
   __shared__ unsigned char s_mode[kGatherRows];   // 0: skip the row, 1: copy from s_src, 2: zeros
   __shared__ long long s_off[kGatherRows + 1];    // seq_offset_k[b0 .. b0 + 64], b0 = the sequence of the CTA's first row
@@ -103,6 +118,7 @@ __global__ void __launch_bounds__(kGatherThreads) hstu_paged_gather_kernel(const
   if (threadIdx.x < kGatherRows) {
     const long long row = first + threadIdx.x;
     const unsigned char* src = nullptr;
+    const float* scale = nullptr;
     unsigned char mode = 0;
     long long k_end = load_index(p.offk, p.index_bytes, p.batch);
     if (k_end < 0) k_end = 0;
@@ -154,7 +170,10 @@ __global__ void __launch_bounds__(kGatherThreads) hstu_paged_gather_kernel(const
           if (slot < pg1) {
             const long long pid = load_index(p.page_ids, p.index_bytes, slot);
             if (pid >= 0 && pid < p.num_pages) {
-              src = p.cache + ((pid * 2 + (is_v ? 1 : 0)) * p.page_size + r % p.page_size) * p.row_bytes;
+              src = p.cache + ((pid * 2 + (is_v ? 1 : 0)) * p.page_size + r % p.page_size) *
+                                  (kHeld ? p.heads * p.dim : p.row_bytes);
+              if (kHeld)
+                scale = p.scale + ((pid * 2 + (is_v ? 1 : 0)) * (p.page_size / p.block) + r % p.page_size / p.block) * p.heads;
               mode = 1;
             }
           }
@@ -169,10 +188,44 @@ __global__ void __launch_bounds__(kGatherThreads) hstu_paged_gather_kernel(const
     }
     s_src[threadIdx.x] = src;
     s_mode[threadIdx.x] = mode;
+    if (kHeld) s_scale[threadIdx.x] = scale;
   }
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int kWarps = kGatherThreads / 32;
+  if constexpr (kHeld) {
+    const int n = p.heads * p.dim;
+    for (int r = warp; r < kGatherRows; r += kWarps) {
+      if (!s_mode[r]) continue;
+      T* to = reinterpret_cast<T*>(out) + (first + r) * n;
+      const float* scale = s_scale[r];
+      for (int i = lane * kN; i < n; i += 32 * kN) {
+        alignas(16) T x[kN];
+        if (s_mode[r] == 2) {
+#pragma unroll
+          for (int e = 0; e < kN; ++e) x[e] = simt::from_float<T>(0.f);
+        } else if (scale) {
+          uint8_t v[kN];
+          if constexpr (kN == 8) {
+            const uint2 u = *reinterpret_cast<const uint2*>(s_src[r] + i);
+#pragma unroll
+            for (int e = 0; e < kN; ++e) v[e] = reinterpret_cast<const uint8_t*>(&u)[e];
+          } else {
+            v[0] = s_src[r][i];
+          }
+          const float f = __ldg(scale + i / p.dim);
+#pragma unroll
+          for (int e = 0; e < kN; ++e) x[e] = simt::from_float<T>(H::to_float(v[e]) * f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kN; ++e) x[e] = reinterpret_cast<const T*>(s_src[r])[i + e];
+        }
+#pragma unroll
+        for (int e = 0; e < kN; ++e) to[i + e] = x[e];
+      }
+    }
+    return;
+  }
   constexpr int kBatch = 4;   // rows in flight per warp
   for (int r0 = warp * kBatch; r0 < kGatherRows; r0 += kWarps * kBatch) {
     for (int i = lane * static_cast<int>(sizeof(V)); i < p.row_bytes; i += 32 * static_cast<int>(sizeof(V))) {
@@ -188,10 +241,17 @@ __global__ void __launch_bounds__(kGatherThreads) hstu_paged_gather_kernel(const
 
 }  // namespace
 
+template <typename T, int kN>
+static void launch_held(const GatherParams& g, int held, dim3 grid, cudaStream_t stream) {
+  if (held == HSTU_HELD_E4M3) hstu_paged_gather_kernel<uint4, E4m3, T, kN><<<grid, kGatherThreads, 0, stream>>>(g);
+  else hstu_paged_gather_kernel<uint4, Int8, T, kN><<<grid, kGatherThreads, 0, stream>>>(g);
+}
+
 // Enqueues the gather.  All pointers are device pointers; capacity = rows of each staging tensor.
 cudaError_t launch_paged_gather(const KParams& p, const void* kv_cache, const void* k_in, const void* v_in,
                                 void* k_out, void* v_out, long long capacity, long long num_pages,
-                                long long num_page_ids, int esize, cudaStream_t stream) {
+                                long long num_page_ids, int dtype, cudaStream_t stream) {
+  const int esize = dtype == HSTU_DTYPE_FP32 ? 4 : 2;
   GatherParams g;
   g.cache = static_cast<const unsigned char*>(kv_cache);
   g.k_in = static_cast<const unsigned char*>(k_in);
@@ -212,16 +272,28 @@ cudaError_t launch_paged_gather(const KParams& p, const void* kv_cache, const vo
   g.page_size = p.page_size;
   g.row_bytes = p.hk * p.dqk * esize;
   g.skip_full_pages = p.paged_direct;
+  g.scale = p.kv_scale;
+  g.block = p.scale_block;
+  g.heads = p.hk;
+  g.dim = p.dqk;
   const dim3 grid(static_cast<unsigned>((capacity + kGatherRows - 1) / kGatherRows), 2, 1);
   const uintptr_t align = reinterpret_cast<uintptr_t>(kv_cache) | reinterpret_cast<uintptr_t>(k_in) |
                           reinterpret_cast<uintptr_t>(v_in) | reinterpret_cast<uintptr_t>(k_out) |
                           reinterpret_cast<uintptr_t>(v_out) | static_cast<uintptr_t>(g.row_bytes);
-  if ((align & 15u) == 0)
-    hstu_paged_gather_kernel<uint4><<<grid, kGatherThreads, 0, stream>>>(g);
+  if (p.kv_scale) {
+    const bool vec = p.dqk % 8 == 0 && (reinterpret_cast<uintptr_t>(kv_cache) & 7u) == 0;
+    if (dtype == HSTU_DTYPE_BF16)
+      vec ? launch_held<__nv_bfloat16, 8>(g, p.held, grid, stream) : launch_held<__nv_bfloat16, 1>(g, p.held, grid, stream);
+    else if (dtype == HSTU_DTYPE_FP16)
+      vec ? launch_held<__half, 8>(g, p.held, grid, stream) : launch_held<__half, 1>(g, p.held, grid, stream);
+    else
+      vec ? launch_held<float, 8>(g, p.held, grid, stream) : launch_held<float, 1>(g, p.held, grid, stream);
+  } else if ((align & 15u) == 0)
+    hstu_paged_gather_kernel<uint4, AsIs, float, 1><<<grid, kGatherThreads, 0, stream>>>(g);
   else if ((align & 3u) == 0)
-    hstu_paged_gather_kernel<uint32_t><<<grid, kGatherThreads, 0, stream>>>(g);
+    hstu_paged_gather_kernel<uint32_t, AsIs, float, 1><<<grid, kGatherThreads, 0, stream>>>(g);
   else
-    hstu_paged_gather_kernel<uint16_t><<<grid, kGatherThreads, 0, stream>>>(g);
+    hstu_paged_gather_kernel<uint16_t, AsIs, float, 1><<<grid, kGatherThreads, 0, stream>>>(g);
   return cudaGetLastError();
 }
 

@@ -841,6 +841,162 @@ at::Tensor hstu_window_autograd(const at::Tensor& q, const at::Tensor& k, const 
                                    alpha, deterministic);
 }
 
+// The 8-bit cache: hstu_cache_append writes it, hstu_paged_8bit attends over it.
+int held_code(const at::Tensor& kv_cache) {
+  const auto t = kv_cache.scalar_type();
+  TORCH_CHECK(t == at::kFloat8_e4m3fn || t == at::kChar, "kv_cache must be float8_e4m3fn or int8, but is ", t);
+  return t == at::kChar ? HSTU_HELD_INT8 : HSTU_HELD_E4M3;
+}
+// the rows of a scale's block
+int32_t check_held(const at::Tensor& kv_cache, const at::Tensor& kv_scale, const at::Tensor& k) {
+  TORCH_CHECK(kv_cache.dim() == 5 && kv_cache.size(1) == 2 && kv_cache.size(3) == k.size(1) && kv_cache.size(4) == k.size(2) &&
+                  kv_cache.numel() > 0,
+              "kv_cache must be [pages, 2, page_size, heads_k, dim] and not empty");
+  TORCH_CHECK(kv_scale.scalar_type() == at::kFloat && kv_scale.dim() == 4 && kv_scale.size(2) >= 1 &&
+                  kv_cache.size(2) % kv_scale.size(2) == 0 && kv_scale.size(0) == kv_cache.size(0) && kv_scale.size(1) == 2 &&
+                  kv_scale.size(3) == k.size(1),
+              "kv_scale must be [pages, 2, page_size / block, heads_k] in float32");
+  TORCH_CHECK(kv_cache.size(2) <= INT32_MAX, "kv_cache: page_size is too large");
+  return static_cast<int32_t>(kv_cache.size(2) / kv_scale.size(2));
+}
+
+void check_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kv_cache, const at::Tensor& kv_scale,
+                  const at::Tensor& seq_offset) {
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(),
+              "hstu_cache_append: k and v must be [tokens, heads_k, dim], of one shape and dtype");
+  TORCH_CHECK(seq_offset.scalar_type() == at::kInt || seq_offset.scalar_type() == at::kLong, "seq_offset must be int32 or int64");
+  held_code(kv_cache);
+  check_held(kv_cache, kv_scale, k);
+  // (they are written where they lie)
+  TORCH_CHECK(kv_cache.is_contiguous() && kv_scale.is_contiguous(), "kv_cache and kv_scale must be contiguous");
+  TORCH_CHECK(!(k.requires_grad() || v.requires_grad()) || !at::GradMode::is_enabled(),
+              "hstu_cache_append: a cache has no gradients (call it under torch.no_grad())");
+}
+
+void hstu_cache_append_op(const at::Tensor& k, const at::Tensor& v, at::Tensor& kv_cache, at::Tensor& kv_scale,
+                          const at::Tensor& seq_offset, const at::Tensor& page_offsets, const at::Tensor& page_ids,
+                          const at::Tensor& last_page_len, const OptTensor& num_target) {
+  check_append(k, v, kv_cache, kv_scale, seq_offset);
+  TORCH_CHECK(k.is_cuda(), "hstu_cache_append: tensors must be CUDA tensors (there is no CPU implementation)");
+  for (const auto* t : {&v, static_cast<const at::Tensor*>(&kv_cache), static_cast<const at::Tensor*>(&kv_scale), &seq_offset,
+                        &page_offsets, &page_ids, &last_page_len})
+    TORCH_CHECK(t->device() == k.device(), "hstu_cache_append: every tensor must be on k's device ", k.device(), ", but one is on ",
+                t->device());
+  c10::cuda::CUDAGuard guard(k.device());
+  const auto it = seq_offset.scalar_type();
+  auto kc = k.contiguous(), vc = v.contiguous(), off = seq_offset.contiguous();
+  auto po = page_offsets.to(it).contiguous(), pi = page_ids.to(it).contiguous(), ll = last_page_len.to(it).contiguous();
+  TORCH_CHECK(off.dim() == 1 && off.numel() >= 2, "seq_offset params error should have at least two element.");
+  const int64_t batch = off.numel() - 1;
+  TORCH_CHECK(batch <= INT32_MAX, "hstu_cache_append: the batch is too large");
+  TORCH_CHECK(po.numel() == off.numel(), "page_offsets must have batch + 1 entries");
+  TORCH_CHECK(ll.numel() >= batch, "last_page_len is shorter than the batch");
+  HstuCacheAppendArgs a;
+  memset(&a, 0, sizeof(a));
+  a.struct_bytes = sizeof(a);
+  at::Tensor tgt;
+  if (num_target.has_value() && num_target->defined()) {
+    TORCH_CHECK(num_target->device() == k.device(), "hstu_cache_append: num_target must be on k's device");
+    tgt = num_target->to(it).contiguous();
+    TORCH_CHECK(tgt.numel() >= batch, "num_target is shorter than the batch");
+    a.num_target = tgt.data_ptr();
+  }
+  a.dtype = dtype_code(k.scalar_type());
+  a.held = held_code(kv_cache);
+  a.page_size = static_cast<int32_t>(kv_cache.size(2));
+  a.block = check_held(kv_cache, kv_scale, k);
+  TORCH_CHECK(k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX, "hstu_cache_append: k is too large");
+  a.heads_k = static_cast<int32_t>(k.size(1));
+  a.dim = static_cast<int32_t>(k.size(2));
+  a.index_bytes = static_cast<int32_t>(off.element_size());
+  a.batch = static_cast<int32_t>(batch);
+  a.total = k.size(0);
+  a.num_pages = kv_cache.size(0);
+  a.num_page_ids = pi.numel();
+  a.k = kc.data_ptr();
+  a.v = vc.data_ptr();
+  a.kv_cache = kv_cache.data_ptr();
+  a.kv_scale = kv_scale.data_ptr();
+  a.seq_offset = off.data_ptr();
+  a.page_offsets = po.data_ptr();
+  a.page_ids = pi.data_ptr();
+  a.last_page_len = ll.data_ptr();
+  const int rc = hstu_cache_append(&a, at::cuda::getCurrentCUDAStream().stream());
+  TORCH_CHECK(rc == 0, "hstu_cache_append: ", hstu_last_error());
+}
+
+void hstu_cache_append_meta(const at::Tensor& k, const at::Tensor& v, at::Tensor& kv_cache, at::Tensor& kv_scale,
+                            const at::Tensor& seq_offset, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                            const OptTensor&) {
+  check_append(k, v, kv_cache, kv_scale, seq_offset);
+}
+
+at::Tensor hstu_paged_8bit(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& kv_cache,
+                           const at::Tensor& kv_scale, int64_t max_seq_len, int64_t max_seq_len_k, double silu_scale,
+                           const OptTensor& seq_offset, const OptTensor& seq_offset_k, const OptTensor& page_offsets,
+                           const OptTensor& page_ids, const OptTensor& last_page_len, const OptTensor& num_target,
+                           OptInt target_group_size, OptDouble alpha, int64_t window, int64_t num_sink, bool deterministic) {
+  for (const auto* t : {&seq_offset, &seq_offset_k, &page_offsets, &page_ids, &last_page_len})
+    TORCH_CHECK(t->has_value() && (*t)->defined() && (*t)->numel() > 0,
+                "hstu_paged_8bit: seq_offset, seq_offset_k, page_offsets, page_ids and last_page_len are required");
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3, "The q should be 3D in jagged layout");
+  TORCH_CHECK(window >= 0, "hstu_paged_8bit: window expect at least 0, but value is ", window);
+  TORCH_CHECK(num_sink >= 0, "hstu_paged_8bit: num_sink expect at least 0, but value is ", num_sink);
+  const bool has_tgt = num_target.has_value() && num_target->defined();
+  TORCH_CHECK(!has_tgt || (target_group_size.value_or(0) > 0 && target_group_size.value_or(0) <= INT32_MAX),
+              "targetGroupSize must be greater than 0 when numTarget is defined");
+  const int held = held_code(kv_cache);
+  const int32_t block = check_held(kv_cache, kv_scale, k);
+  TORCH_CHECK(k.size(0) == q.size(0), "k and v hold the same tokens as q (only their target rows are read)");
+  c10::cuda::CUDAGuard guard(q.device());
+  Prepared pr = prepare(q, k, v, c10::nullopt, c10::nullopt, HSTU_MASK_TRIL, max_seq_len, max_seq_len_k ? max_seq_len_k : max_seq_len,
+                        silu_scale, *seq_offset, *seq_offset_k, c10::nullopt, num_target, has_tgt ? target_group_size : OptInt(0),
+                        alpha, deterministic);
+  for (const at::Tensor* t : {&kv_cache, &kv_scale, &*page_offsets, &*page_ids, &*last_page_len})
+    check_same_device(*t, q, "a tensor of the cache");
+  const auto it = pr.off_q.scalar_type();
+  auto cache = kv_cache.contiguous(), scale = kv_scale.contiguous();
+  auto po = page_offsets->to(it).contiguous(), pi = page_ids->to(it).contiguous(), ll = last_page_len->to(it).contiguous();
+  TORCH_CHECK(po.numel() == pr.off_q.numel(), "page_offsets must have batch + 1 entries");
+  TORCH_CHECK(ll.numel() >= pr.off_q.numel() - 1, "last_page_len is shorter than the batch");
+  HstuPaged8Args a;
+  memset(&a, 0, sizeof(a));
+  a.struct_bytes = sizeof(a);
+  a.held = held;
+  a.block = block;
+  a.window = static_cast<int32_t>(std::min<int64_t>(window, INT32_MAX));
+  a.num_sink = static_cast<int32_t>(std::min<int64_t>(num_sink, INT32_MAX));
+  a.kv_scale = scale.data_ptr();
+  a.paged.struct_bytes = sizeof(a.paged);
+  a.paged.page_size = static_cast<int32_t>(cache.size(2));
+  a.paged.base = pr.a;
+  auto out = at::empty({pr.q.size(0), pr.q.size(1), pr.v.size(2)}, pr.q.options());
+  a.paged.base.out = out.data_ptr();
+  a.paged.kv_cache = cache.data_ptr();
+  a.paged.page_offsets = po.data_ptr();
+  a.paged.page_ids = pi.data_ptr();
+  a.paged.last_page_len = ll.data_ptr();
+  a.paged.num_pages = cache.size(0);
+  a.paged.num_page_ids = pi.numel();
+  uint64_t ws_bytes = 0;
+  int rc = hstu_paged_8bit_fwd_get_workspace_size(&a, &ws_bytes);
+  TORCH_CHECK(rc == 0, "hstu_paged_8bit: ", hstu_last_error());
+  auto ws = at::empty({static_cast<int64_t>(ws_bytes)}, pr.q.options().dtype(at::kByte));
+  rc = hstu_paged_8bit_fwd(&a, ws.data_ptr(), ws_bytes, at::cuda::getCurrentCUDAStream().stream());
+  TORCH_CHECK(rc == 0, "hstu_paged_8bit: ", hstu_last_error());
+  return out;
+}
+
+at::Tensor hstu_paged_8bit_meta(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& kv_cache,
+                                const at::Tensor& kv_scale, int64_t, int64_t, double, const OptTensor&, const OptTensor&,
+                                const OptTensor&, const OptTensor&, const OptTensor&, const OptTensor&, OptInt, OptDouble, int64_t,
+                                int64_t, bool) {
+  TORCH_CHECK(k.dim() == 3, "The k and v should be 3D in jagged layout");
+  held_code(kv_cache);
+  check_held(kv_cache, kv_scale, k);
+  return meta_out(q, v);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(ops_rec, m) {
@@ -880,6 +1036,12 @@ TORCH_LIBRARY_FRAGMENT(ops_rec, m) {
   m.def("hstu_window_backward(Tensor grad, Tensor q, Tensor k, Tensor v, int window, int num_sink=0, int max_seq_len=0, "
         "int max_seq_len_k=0, float silu_scale=0.0, Tensor? seq_offset=None, Tensor? seq_offset_k=None, "
         "Tensor? num_target=None, int? target_group_size=0, float? alpha=1.0) -> (Tensor, Tensor, Tensor)");
+  m.def("hstu_cache_append(Tensor k, Tensor v, Tensor(a!) kv_cache, Tensor(b!) kv_scale, Tensor seq_offset, "
+        "Tensor page_offsets, Tensor page_ids, Tensor last_page_len, Tensor? num_target=None) -> ()");
+  m.def("hstu_paged_8bit(Tensor q, Tensor k, Tensor v, Tensor kv_cache, Tensor kv_scale, int max_seq_len=0, "
+        "int max_seq_len_k=0, float silu_scale=0.0, Tensor? seq_offset=None, Tensor? seq_offset_k=None, "
+        "Tensor? page_offsets=None, Tensor? page_ids=None, Tensor? last_page_len=None, Tensor? num_target=None, "
+        "int? target_group_size=0, float? alpha=1.0, int window=0, int num_sink=0, bool deterministic=False) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(ops_rec, CUDA, m) {
@@ -894,6 +1056,8 @@ TORCH_LIBRARY_IMPL(ops_rec, CUDA, m) {
   m.impl("in_linear_silu_backward", TORCH_FN(in_linear_silu_bwd));
   m.impl("hstu_window", TORCH_FN(hstu_window));
   m.impl("hstu_window_backward", TORCH_FN(hstu_window_backward));
+  m.impl("hstu_cache_append", TORCH_FN(hstu_cache_append_op));
+  m.impl("hstu_paged_8bit", TORCH_FN(hstu_paged_8bit));
 }
 
 TORCH_LIBRARY_IMPL(ops_rec, Autograd, m) {
@@ -914,4 +1078,6 @@ TORCH_LIBRARY_IMPL(ops_rec, Meta, m) {
   m.impl("in_linear_silu_backward", TORCH_FN(in_linear_silu_bwd_meta));
   m.impl("hstu_window", TORCH_FN(hstu_window_meta));
   m.impl("hstu_window_backward", TORCH_FN(hstu_window_backward_meta));
+  m.impl("hstu_cache_append", TORCH_FN(hstu_cache_append_meta));
+  m.impl("hstu_paged_8bit", TORCH_FN(hstu_paged_8bit_meta));
 }

@@ -37,8 +37,9 @@ def window_mask(len_q, len_k, tgt, group, window, sink, device="cpu"):
     return see
 
 
-def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False):
-    """One sequence: q [lq, hq, d], k, v [lk, hk, .] -> {"out": (value, tolerance)} and with grad also dq, dk, dv."""
+def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=False):
+    """One sequence: q [lq, hq, d], k, v [lk, hk, .] -> {"out": (value, tolerance)} and with grad also dq, dk, dv.
+    staged: k and v may have been rounded to the element type on their way (one rounding each)."""
     u = torch.finfo(dtype).eps / 2
     hq, hk = q.shape[1], k.shape[1]
     q, k, v = (t.double().transpose(0, 1) for t in (q, k, v))                     # [heads, rows, dim]
@@ -46,12 +47,14 @@ def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False):
     f32, tiny = 2.0 ** -24, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
     x = alpha * q @ kk.transpose(1, 2)
     xerr = (q.shape[2] + 4) * f32 * abs(alpha) * (q.abs() @ kk.abs().transpose(1, 2))
+    if staged:
+        xerr = xerr + (u + f32) * abs(alpha) * (q.abs() @ kk.abs().transpose(1, 2))
     sg = torch.sigmoid(x)
     approx = x.abs() * 2.0 ** -12 if tanh else (x * sg).abs() * 2.0 ** -20
     perr = torch.where(see, scale * (1.1 * (xerr + approx) + (u + 4 * f32) * (x * sg).abs()) + tiny, 0.0)
     p = torch.where(see, x * sg * scale, 0.0)
     out = p @ vv
-    n = k.shape[1] + 4
+    n = k.shape[1] + 4 + (u / f32 + 1 if staged else 0)
     got = {"out": (out, u * out.abs() + perr @ vv.abs() + n * f32 * (p.abs() @ vv.abs()))}
     if grad is not None:
         g = grad.double().transpose(0, 1)
