@@ -37,6 +37,9 @@ cudaError_t launch_in_linear_silu_bwd(const LinSiluParams& shape, const void* x,
 cudaError_t launch_paged_gather(const KParams& p, const void* kv_cache, const void* k_in, const void* v_in,
                                 void* k_out, void* v_out, long long capacity, long long num_pages,
                                 long long num_page_ids, int dtype, cudaStream_t stream);
+bool decode8_supported(const KParams& p, int dtype);
+uint64_t decode8_workspace(const KParams& p);
+cudaError_t launch_decode8(const KParams& p, int dtype, void* workspace, cudaStream_t stream);
 cudaError_t launch_append(const HstuCacheAppendArgs& a, cudaStream_t stream);
 }  // namespace hstu
 
@@ -460,13 +463,38 @@ int plan_paged8(const HstuPaged8Args* a, PagedPlan* pl) {
 }
 }  // namespace
 
+// What the kernels are told of a call: its own tensors, nothing staged.
+static hstu::KParams paged8_params(const HstuPaged8Args* args, const PagedPlan& pl) {
+  const HstuPagedArgs* a = &args->paged;
+  hstu::KParams p = to_params(&pl.fwd, nullptr, 0);
+  set_window(&p, args->window, args->num_sink);
+  p.q = a->base.q;
+  p.out = a->base.out;
+  p.page_offsets = a->page_offsets;
+  p.page_ids = a->page_ids;
+  p.last_page_len = a->last_page_len;
+  p.page_size = a->page_size;
+  p.num_pages = a->num_pages;
+  p.num_page_ids = a->num_page_ids;
+  p.kv_cache = a->kv_cache;
+  p.kv_scale = static_cast<const float*>(args->kv_scale);
+  p.held = args->held;
+  p.scale_block = args->block;
+  p.k_new = a->base.k;
+  p.v_new = a->base.v;
+  return p;
+}
+static uint64_t paged8_workspace(const hstu::KParams& p, const PagedPlan& pl) {
+  return hstu::decode8_supported(p, pl.fwd.dtype) ? hstu::decode8_workspace(p) : pl.fwd_bytes + 2 * pl.stage_bytes;
+}
+
 int hstu_paged_8bit_fwd_get_workspace_size(const HstuPaged8Args* args, uint64_t* workspace_bytes) {
   g_err[0] = 0;
   if (!workspace_bytes) return fail(HSTU_E_NULL, "workspace_bytes is null");
   PagedPlan pl;
   const int rc = plan_paged8(args, &pl);
   if (rc) return rc;
-  *workspace_bytes = pl.fwd_bytes + 2 * pl.stage_bytes;
+  *workspace_bytes = paged8_workspace(paged8_params(args, pl), pl);
   return HSTU_OK;
 }
 
@@ -482,30 +510,27 @@ int hstu_paged_8bit_fwd(const HstuPaged8Args* args, void* workspace, uint64_t wo
     return fail(HSTU_E_NULL, "kv_cache / kv_scale / page_offsets / page_ids / last_page_len is null");
   if (reinterpret_cast<uintptr_t>(args->kv_scale) & 3u) return fail(HSTU_E_PARAM, "kv_scale must be 4-byte aligned");
   if (b->total_q > 0 && (!b->q || !b->out || !b->k || !b->v)) return fail(HSTU_E_NULL, "q / k / v / out is null");
-  const uint64_t need = pl.fwd_bytes + 2 * pl.stage_bytes;
+  hstu::KParams p = paged8_params(args, pl);
+  const uint64_t need = paged8_workspace(p, pl);
   if (!workspace) return fail(HSTU_E_WORKSPACE, "workspace is null (%llu bytes needed)", (unsigned long long)need);
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSTU_E_WORKSPACE, "workspace must be 256-byte aligned");
   if (workspace_bytes < need)
     return fail(HSTU_E_WORKSPACE, "workspace has %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
                 (unsigned long long)need);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
+  if (hstu::decode8_supported(p, pl.fwd.dtype)) {
+    DeviceInfo dev;
+    rc = device_info(&dev);
+    if (rc) return rc;
+    if (dev.major != 10) return fail(HSTU_E_ARCH, "this library is built for sm_100a only; device has compute capability %d.x", dev.major);
+    const cudaError_t e = hstu::launch_decode8(p, pl.fwd.dtype, workspace, stream);
+    return e == cudaSuccess ? HSTU_OK : fail(HSTU_E_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+  }
   char* base = static_cast<char*>(workspace);
   pl.fwd.q = b->q;
   pl.fwd.out = b->out;
   pl.fwd.k = base + pl.fwd_bytes;
   pl.fwd.v = base + pl.fwd_bytes + pl.stage_bytes;
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  hstu::KParams p = to_params(&pl.fwd, nullptr, 0);
-  set_window(&p, args->window, args->num_sink);
-  p.page_offsets = a->page_offsets;
-  p.page_ids = a->page_ids;
-  p.last_page_len = a->last_page_len;
-  p.page_size = a->page_size;
-  p.num_pages = a->num_pages;
-  p.num_page_ids = a->num_page_ids;
-  p.kv_cache = a->kv_cache;
-  p.kv_scale = static_cast<const float*>(args->kv_scale);
-  p.held = args->held;
-  p.scale_block = args->block;
   const cudaError_t e = hstu::launch_paged_gather(p, a->kv_cache, b->k, b->v, base + pl.fwd_bytes, base + pl.fwd_bytes + pl.stage_bytes,
                                                   pl.capacity, a->num_pages, a->num_page_ids, pl.fwd.dtype, stream);
   if (e != cudaSuccess) return fail(HSTU_E_CUDA, "gather launch: %s", cudaGetErrorString(e));

@@ -209,8 +209,8 @@ HSTU_HD int paged_full_tiles(const void* offq, const void* offk, const void* tgt
 // hstu_paged: the page table of sequence b must describe exactly the cached part of its keys,
 // (pages - 1) * page_size + last_page_len == len_k - num_target, with page ids inside the cache
 // (the reference golden asserts the former, hstu_forward_v1/test/pytest/common.py:286).
-HSTU_HD unsigned check_pages(const KParams& p, int b) {
-  if (!p.page_offsets) return 0;
+// (the number of pages and rows only: not the ids)
+HSTU_HD unsigned check_page_count(const KParams& p, int b) {
   const long long pg0 = load_index(p.page_offsets, p.index_bytes, b), pg1 = load_index(p.page_offsets, p.index_bytes, b + 1);
   if (pg0 < 0 || pg1 < pg0 || pg1 > p.num_page_ids) return HSTU_ST_BAD_PAGES;
   const long long last = p.last_page_len ? load_index(p.last_page_len, p.index_bytes, b) : p.page_size;
@@ -219,7 +219,12 @@ HSTU_HD unsigned check_pages(const KParams& p, int b) {
   if (t < 0) t = 0;
   const long long pages = pg1 - pg0;
   const long long cached = pages > 0 ? (pages - 1) * p.page_size + last : 0;
-  if (last < 0 || last > p.page_size || (pages > 0 && last == 0) || cached != (k1 - k0) - t) return HSTU_ST_BAD_PAGES;
+  return last < 0 || last > p.page_size || (pages > 0 && last == 0) || cached != (k1 - k0) - t ? HSTU_ST_BAD_PAGES : 0;
+}
+HSTU_HD unsigned check_pages(const KParams& p, int b) {
+  if (!p.page_offsets) return 0;
+  if (check_page_count(p, b)) return HSTU_ST_BAD_PAGES;
+  const long long pg0 = load_index(p.page_offsets, p.index_bytes, b), pg1 = load_index(p.page_offsets, p.index_bytes, b + 1);
   bool bad = false;   // (no early return: several reads are in flight)
 #pragma unroll 4
   for (long long s = pg0; s < pg1; ++s) {

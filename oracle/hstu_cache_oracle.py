@@ -77,11 +77,13 @@ def paged(q, k, v, kv_cache, kv_scale, max_seq_len, max_seq_len_k=0, silu_scale=
         mine = ids[po[b]:po[b + 1]]
         rows = slice(off[b], off[b + 1])
         kv = []
+        unit = torch.ones(n + t, k.shape[1], device=q.device)
+        unit[:n] = kv_scale[mine, 1].repeat_interleave(page // per_page, 1).flatten(0, 1)[:n]
         for which, new in ((0, k), (1, v)):
             x = kv_cache[mine, which].float().double().flatten(0, 1) * \
                 kv_scale[mine, which].double().repeat_interleave(page // per_page, 1).flatten(0, 1)[..., None]
             kv.append(torch.cat((x[:n], new[off[b + 1] - t:off[b + 1]].double())))
         see = WO.window_mask(off[b + 1] - off[b], off_k[b + 1] - off_k[b], t, target_group_size, window, num_sink, q.device)
-        one = WO.attention(q[rows], *kv, see, alpha, silu_scale or 1.0 / max_seq_len, q.dtype, tanh=tanh, staged=True)
+        one = WO.attention(q[rows], *kv, see, alpha, silu_scale or 1.0 / max_seq_len, q.dtype, tanh=tanh, staged=True, unit=unit)
         out[rows], tol[rows] = one["out"]
     return out, tol

@@ -37,9 +37,15 @@ def window_mask(len_q, len_k, tgt, group, window, sink, device="cpu"):
     return see
 
 
-def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=False):
+def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=False, unit=None):
     """One sequence: q [lq, hq, d], k, v [lk, hk, .] -> {"out": (value, tolerance)} and with grad also dq, dk, dv.
-    staged: k and v may have been rounded to the element type on their way (one rounding each)."""
+    staged: k and v may have been rounded to the element type on their way, one rounding each: u relative, and below the type's
+    normal range half of its smallest step.  Such a cache's blocks may differ by any power of two, and that shows how tensor
+    cores add: the products of 16 keys and the accumulator are shifted to the largest exponent among them and cut off some 25
+    bits below it, and a P of zero has the exponent of one there.  So a masked value v costs the rows that do not see it up to
+    2^-25 |v| for its group of 16 keys (seen as errors that are multiples of 2^-17 beside hidden values of 256).
+    unit: [keys, hk], the scales of the values (value = number * scale).  A kernel may round P * scale instead of P, to fp16
+    relative to the row's largest: half a smallest step is then 2^-25 of that largest, for every number."""
     u = torch.finfo(dtype).eps / 2
     hq, hk = q.shape[1], k.shape[1]
     q, k, v = (t.double().transpose(0, 1) for t in (q, k, v))                     # [heads, rows, dim]
@@ -48,14 +54,20 @@ def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=F
     x = alpha * q @ kk.transpose(1, 2)
     xerr = (q.shape[2] + 4) * f32 * abs(alpha) * (q.abs() @ kk.abs().transpose(1, 2))
     if staged:
-        xerr = xerr + (u + f32) * abs(alpha) * (q.abs() @ kk.abs().transpose(1, 2))
+        xerr = xerr + (u + f32) * abs(alpha) * (q.abs() @ kk.abs().transpose(1, 2)) + tiny * abs(alpha) * q.abs().sum(2, keepdim=True)
     sg = torch.sigmoid(x)
     approx = x.abs() * 2.0 ** -12 if tanh else (x * sg).abs() * 2.0 ** -20
     perr = torch.where(see, scale * (1.1 * (xerr + approx) + (u + 4 * f32) * (x * sg).abs()) + tiny, 0.0)
     p = torch.where(see, x * sg * scale, 0.0)
     out = p @ vv
-    n = k.shape[1] + 4 + (u / f32 + 1 if staged else 0)
-    got = {"out": (out, u * out.abs() + perr @ vv.abs() + n * f32 * (p.abs() @ vv.abs()))}
+    n = k.shape[1] + 4
+    got = {"out": (out, u * out.abs() + perr @ vv.abs() + (n * f32 + (u if staged else 0)) * (p.abs() @ vv.abs()) +
+                   (tiny * p.abs().sum(2, keepdim=True) + (n // 16 + 1) * 2.0 ** -25 * vv.abs().amax(1, keepdim=True)
+                    if staged and vv.shape[1] else 0.0))}
+    if unit is not None and vv.shape[1] and dtype == torch.float16:
+        scales = unit.double().t().repeat_interleave(hq // hk, 0)
+        most = (p.abs() * scales[:, None, :]).amax(2, keepdim=True)
+        got["out"] = got["out"][0], got["out"][1] + 2.0 ** -25 * most * (vv.abs() / scales[..., None]).sum(1, keepdim=True)
     if grad is not None:
         g = grad.double().transpose(0, 1)
         dp = g @ vv.transpose(1, 2)

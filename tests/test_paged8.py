@@ -401,3 +401,36 @@ def test_tensors_that_start_anywhere():
     t = table(args) | {n: shifted[n] for n in ("k", "v", "kv_cache")}
     assert cabi.hstu_cache_append(**t, return_status=True) == 0
     assert torch.equal(t["kv_cache"].cpu().view(torch.uint8), cache.view(torch.uint8)) and torch.equal(t["kv_scale"].cpu(), scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("new", [1, 30])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 300.0])
+def test_paged_small_numbers_and_uneven_scales(dtype, new, size):
+    """Numbers below e4m3's normal range only, and scales that differ by 2^20 from block to block."""
+    args = make([200, 77, 640], [new] * 3, None, 2, 2, 64, dtype, page=64, block=16, seed=12)
+    raw = args["kv_cache"].view(torch.uint8)
+    raw[:, 0] = (raw[:, 0] & 0x87)                   # keys: at most 7 * 2^-9
+    raw[::2, 1] &= 0x87
+    args["kv_scale"][:, 0] *= 64
+    args["kv_scale"][:, 1] *= torch.exp2(torch.randint(-10, 11, args["kv_scale"][:, 1].shape, generator=torch.Generator().manual_seed(1)).float())
+    args["q"] = args["q"] * size
+    check_paged(args)
+    check_paged(args, 100, 20)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("new", [1, 30])
+def test_paged_keeps_what_is_not_finite(dtype, new):
+    args = make([200, 77], [new] * 2, None, 2, 2, 64, dtype, page=64, block=32, seed=13)
+    want, tol = CO.paged(**on_gpu(args))
+    page = int(args["page_ids"][0])
+    args["kv_cache"].view(torch.uint8)[page, 1, 3, 0, 5] = 0x7f      # a value: its column of head 0 of the first user
+    args["kv_cache"].view(torch.uint8)[page, 0, 4, 1, 6] = 0xff      # a key: everything of head 1
+    out = cabi.hstu_paged_8bit_forward(**on_gpu(args))
+    assert out[:new, 0, 5].isnan().all() and out[:new, 1].isnan().all()
+    out[:new, 0, 5], out[:new, 1] = 0, 0
+    want[:new, 0, 5], want[:new, 1] = 0, 0
+    assert ((out.double() - want).abs() <= tol + 1e-9).all()
