@@ -3,28 +3,32 @@
 //
 // HBM-bound: a decode step reads every visible cached row once, at one byte per element (128 users of 200 - 2048 rows, 8 heads
 // of 128: 294 MB, 46 us), and there is next to nothing to compute per byte.  So nothing is staged: a warp streams tiles of 16 keys
-// through a ring of its own in shared memory (cp.async, four stages in flight, no barrier of the CTA in the loop), turns the 8-bit
-// numbers into 16-bit ones in registers where the matrix instructions want them, and keeps its 16 rows of the output in registers.
+// through a ring of its own in shared memory (cp.async, four stages, no barrier of the CTA in the loop; TMA boxes of 16 rows of 128
+// bytes, one for keys and one for values, came in at 3.4 TB/s at most, whatever the number of CTAs), turns the 8-bit numbers
+// into 16-bit ones in registers where the matrix instructions want them, and keeps its 16 rows of the output in registers.
 // There is no softmax: partial outputs of any split of the keys add up, first over the four warps of a CTA, then - where a
 // sequence has more keys than a CTA takes - over CTAs: each leaves its partial sums in the workspace, and the last one to arrive
 // adds them in the order of the keys (the same bits every time).
 //
-// The rows of a call are (query, head of the group) pairs of one key head, 16 at a time: grouped heads share the cache's reads.
-//   S = Q.K^T      mma.sync m16n8k16 in fp16: e4m3 and int8 numbers are exact there, one conversion per pair; bf16 queries are
-//                  scaled by a power of two per row (their largest element to [1, 2)), which keeps all 8 bits of every element
-//                  that counts.  A thread's 16 bytes of a key are contiguous; the same permutation of the contraction is applied
-//                  to Q.  The key's scale, alpha and the row's power of two multiply the 32-bit score.
-//   P              silu(x) * (scale of the value's block), rounded to 16 bits once: in bf16 as it is; in fp16 divided by a power
-//                  of two per row that follows the largest P so far (raised, and the output rescaled, when P outgrows 2^14),
-//                  since neither scores nor scales keep P inside fp16's narrow range
-//   O += P.V       V is read with ldmatrix.trans as pairs of bytes, which puts the even and the odd columns of the head into
-//                  two B operands.  bf16: the bits of an e4m3 number, shifted into place, are the number times 2^-120 (and
-//                  exact, the small ones as subnormals); P carries 2^60 of what is missing, the output the rest.
+// The rows of a call are (query, head of the group) pairs of one key head, 8 kN at a time: grouped heads share the cache's reads.
+// Both products have the cache as their A operand (16 keys, 16 columns of the head) and the rows as the 8 columns of B, so that
+// a number is converted once for all rows and one row does not cost what sixteen do.  All operands are fp16, whatever the call's
+// type: e4m3 and int8 numbers are exact there, one conversion per pair (bf16 has no such instruction, and five integer
+// operations per pair made the kernel issue-bound: 875 instructions a tile and 104 us above), and P has three bits more.
+//   S^T = K.Q^T    bf16 queries are divided by a power of two per row (their largest element to [1, 2)), which keeps all 8 bits
+//                  of every element that counts.  A thread's 16 bytes of a key are contiguous; the same permutation of the
+//                  contraction is applied to Q.  The key's scale, alpha and the row's power of two multiply the 32-bit score.
+//   P              silu(x) * (scale of the value's block), rounded once, divided by a power of two per row that follows the
+//                  largest P so far (raised, and the output rescaled, when P outgrows 2^14), since neither scores nor scales
+//                  keep P inside fp16's narrow range
+//   O^T += V^T.P^T V is read with ldmatrix.trans as pairs of bytes; the even columns of the head are the rows 0-7 of A, the odd
+//                  ones the rows 8-15.  P changes from accumulator to operand with movmatrix.
 // tcgen05 would need M = 128 rows and its operands in shared memory in 16 bits: the conversion would go through shared memory
 // twice for a tile of which one row counts.
 #include <type_traits>
 
 #include "hstu_held.cuh"
+#include "ptx_sm100.cuh"
 
 namespace hstu {
 
@@ -32,16 +36,17 @@ namespace {
 
 constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16;      // keys of a tile
-constexpr int kDecRows = 16;      // rows of a CTA
 constexpr int kDecMostTiles = 128;   // of a CTA
 
-template <int D> struct DecCfg {
+template <int D, int kN> struct DecCfg {
+  static constexpr int kRows = 8 * kN;                          // rows of a CTA
   static constexpr int kStages = 4;
   static constexpr int kTile = kDecKeys * D;                    // bytes of K (V) of a tile
-  static constexpr int kStage = 2 * kTile + 2 * kDecKeys * 4;   // K, V and their scales
+  static constexpr int kStage = 2 * kTile;
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kSmem = kDecWarps * kRing;
-  static_assert(kSmem >= kDecWarps * kDecRows * D * 4, "the rings hold the warps' partial outputs at the end");
+  static constexpr int kScales = kDecWarps * kStages * 2 * kDecKeys * 4;
+  static constexpr int kSmem = kDecWarps * kRing + kScales;
+  static_assert(kDecWarps * kRing >= kDecWarps * kRows * D * 4, "the rings hold the warps' partial outputs at the end");
 };
 
 struct DecParams {
@@ -52,9 +57,8 @@ struct DecParams {
   int block_shift;      // log2 of a scale's block, 4 at most (a tile has one scale from there on)
 };
 
-__device__ __forceinline__ uint32_t smem_of(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {   // (the rest of the 16 becomes zeros)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
@@ -65,50 +69,35 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
-template <typename T> __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+// An 8 x 8 matrix of halves, a row's pair per thread -> its transpose.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-// The bytes 0, 1 (2, 3) of w as two halves.
-template <typename H, bool kHigh> __device__ __forceinline__ uint32_t halves_of(uint32_t w) {
+// The four numbers of w as two pairs of halves.
+template <typename H> __device__ __forceinline__ void to_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (std::is_same<H, E4m3>::value) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(kHigh ? w >> 16 : w & 0xffffu), __NV_E4M3);
-    return static_cast<uint32_t>(h.x) | (static_cast<uint32_t>(h.y) << 16);
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
   } else {
     // 0x6400 + (v + 128) is 1024 + 128 + v
-    const uint32_t u = __byte_perm(w ^ 0x80808080u, 0x64646464u, kHigh ? 0x4342 : 0x4140);
-    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&u), __floats2half2_rn(1152.f, 1152.f));
-    return *reinterpret_cast<const uint32_t*>(&d);
+    const uint32_t u = w ^ 0x80808080u, ul = __byte_perm(u, 0x64646464u, 0x4140), uh = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 off = __floats2half2_rn(1152.f, 1152.f);
+    const __half2 l = __hsub2(*reinterpret_cast<const __half2*>(&ul), off), h = __hsub2(*reinterpret_cast<const __half2*>(&uh), off);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
   }
-}
-// The bytes 0, 2 (kOdd: 1, 3) of w as a pair of the call's type, times 2^-120 where it is bf16 and the cache e4m3.
-template <typename H, typename T, bool kOdd> __device__ __forceinline__ uint32_t pair_of(uint32_t w) {
-  if constexpr (std::is_same<T, __half>::value) {
-    return halves_of<H, false>(__byte_perm(w, 0u, kOdd ? 0x4431 : 0x4420));
-  } else if constexpr (std::is_same<H, E4m3>::value) {
-    return kOdd ? ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u) : ((w << 4) & 0x07f007f0u) | ((w << 8) & 0x80008000u);
-  } else {
-    // 0x4b000000 + (v + 128) is 2^23 + 128 + v
-    const uint32_t u = w ^ 0x80808080u;
-    const float lo = __uint_as_float(__byte_perm(u, 0x4b000000u, kOdd ? 0x7441 : 0x7440)) - 8388736.f;
-    const float hi = __uint_as_float(__byte_perm(u, 0x4b000000u, kOdd ? 0x7443 : 0x7442)) - 8388736.f;
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-// Whether a byte of w is an e4m3 NaN, which shifted into a bf16's place would be the number 480.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-// pair_of() of bytes that may be NaN.
-template <bool kOdd> __device__ __forceinline__ uint32_t pair_with_nan(uint32_t w) {
-  const uint32_t v = pair_of<E4m3, __nv_bfloat16, kOdd>(w), nan = kOdd ? nan_bytes(w) : nan_bytes(w) << 8;
-  return v | ((nan & 0x8000u) ? 0x7fffu : 0u) | ((nan & 0x80000000u) ? 0x7fff0000u : 0u);
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -119,16 +108,7 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
 
 // Clears the status word and the counters; the attention kernel, launched with programmatic stream serialization, streams
 // keys meanwhile and waits before it touches either.
@@ -139,18 +119,17 @@ __global__ void hstu_decode8_init_kernel(uint32_t* header, uint32_t* counters, l
   if (i < n) counters[i] = 0;
 }
 
-template <int D, typename T, typename H, bool kWin>
+template <int D, int kN, typename T, typename H, bool kWin>
 __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecParams d) {
-  using C = DecCfg<D>;
+  using C = DecCfg<D, kN>;
   using Mask = MaskOf<kWin>;
   const KParams& p = d.f;
   extern __shared__ __align__(128) uint8_t ring_of_all[];
-  __shared__ long long s_row[kDecMostTiles];     // first row of the tile's keys in the cache, -1: no such page
-  __shared__ long long s_scale[kDecMostTiles];   // its place in the scales
+  __shared__ long long s_row[kDecMostTiles];     // where the tile's keys start in the cache, -1: no such page
+  __shared__ long long s_scale[kDecMostTiles];   // where its scales start
   __shared__ int s_last;
-  constexpr bool kHalf = std::is_same<T, __half>::value;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const int b = blockIdx.x / p.hk, hk = blockIdx.x - b * p.hk, split = blockIdx.y, r_first = blockIdx.z * kDecRows;
+  const int b = blockIdx.x / p.hk, hk = blockIdx.x - b * p.hk, split = blockIdx.y, r_first = blockIdx.z * C::kRows;
 
   const SeqInfo s = load_seq(p, b);
   const int ratio = p.gqa_ratio, rows = s.lq * ratio - r_first;   // rows of this block, the group's heads inside a query
@@ -170,7 +149,7 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
       atomicOr(p.ws_header, st);
     }
   }
-  const int q_lo = r_first / ratio, q_n = (min(rows, kDecRows) + r_first + ratio - 1) / ratio - q_lo;   // the block's queries
+  const int q_lo = r_first / ratio, q_n = (min(rows, C::kRows) + r_first + ratio - 1) / ratio - q_lo;   // the block's queries
   const KeyTiles tiles = rows > 0 ? Mask::tiles(p, s, q_lo, q_n, kDecKeys) : KeyTiles{0, 0, 0};
   const int active = max(1, (tiles.n + d.tiles - 1) / d.tiles);   // CTAs that share this block's keys
   const int t0 = split * d.tiles, t1 = min(tiles.n, t0 + d.tiles);
@@ -179,41 +158,49 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
     return;
   }
   // The places of this CTA's tiles: a tile lies in one page.
-  const int per_page = p.page_size / p.scale_block;
+  const int per_page = p.page_size / p.scale_block, row_bytes = p.hk * p.dqk;
   for (int i = tid; i < t1 - t0; i += kDecThreads) {
     const int key = key_of_tile(tiles, t0 + i, kDecKeys), slot = key / p.page_size, in_page = key - slot * p.page_size;
     const long long pid = pg0 + slot < pg1 ? load_index(p.page_ids, p.index_bytes, pg0 + slot) : -1;
     const bool ok = pid >= 0 && pid < p.num_pages;
-    s_row[i] = ok ? pid * 2 * p.page_size + in_page : -1;
-    s_scale[i] = ok ? (pid * 2 * per_page + in_page / p.scale_block) * p.hk + hk : -1;
+    s_row[i] = ok ? (pid * 2 * p.page_size + in_page) * row_bytes : -1;
+    s_scale[i] = ok ? (pid * 2 * per_page + in_page / p.scale_block) * p.hk : 0;
   }
   __syncthreads();
 
-  uint8_t* ring = ring_of_all + warp * C::kRing;
-  const uint32_t ring_at = smem_of(ring);
-  const uint8_t* cache = static_cast<const uint8_t*>(p.kv_cache);
-  const long long row_bytes = static_cast<long long>(p.hk) * p.dqk;
-  constexpr int kChunks = D / 16;   // 16-byte chunks of a row
-  // Requests tile t0 + i into stage i's slot: rows behind the last cached one and chunks behind the head read as zeros.
+  float* const scales_of_mine = reinterpret_cast<float*>(ring_of_all + kDecWarps * C::kRing) + warp * C::kStages * 2 * kDecKeys;
+  const uint32_t ring_at = ptx::smem_u32(ring_of_all) + warp * C::kRing;
+  constexpr int kChunks = D / 16, kAtOnce = 32 / kChunks;   // 16-byte chunks of a row, rows that 32 lanes copy at once
+  const int my_row = lane / kChunks, my_chunk = lane % kChunks;
+  const int bytes = my_chunk * 16 < p.dqk ? 16 : 0;         // (chunks behind the head read as zeros)
+  const uint8_t* const from_lane = static_cast<const uint8_t*>(p.kv_cache) + my_row * row_bytes + hk * p.dqk + (bytes ? my_chunk * 16 : 0);
+  const long long to_v = static_cast<long long>(p.page_size) * row_bytes;
+  const int to_rows = kAtOnce * row_bytes;
+  const float* scale_from = p.kv_scale + hk + ((lane < 16 ? 0 : per_page) + ((lane & 15) >> d.block_shift)) * static_cast<long long>(p.hk);
+  // Requests tile t0 + i into stage i's slot; rows behind the last cached one read as zeros.  (Chunks are permuted so that the
+  // pieces of 16 bytes eight lanes read at once fall on different banks.)
   auto request = [&](int i, int stage) {
-    const long long row0 = s_row[i];
-    const int left = s.lk - key_of_tile(tiles, t0 + i, kDecKeys);
+    const long long at = s_row[i];
+    const int left = at < 0 ? 0 : s.lk - key_of_tile(tiles, t0 + i, kDecKeys);
     const uint32_t to = ring_at + stage * C::kStage;
+    const uint8_t* k_at = from_lane + (at < 0 ? 0 : at);
+    const uint8_t* v_at = k_at + to_v;
+    auto copy = [&](auto whole) {
 #pragma unroll
-    for (int u = 0; u < kDecKeys * kChunks / 32; ++u) {
-      const int at = u * 32 + lane, r = at / kChunks, ch = at % kChunks;
-      const bool on = row0 >= 0 && r < left && ch * 16 < p.dqk;
-      const uint8_t* k_from = on ? cache + (row0 + r) * row_bytes + hk * p.dqk + ch * 16 : cache;
-      const uint8_t* v_from = on ? k_from + p.page_size * row_bytes : cache;
-      // (the chunks are permuted so that eight lanes' 16 bytes of a load fall on different banks)
-      const int k_ch = D == 128 ? ch ^ ((r & 1) << 2) : ch, v_ch = D == 128 ? ch ^ (r & 7) : ch ^ ((r >> 1) & 3);
-      cp16(to + r * D + k_ch * 16, k_from, on);
-      cp16(to + C::kTile + r * D + v_ch * 16, v_from, on);
-    }
-    const int r = lane & 15;
-    const bool on = row0 >= 0 && r < left;
-    cp4(to + 2 * C::kTile + lane * 4,
-        on ? p.kv_scale + s_scale[i] + ((lane < 16 ? 0 : per_page) + (r >> d.block_shift)) * static_cast<long long>(p.hk) : p.kv_scale, on);
+      for (int u = 0; u < kDecKeys / kAtOnce; ++u) {
+        const int r = u * kAtOnce + my_row;
+        const int k_ch = D == 128 ? my_chunk ^ ((r & 1) << 2) : my_chunk, v_ch = D == 128 ? my_chunk ^ (r & 7) : my_chunk ^ ((r >> 1) & 3);
+        const bool on = decltype(whole)::value || r < left;
+        cp16(to + r * D + k_ch * 16, on ? k_at : from_lane, on ? bytes : 0);
+        cp16(to + C::kTile + r * D + v_ch * 16, on ? v_at : from_lane, on ? bytes : 0);
+        k_at += to_rows;
+        v_at += to_rows;
+      }
+    };
+    if (left >= kDecKeys) copy(std::true_type{});
+    else copy(std::false_type{});
+    const bool on = (lane & 15) < left;
+    cp4(ptx::smem_u32(scales_of_mine + stage * 2 * kDecKeys + lane), on ? scale_from + s_scale[i] : p.kv_scale, on);
   };
   const int mine = (t1 - t0 - warp + kDecWarps - 1) / kDecWarps;   // tiles of this warp: warp, warp + 4, ..
 #pragma unroll
@@ -222,15 +209,17 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
-  // Q: rows g and g + 8 of the block; of each 64 columns the 16 from 16 c on.
-  uint32_t qa[D / 16][4];
-  float factor[2];   // alpha and the power of two a row was divided by
+  // Q: this thread's row of each eight, of each 64 columns the 16 from 16 c on.
+  uint32_t qb[kN][D / 16][2];
+  float factor[kN][2];   // of the rows 2 c and 2 c + 1: alpha and the power of two a row was divided by
+  int query[kN][2];      // and their queries
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = g + 8 * h;
+  for (int n = 0; n < kN; ++n) {
+    const int r = 8 * n + g;
     const bool on = r < rows;
-    const T* from = static_cast<const T*>(p.q) + ((s.q0 + (on ? (r_first + r) / ratio : 0)) * p.hq + hk * ratio + (on ? (r_first + r) % ratio : 0)) * p.dqk;
-    uint32_t w[D / 8];   // the thread's pairs, in memory's order
+    const int row = on ? r_first + r : 0;
+    const T* from = static_cast<const T*>(p.q) + ((s.q0 + row / ratio) * p.hq + hk * ratio + row % ratio) * p.dqk;
+    uint32_t w[D / 8];   // pairs in memory's order
 #pragma unroll
     for (int blk = 0; blk < D / 64; ++blk) {
       const bool in = on && blk * 64 + 16 * c < p.dqk;
@@ -240,179 +229,160 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
         w[blk * 8 + 4 * u] = v.x, w[blk * 8 + 4 * u + 1] = v.y, w[blk * 8 + 4 * u + 2] = v.z, w[blk * 8 + 4 * u + 3] = v.w;
       }
     }
-    factor[h] = p.alpha;
-    if (!kHalf) {
-      uint32_t top = 0;   // the largest exponent of the row (its bits: of finite values; an infinity keeps the row as it is)
+    float f = p.alpha;
+    if constexpr (!std::is_same<T, __half>::value) {
+      uint32_t top = 0;   // the largest exponent of the row; an infinity or NaN leaves the row as it is
 #pragma unroll
       for (int u = 0; u < D / 8; ++u) top = max(top, max(w[u] & 0x7f80u, (w[u] >> 16) & 0x7f80u));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const int e = top == 0x7f80u || top == 0 ? 0 : static_cast<int>(top >> 7) - 127;
-      // (in two steps: 2^-e alone may lie outside of the normal range)
-      const float down1 = __uint_as_float(static_cast<uint32_t>(127 - e / 2) << 23), down2 = __uint_as_float(static_cast<uint32_t>(127 - (e - e / 2)) << 23);
-      const float up1 = __uint_as_float(static_cast<uint32_t>(127 + e / 2) << 23), up2 = __uint_as_float(static_cast<uint32_t>(127 + (e - e / 2)) << 23);
-      factor[h] = p.alpha * up1 * up2;
+      const float d1 = power_of_two(-(e / 2)), d2 = power_of_two(-(e - e / 2));   // (2^-e itself may lie outside of fp32's normal range)
+      f = p.alpha * power_of_two(e / 2) * power_of_two(e - e / 2);
 #pragma unroll
-      for (int u = 0; u < D / 8; ++u) {
-        const float lo = __uint_as_float(w[u] << 16) * down1 * down2, hi = __uint_as_float(w[u] & 0xffff0000u) * down1 * down2;
-        w[u] = pack2<__half>(lo, hi);
-      }
+      for (int u = 0; u < D / 8; ++u)
+        w[u] = pack2<__half>(__uint_as_float(w[u] << 16) * d1 * d2, __uint_as_float(w[u] & 0xffff0000u) * d1 * d2);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      factor[n][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + e));
+      query[n][e] = (r_first + min(8 * n + 2 * c + e, rows - 1)) / ratio;
     }
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      qa[k][h] = w[(k >> 2) * 8 + (k & 3) * 2];
-      qa[k][2 + h] = w[(k >> 2) * 8 + (k & 3) * 2 + 1];
+      qb[n][k][0] = w[(k >> 2) * 8 + (k & 3) * 2];
+      qb[n][k][1] = w[(k >> 2) * 8 + (k & 3) * 2 + 1];
     }
   }
-  typename Mask::Bounds bounds[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) bounds[h] = Mask::bounds(p, s, min((r_first + min(g + 8 * h, rows - 1)) / ratio, s.lq - 1));
+  // Tiles that every row of the block sees whole (tile_is_full's rule).
+  const int full_end = min(s.lk, q_lo + (s.lk - s.lq) + 1), full_from = kWin ? win_anchor(s, q_lo + q_n - 1, 0) - p.window : 0;
 
-  float o[D / 16][2][4];   // even and odd columns of 16
+  float o[kN][D / 16][4];   // column 2 g of 16 in rows 2 c, 2 c + 1; column 2 g + 1
+  float down[kN][2];        // what P of a row is multiplied by, a power of two
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j)
+  for (int n = 0; n < kN; ++n) {
+    down[n][0] = down[n][1] = 0x1p126f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[j][e >> 2][e & 3] = 0.f;
-  constexpr bool kShifted = std::is_same<H, E4m3>::value && !kHalf;   // V's numbers come times 2^-120
-  constexpr float kUp = kShifted ? 0x1p60f : 1.f;
-  const float p_scale = kHalf ? 1.f : p.scale * kUp;
-  float down[2] = {0x1p126f, 0x1p126f};   // (fp16) what P of a row is multiplied by, a power of two
+    for (int j = 0; j < D / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+  }
+  // this thread's places in a stage: K row g and g + 8, V for ldmatrix (lanes 0-7 and 16-23 name keys 0-7, the others 8-15)
+  const int v_row = (lane & 7) + ((lane >> 3) & 1) * 8;
 
-  for (int n = 0; n < mine; ++n) {
-    if (n + C::kStages - 1 < mine) request(warp + (n + C::kStages - 1) * kDecWarps, (n + C::kStages - 1) % C::kStages);
+  for (int i = 0; i < mine; ++i) {
+    if (i + C::kStages - 1 < mine) request(warp + (i + C::kStages - 1) * kDecWarps, (i + C::kStages - 1) % C::kStages);
     asm volatile("cp.async.commit_group;" ::: "memory");
     asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
     __syncwarp();
-    const uint8_t* at = ring + (n % C::kStages) * C::kStage;
-    const float* scales = reinterpret_cast<const float*>(at + 2 * C::kTile);
-    // scores of the keys 0 .. 7 and 8 .. 15
-    float sc[2][4];
+    const uint32_t at = (i % C::kStages) * C::kStage;
+    const uint8_t* const stage = ring_of_all + warp * C::kRing + at;
+    const float* scales = scales_of_mine + (i % C::kStages) * 2 * kDecKeys;
+    const int key = key_of_tile(tiles, t0 + warp + i * kDecWarps, kDecKeys);
+    float sc[kN][4];   // keys g and g + 8, rows 2 c and 2 c + 1
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
-      const int r = 8 * t + g;
+    for (int n = 0; n < kN; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
-      for (int blk = 0; blk < D / 64; ++blk) {
-        const int ch = D == 128 ? (4 * blk + c) ^ ((r & 1) << 2) : c;
-        const uint4 w = *reinterpret_cast<const uint4*>(at + r * D + ch * 16);
-        mma16816<__half>(sc[t], qa[4 * blk], halves_of<H, false>(w.x), halves_of<H, true>(w.x));
-        mma16816<__half>(sc[t], qa[4 * blk + 1], halves_of<H, false>(w.y), halves_of<H, true>(w.y));
-        mma16816<__half>(sc[t], qa[4 * blk + 2], halves_of<H, false>(w.z), halves_of<H, true>(w.z));
-        mma16816<__half>(sc[t], qa[4 * blk + 3], halves_of<H, false>(w.w), halves_of<H, true>(w.w));
-      }
+    for (int blk = 0; blk < D / 64; ++blk) {
+      const int ch = D == 128 ? (4 * blk + c) ^ ((g & 1) << 2) : c;
+      const uint4 w0 = *reinterpret_cast<const uint4*>(stage + g * D + ch * 16);
+      const uint4 w1 = *reinterpret_cast<const uint4*>(stage + (g + 8) * D + ch * 16);
+      auto step = [&](int k, uint32_t lo, uint32_t hi) {
+        uint32_t a[4];
+        to_halves<H>(lo, a[0], a[2]);
+        to_halves<H>(hi, a[1], a[3]);
+#pragma unroll
+        for (int n = 0; n < kN; ++n) mma16816(sc[n], a, qb[n][4 * blk + k]);
+      };
+      step(0, w0.x, w1.x);
+      step(1, w0.y, w1.y);
+      step(2, w0.z, w1.z);
+      step(3, w0.w, w1.w);
     }
     // P
-    const int key = key_of_tile(tiles, t0 + warp + n * kDecWarps, kDecKeys);
-    const bool full = Mask::full(p, s, q_lo, q_n, key, kDecKeys);
-    float pv[2][4];
+    const bool full = key + kDecKeys <= full_end && (!kWin || key > full_from || key + kDecKeys <= p.sink);
+    const float ks[2] = {scales[g], scales[g + 8]}, vs[2] = {scales[kDecKeys + g], scales[kDecKeys + g + 8]};
+    uint32_t pb[kN][2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float2 ks = *reinterpret_cast<const float2*>(scales + 8 * t + 2 * c);
-      const float2 vs = *reinterpret_cast<const float2*>(scales + kDecKeys + 8 * t + 2 * c);
+    for (int n = 0; n < kN; ++n) {
+      float pv[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float x = sc[t][e] * ((e & 1 ? ks.y : ks.x) * factor[e >> 1]);
-        const float sg = rcp(1.f + ex2(x * -1.4426950408889634f));
-        pv[t][e] = x * sg * ((e & 1 ? vs.y : vs.x) * p_scale);
-        // (a select, not a multiply: a masked score may be anything)
-        if (!full && !allowed(bounds[e >> 1], key + 8 * t + 2 * c + (e & 1))) pv[t][e] = 0.f;
+        const float x = sc[n][e] * (ks[e >> 1] * factor[n][e & 1]);
+        pv[e] = x * ptx::rcp_approx(1.f + ptx::ex2_approx(x * -1.4426950408889634f)) * vs[e >> 1];
       }
-    }
-    if (kHalf) {
-      float top[2];
-      bool grow = false;
+      if (!full) {   // (a select, not a multiply: a masked score may be anything)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        top[h] = fmaxf(fmaxf(fabsf(pv[0][2 * h]), fabsf(pv[0][2 * h + 1])), fmaxf(fabsf(pv[1][2 * h]), fabsf(pv[1][2 * h + 1])));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        grow |= top[h] * down[h] > 16384.f;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!(top[h] * down[h] > 16384.f) || top[h] > 3.402823466e38f) continue;
-          // the largest P to [1, 2)
-          const float next = __uint_as_float((254u - min(__float_as_uint(top[h]) >> 23, 253u)) << 23), ratio = next / down[h];
-          down[h] = next;
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) o[j][u][2 * h] *= ratio, o[j][u][2 * h + 1] *= ratio;
+        for (int e = 0; e < 2; ++e) {
+          const typename Mask::Bounds rb = Mask::bounds(p, s, query[n][e]);
+          if (!allowed(rb, key + g)) pv[e] = 0.f;
+          if (!allowed(rb, key + g + 8)) pv[2 + e] = 0.f;
         }
       }
-    }
-    uint32_t pa[4];
+      const float m0 = fmaxf(fabsf(pv[0]), fabsf(pv[2])), m1 = fmaxf(fabsf(pv[1]), fabsf(pv[3]));
+      if (__any_sync(0xffffffffu, m0 * down[n][0] > 16384.f || m1 * down[n][1] > 16384.f)) {
+        float top[2] = {m0, m1};
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        pa[2 * t + h] = pack2<T>(pv[t][2 * h] * (kHalf ? down[h] : 1.f), pv[t][2 * h + 1] * (kHalf ? down[h] : 1.f));
-    // O += P.V
-    const uint32_t v_at = ring_at + (n % C::kStages) * C::kStage + C::kTile;
-    const int v_row = (lane & 7) + ((lane >> 3) & 1) * 8;   // ldmatrix: lanes 0-7 and 16-23 name keys 0-7, the others 8-15
-    uint32_t w[D / 32][4];
-    uint32_t nan = 0;
+          for (int x = 4; x < 32; x <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
+          if (!(top[e] * down[n][e] > 16384.f) || top[e] > 3.402823466e38f) continue;
+          // the row's largest P to [1, 2)
+          const float next = __uint_as_float((254u - min(__float_as_uint(top[e]) >> 23, 253u)) << 23), ratio2 = next / down[n][e];
+          down[n][e] = next;
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      const int chunk = 2 * j + (lane >> 4);
-      ldsm_x4_trans(v_at + v_row * D + (D == 128 ? chunk ^ (v_row & 7) : chunk ^ ((v_row >> 1) & 3)) * 16, w[j]);
-      if (kShifted) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) nan |= nan_bytes(w[j][u]);
+          for (int j = 0; j < D / 16; ++j) o[n][j][e] *= ratio2, o[n][j][2 + e] *= ratio2;
+        }
       }
+      pb[n][0] = transposed(pack2<__half>(pv[0] * down[n][0], pv[1] * down[n][1]));
+      pb[n][1] = transposed(pack2<__half>(pv[2] * down[n][0], pv[3] * down[n][1]));
     }
-    if (kShifted && __any_sync(0xffffffffu, nan != 0)) {
+    // O^T += V^T.P^T
+    const uint32_t v_at = ring_at + at + C::kTile + v_row * D;
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j)
+    for (int j = 0; j < D / 16; j += 2) {
+      const int chunk = j + (lane >> 4);
+      uint32_t w[4];
+      ldsm_x4_trans(v_at + (D == 128 ? chunk ^ (v_row & 7) : chunk ^ ((v_row >> 1) & 3)) * 16, w);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          mma16816<T>(o[2 * j + u][0], pa, pair_with_nan<false>(w[j][2 * u]), pair_with_nan<false>(w[j][2 * u + 1]));
-          mma16816<T>(o[2 * j + u][1], pa, pair_with_nan<true>(w[j][2 * u]), pair_with_nan<true>(w[j][2 * u + 1]));
-        }
-    } else {
+      for (int u = 0; u < 2; ++u) {
+        uint32_t a[4];   // columns 2 g (a pair of keys) and 2 g + 1, keys 0-7; the same, keys 8-15
+        to_halves<H>(__byte_perm(w[2 * u], 0u, 0x3120), a[0], a[1]);
+        to_halves<H>(__byte_perm(w[2 * u + 1], 0u, 0x3120), a[2], a[3]);
 #pragma unroll
-      for (int j = 0; j < D / 32; ++j)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          mma16816<T>(o[2 * j + u][0], pa, pair_of<H, T, false>(w[j][2 * u]), pair_of<H, T, false>(w[j][2 * u + 1]));
-          mma16816<T>(o[2 * j + u][1], pa, pair_of<H, T, true>(w[j][2 * u]), pair_of<H, T, true>(w[j][2 * u + 1]));
-        }
+        for (int n = 0; n < kN; ++n) mma16816(o[n][j + u], a, pb[n]);
+      }
     }
     __syncwarp();   // the stage is free
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();   // every warp is through with its ring
   // The warps' outputs, added in order.
-  float* all = reinterpret_cast<float*>(ring_of_all);   // [warps][16][D]
+  float* all = reinterpret_cast<float*>(ring_of_all);   // [warps][rows][D]
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j)
+  for (int n = 0; n < kN; ++n)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float4 v = make_float4(o[j][0][2 * h], o[j][1][2 * h], o[j][0][2 * h + 1], o[j][1][2 * h + 1]);
-      const float f = kHalf ? 1.f / down[h] : kUp;
-      v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-      *reinterpret_cast<float4*>(all + (warp * kDecRows + g + 8 * h) * D + 16 * j + 4 * c) = v;
+    for (int e = 0; e < 2; ++e) {
+      const float f = 1.f / down[n][e];
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j)
+        *reinterpret_cast<float2*>(all + (warp * C::kRows + 8 * n + 2 * c + e) * D + 16 * j + 2 * g) = make_float2(o[n][j][e] * f, o[n][j][2 + e] * f);
     }
   __syncthreads();
-  const int valid = min(rows, kDecRows);
-  const float o_scale = kHalf ? p.scale : 1.f;
+  const int valid = min(rows, C::kRows);
   const long long group = static_cast<long long>(blockIdx.x) * gridDim.z + blockIdx.z;
   auto store = [&](int r, int col, float4 v) {
     if (col >= p.dqk) return;
     const int row = r_first + r;
     T* to = static_cast<T*>(p.out) + ((s.q0 + row / ratio) * p.hq + hk * ratio + row % ratio) * p.dqk + col;
-    *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * p.scale, v.y * p.scale), pack2<T>(v.z * p.scale, v.w * p.scale));
   };
   for (int i = tid; i < valid * (D / 4); i += kDecThreads) {
     const int r = i / (D / 4), col = i % (D / 4) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
-      const float4 x = *reinterpret_cast<const float4*>(all + (w * kDecRows + r) * D + col);
+      const float4 x = *reinterpret_cast<const float4*>(all + (w * C::kRows + r) * D + col);
       v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
     }
-    v.x *= o_scale, v.y *= o_scale, v.z *= o_scale, v.w *= o_scale;
     if (active == 1) store(r, col, v);
     else *reinterpret_cast<float4*>(d.partial + ((group * d.splits + split) * d.rows + r) * D + col) = v;
   }
@@ -440,11 +410,18 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
 struct DecPlan {
   int tiles, splits, row_blocks, rows;
 };
+int tile_width(const KParams& p) { return p.dqk <= 64 ? 64 : 128; }
+// Rows of a CTA: as many groups of eight as its registers hold (1, 2; 4 at width 64).
+int row_groups(const KParams& p) {
+  const long long rows = static_cast<long long>(p.maxq) * p.gqa_ratio;
+  return rows <= 8 ? 1 : rows <= 16 || tile_width(p) == 128 ? 2 : 4;
+}
 DecPlan plan(const KParams& p) {
   DecPlan d;
   const long long rows = static_cast<long long>(p.maxq) * p.gqa_ratio;
-  d.row_blocks = static_cast<int>((rows + kDecRows - 1) / kDecRows);
-  d.rows = rows < kDecRows ? static_cast<int>(rows) : kDecRows;
+  const int at_once = 8 * row_groups(p);
+  d.row_blocks = static_cast<int>((rows + at_once - 1) / at_once);
+  d.rows = rows < at_once ? static_cast<int>(rows) : at_once;
   long long most = (p.maxk + kDecKeys - 1) / kDecKeys;   // tiles of the longest sequence
   long long all = p.num_page_ids * p.page_size / kDecKeys;   // and of all of them together, at most
   if (p.window) {
@@ -464,12 +441,11 @@ DecPlan plan(const KParams& p) {
 uint64_t counters_bytes(const KParams& p, const DecPlan& d) {
   return (static_cast<uint64_t>(p.batch) * p.hk * d.row_blocks * 4 + 255) & ~static_cast<uint64_t>(255);
 }
-int tile_width(const KParams& p) { return p.dqk <= 64 ? 64 : 128; }
 
-template <int D, typename T, typename H>
-cudaError_t launch_dec(const DecParams& d, const DecPlan& pl, cudaStream_t stream) {
-  using C = DecCfg<D>;
-  auto kern = d.f.window ? hstu_decode8_kernel<D, T, H, true> : hstu_decode8_kernel<D, T, H, false>;
+template <int D, int kN, typename T, typename H>
+cudaError_t launch_dec_of(const DecParams& d, const DecPlan& pl, cudaStream_t stream) {
+  using C = DecCfg<D, kN>;
+  auto kern = d.f.window ? hstu_decode8_kernel<D, kN, T, H, true> : hstu_decode8_kernel<D, kN, T, H, false>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
@@ -483,6 +459,14 @@ cudaError_t launch_dec(const DecParams& d, const DecPlan& pl, cudaStream_t strea
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, d);
+}
+template <int D, typename T, typename H>
+cudaError_t launch_dec(const DecParams& d, const DecPlan& pl, cudaStream_t stream) {
+  switch (row_groups(d.f)) {
+    case 1: return launch_dec_of<D, 1, T, H>(d, pl, stream);
+    case 2: return launch_dec_of<D, 2, T, H>(d, pl, stream);
+    default: return launch_dec_of<64, 4, T, H>(d, pl, stream);   // (of width 64 only)
+  }
 }
 
 }  // namespace
