@@ -36,15 +36,16 @@ namespace {
 
 constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16;      // keys of a tile
+constexpr int kPair = 2;          // tiles a warp works on at a time: their chains of dependent steps overlap
 constexpr int kDecMostTiles = 128;   // of a CTA
 
 template <int D, int kN> struct DecCfg {
   static constexpr int kRows = 8 * kN;                          // rows of a CTA
-  static constexpr int kStages = 4;
+  static constexpr int kStages = 2;                             // of kPair tiles each
   static constexpr int kTile = kDecKeys * D;                    // bytes of K (V) of a tile
-  static constexpr int kStage = 2 * kTile;
+  static constexpr int kStage = kPair * 2 * kTile;
   static constexpr int kRing = kStages * kStage;
-  static constexpr int kScales = kDecWarps * kStages * 2 * kDecKeys * 4;
+  static constexpr int kScales = kDecWarps * kStages * kPair * 2 * kDecKeys * 4;
   static constexpr int kSmem = kDecWarps * kRing + kScales;
   static_assert(kDecWarps * kRing >= kDecWarps * kRows * D * 4, "the rings hold the warps' partial outputs at the end");
 };
@@ -55,6 +56,9 @@ struct DecParams {
   float* partial;       // [batch * hk * row blocks][splits][rows][D]
   int splits, tiles, rows;   // CTAs along the keys, tiles of a CTA, rows of a partial block
   int block_shift;      // log2 of a scale's block, 4 at most (a tile has one scale from there on)
+  // ceil(2^32 / n): x / n is the upper half of the product, exactly, while x n < 2^32 (a warp with 20 tiles to do feels a
+  // handful of divisions)
+  uint32_t by_hk, by_ratio, by_page, by_block;
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {   // (the rest of the 16 becomes zeros)
@@ -76,7 +80,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
   return y;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
@@ -129,7 +133,8 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   __shared__ long long s_scale[kDecMostTiles];   // where its scales start
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  const int b = blockIdx.x / p.hk, hk = blockIdx.x - b * p.hk, split = blockIdx.y, r_first = blockIdx.z * C::kRows;
+  auto over = [](int x, uint32_t inverse) { return static_cast<int>(inverse ? __umulhi(static_cast<uint32_t>(x), inverse) : static_cast<uint32_t>(x)); };
+  const int b = over(blockIdx.x, d.by_hk), hk = blockIdx.x - b * p.hk, split = blockIdx.y, r_first = blockIdx.z * C::kRows;
 
   const SeqInfo s = load_seq(p, b);
   const int ratio = p.gqa_ratio, rows = s.lq * ratio - r_first;   // rows of this block, the group's heads inside a query
@@ -149,10 +154,14 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
       atomicOr(p.ws_header, st);
     }
   }
-  const int q_lo = r_first / ratio, q_n = (min(rows, C::kRows) + r_first + ratio - 1) / ratio - q_lo;   // the block's queries
+  const int q_lo = over(r_first, d.by_ratio), q_n = over(min(rows, C::kRows) + r_first + ratio - 1, d.by_ratio) - q_lo;   // the block's queries
   const KeyTiles tiles = rows > 0 ? Mask::tiles(p, s, q_lo, q_n, kDecKeys) : KeyTiles{0, 0, 0};
-  const int active = max(1, (tiles.n + d.tiles - 1) / d.tiles);   // CTAs that share this block's keys
-  const int t0 = split * d.tiles, t1 = min(tiles.n, t0 + d.tiles);
+  // CTAs that share this block's keys, evenly, in whole rounds of the four warps' pairs
+  int active = 1;
+  while (active * d.tiles < tiles.n) ++active;
+  constexpr int kRound = kDecWarps * kPair;
+  const int each = active == 1 ? d.tiles : (tiles.n + active * kRound - 1) / (active * kRound) * kRound;
+  const int t0 = split * each, t1 = min(tiles.n, t0 + each);
   if (rows <= 0 || split >= active) {   // uniform over the CTA
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
@@ -160,15 +169,15 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   // The places of this CTA's tiles: a tile lies in one page.
   const int per_page = p.page_size / p.scale_block, row_bytes = p.hk * p.dqk;
   for (int i = tid; i < t1 - t0; i += kDecThreads) {
-    const int key = key_of_tile(tiles, t0 + i, kDecKeys), slot = key / p.page_size, in_page = key - slot * p.page_size;
+    const int key = key_of_tile(tiles, t0 + i, kDecKeys), slot = over(key, d.by_page), in_page = key - slot * p.page_size;
     const long long pid = pg0 + slot < pg1 ? load_index(p.page_ids, p.index_bytes, pg0 + slot) : -1;
     const bool ok = pid >= 0 && pid < p.num_pages;
     s_row[i] = ok ? (pid * 2 * p.page_size + in_page) * row_bytes : -1;
-    s_scale[i] = ok ? (pid * 2 * per_page + in_page / p.scale_block) * p.hk : 0;
+    s_scale[i] = ok ? (pid * 2 * per_page + over(in_page, d.by_block)) * p.hk : 0;
   }
   __syncthreads();
 
-  float* const scales_of_mine = reinterpret_cast<float*>(ring_of_all + kDecWarps * C::kRing) + warp * C::kStages * 2 * kDecKeys;
+  float* const scales_of_mine = reinterpret_cast<float*>(ring_of_all + kDecWarps * C::kRing) + warp * C::kStages * kPair * 2 * kDecKeys;
   const uint32_t ring_at = ptx::smem_u32(ring_of_all) + warp * C::kRing;
   constexpr int kChunks = D / 16, kAtOnce = 32 / kChunks;   // 16-byte chunks of a row, rows that 32 lanes copy at once
   const int my_row = lane / kChunks, my_chunk = lane % kChunks;
@@ -177,12 +186,12 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   const long long to_v = static_cast<long long>(p.page_size) * row_bytes;
   const int to_rows = kAtOnce * row_bytes;
   const float* scale_from = p.kv_scale + hk + ((lane < 16 ? 0 : per_page) + ((lane & 15) >> d.block_shift)) * static_cast<long long>(p.hk);
-  // Requests tile t0 + i into stage i's slot; rows behind the last cached one read as zeros.  (Chunks are permuted so that the
+  // Requests tile t0 + i into a slot; rows behind the last cached one, and tiles behind the last, read as zeros.  (Chunks are permuted so that the
   // pieces of 16 bytes eight lanes read at once fall on different banks.)
-  auto request = [&](int i, int stage) {
-    const long long at = s_row[i];
+  auto request_tile = [&](int i, int slot) {
+    const long long at = i < t1 - t0 ? s_row[i] : -1;
     const int left = at < 0 ? 0 : s.lk - key_of_tile(tiles, t0 + i, kDecKeys);
-    const uint32_t to = ring_at + stage * C::kStage;
+    const uint32_t to = ring_at + slot * 2 * C::kTile;
     const uint8_t* k_at = from_lane + (at < 0 ? 0 : at);
     const uint8_t* v_at = k_at + to_v;
     auto copy = [&](auto whole) {
@@ -200,12 +209,17 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
     if (left >= kDecKeys) copy(std::true_type{});
     else copy(std::false_type{});
     const bool on = (lane & 15) < left;
-    cp4(ptx::smem_u32(scales_of_mine + stage * 2 * kDecKeys + lane), on ? scale_from + s_scale[i] : p.kv_scale, on);
+    cp4(ptx::smem_u32(scales_of_mine + slot * 2 * kDecKeys + lane), on ? scale_from + s_scale[i] : p.kv_scale, on);
   };
-  const int mine = (t1 - t0 - warp + kDecWarps - 1) / kDecWarps;   // tiles of this warp: warp, warp + 4, ..
+  // the pair of tiles `i` of this warp: warp + 8 i and warp + 8 i + 4
+  auto request = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < kPair; ++u) request_tile(warp + (i * kPair + u) * kDecWarps, (i % C::kStages) * kPair + u);
+  };
+  const int mine = (t1 - t0 - warp + kDecWarps * kPair - 1) / (kDecWarps * kPair);   // pairs of this warp
 #pragma unroll
   for (int u = 0; u < C::kStages - 1; ++u) {
-    if (u < mine) request(warp + u * kDecWarps, u);
+    if (u < mine) request(u);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
@@ -218,7 +232,8 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
     const int r = 8 * n + g;
     const bool on = r < rows;
     const int row = on ? r_first + r : 0;
-    const T* from = static_cast<const T*>(p.q) + ((s.q0 + row / ratio) * p.hq + hk * ratio + row % ratio) * p.dqk;
+    const int i_row = over(row, d.by_ratio);
+    const T* from = static_cast<const T*>(p.q) + ((s.q0 + i_row) * p.hq + hk * ratio + row - i_row * ratio) * p.dqk;
     uint32_t w[D / 8];   // pairs in memory's order
 #pragma unroll
     for (int blk = 0; blk < D / 64; ++blk) {
@@ -246,7 +261,7 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       factor[n][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + e));
-      query[n][e] = (r_first + min(8 * n + 2 * c + e, rows - 1)) / ratio;
+      query[n][e] = over(r_first + min(8 * n + 2 * c + e, rows - 1), d.by_ratio);
     }
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
@@ -269,88 +284,115 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   const int v_row = (lane & 7) + ((lane >> 3) & 1) * 8;
 
   for (int i = 0; i < mine; ++i) {
-    if (i + C::kStages - 1 < mine) request(warp + (i + C::kStages - 1) * kDecWarps, (i + C::kStages - 1) % C::kStages);
+    if (i + C::kStages - 1 < mine) request(i + C::kStages - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
     asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
     __syncwarp();
     const uint32_t at = (i % C::kStages) * C::kStage;
     const uint8_t* const stage = ring_of_all + warp * C::kRing + at;
-    const float* scales = scales_of_mine + (i % C::kStages) * 2 * kDecKeys;
-    const int key = key_of_tile(tiles, t0 + warp + i * kDecWarps, kDecKeys);
-    float sc[kN][4];   // keys g and g + 8, rows 2 c and 2 c + 1
+    const float* const scales = scales_of_mine + (i % C::kStages) * kPair * 2 * kDecKeys;
+    float sc[kPair][kN][4];   // keys g and g + 8, rows 2 c and 2 c + 1
 #pragma unroll
-    for (int n = 0; n < kN; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+    for (int t = 0; t < kPair; ++t)
+#pragma unroll
+      for (int n = 0; n < kN; ++n) sc[t][n][0] = sc[t][n][1] = sc[t][n][2] = sc[t][n][3] = 0.f;
 #pragma unroll
     for (int blk = 0; blk < D / 64; ++blk) {
       const int ch = D == 128 ? (4 * blk + c) ^ ((g & 1) << 2) : c;
-      const uint4 w0 = *reinterpret_cast<const uint4*>(stage + g * D + ch * 16);
-      const uint4 w1 = *reinterpret_cast<const uint4*>(stage + (g + 8) * D + ch * 16);
-      auto step = [&](int k, uint32_t lo, uint32_t hi) {
-        uint32_t a[4];
-        to_halves<H>(lo, a[0], a[2]);
-        to_halves<H>(hi, a[1], a[3]);
+      uint4 w[kPair][2];
 #pragma unroll
-        for (int n = 0; n < kN; ++n) mma16816(sc[n], a, qb[n][4 * blk + k]);
-      };
-      step(0, w0.x, w1.x);
-      step(1, w0.y, w1.y);
-      step(2, w0.z, w1.z);
-      step(3, w0.w, w1.w);
+      for (int t = 0; t < kPair; ++t) {
+        w[t][0] = *reinterpret_cast<const uint4*>(stage + t * 2 * C::kTile + g * D + ch * 16);
+        w[t][1] = *reinterpret_cast<const uint4*>(stage + t * 2 * C::kTile + (g + 8) * D + ch * 16);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int t = 0; t < kPair; ++t) {
+          uint32_t a[4];
+          to_halves<H>(reinterpret_cast<const uint32_t*>(&w[t][0])[k], a[0], a[2]);
+          to_halves<H>(reinterpret_cast<const uint32_t*>(&w[t][1])[k], a[1], a[3]);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) mma16816(sc[t][n], a, qb[n][4 * blk + k]);
+        }
     }
     // P
-    const bool full = key + kDecKeys <= full_end && (!kWin || key > full_from || key + kDecKeys <= p.sink);
-    const float ks[2] = {scales[g], scales[g + 8]}, vs[2] = {scales[kDecKeys + g], scales[kDecKeys + g + 8]};
-    uint32_t pb[kN][2];
+    uint32_t pb[kPair][kN][2];
+    float ks[kPair][2], vs[kPair][2];
+    int key[kPair];
+    bool full = true;
+#pragma unroll
+    for (int t = 0; t < kPair; ++t) {
+      const float* at_scales = scales + t * 2 * kDecKeys;
+      ks[t][0] = at_scales[g], ks[t][1] = at_scales[g + 8];
+      vs[t][0] = at_scales[kDecKeys + g], vs[t][1] = at_scales[kDecKeys + g + 8];
+      key[t] = key_of_tile(tiles, t0 + warp + (i * kPair + t) * kDecWarps, kDecKeys);
+      full &= key[t] + kDecKeys <= full_end && (!kWin || key[t] > full_from || key[t] + kDecKeys <= p.sink);
+    }
 #pragma unroll
     for (int n = 0; n < kN; ++n) {
-      float pv[4];
+      float pv[kPair][4];
+      float m[2] = {0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = sc[n][e] * (ks[e >> 1] * factor[n][e & 1]);
-        pv[e] = x * ptx::rcp_approx(1.f + ptx::ex2_approx(x * -1.4426950408889634f)) * vs[e >> 1];
-      }
-      if (!full) {   // (a select, not a multiply: a masked score may be anything)
+      for (int t = 0; t < kPair; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = sc[t][n][e] * (ks[t][e >> 1] * factor[n][e & 1]);
+          pv[t][e] = x * ptx::rcp_approx(1.f + ptx::ex2_approx(x * -1.4426950408889634f)) * vs[t][e >> 1];
+        }
+      if (!full) {   // (a select, not a multiply: a masked score may be anything; a tile behind the last one is all masked)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const typename Mask::Bounds rb = Mask::bounds(p, s, query[n][e]);
-          if (!allowed(rb, key + g)) pv[e] = 0.f;
-          if (!allowed(rb, key + g + 8)) pv[2 + e] = 0.f;
+#pragma unroll
+          for (int t = 0; t < kPair; ++t) {
+            if (!allowed(rb, key[t] + g)) pv[t][e] = 0.f;
+            if (!allowed(rb, key[t] + g + 8)) pv[t][2 + e] = 0.f;
+          }
         }
       }
-      const float m0 = fmaxf(fabsf(pv[0]), fabsf(pv[2])), m1 = fmaxf(fabsf(pv[1]), fabsf(pv[3]));
-      if (__any_sync(0xffffffffu, m0 * down[n][0] > 16384.f || m1 * down[n][1] > 16384.f)) {
-        float top[2] = {m0, m1};
+#pragma unroll
+      for (int t = 0; t < kPair; ++t) {
+        m[0] = fmaxf(m[0], fmaxf(fabsf(pv[t][0]), fabsf(pv[t][2])));
+        m[1] = fmaxf(m[1], fmaxf(fabsf(pv[t][1]), fabsf(pv[t][3])));
+      }
+      if (__any_sync(0xffffffffu, m[0] * down[n][0] > 16384.f || m[1] * down[n][1] > 16384.f)) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
-          if (!(top[e] * down[n][e] > 16384.f) || top[e] > 3.402823466e38f) continue;
+          for (int x = 4; x < 32; x <<= 1) m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], x));
+          if (!(m[e] * down[n][e] > 16384.f) || m[e] > 3.402823466e38f) continue;
           // the row's largest P to [1, 2)
-          const float next = __uint_as_float((254u - min(__float_as_uint(top[e]) >> 23, 253u)) << 23), ratio2 = next / down[n][e];
+          const float next = __uint_as_float((254u - min(__float_as_uint(m[e]) >> 23, 253u)) << 23), ratio2 = next / down[n][e];
           down[n][e] = next;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) o[n][j][e] *= ratio2, o[n][j][2 + e] *= ratio2;
         }
       }
-      pb[n][0] = transposed(pack2<__half>(pv[0] * down[n][0], pv[1] * down[n][1]));
-      pb[n][1] = transposed(pack2<__half>(pv[2] * down[n][0], pv[3] * down[n][1]));
+#pragma unroll
+      for (int t = 0; t < kPair; ++t) {
+        pb[t][n][0] = transposed(pack2<__half>(pv[t][0] * down[n][0], pv[t][1] * down[n][1]));
+        pb[t][n][1] = transposed(pack2<__half>(pv[t][2] * down[n][0], pv[t][3] * down[n][1]));
+      }
     }
     // O^T += V^T.P^T
     const uint32_t v_at = ring_at + at + C::kTile + v_row * D;
 #pragma unroll
-    for (int j = 0; j < D / 16; j += 2) {
-      const int chunk = j + (lane >> 4);
-      uint32_t w[4];
-      ldsm_x4_trans(v_at + (D == 128 ? chunk ^ (v_row & 7) : chunk ^ ((v_row >> 1) & 3)) * 16, w);
+    for (int t = 0; t < kPair; ++t)
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t a[4];   // columns 2 g (a pair of keys) and 2 g + 1, keys 0-7; the same, keys 8-15
-        to_halves<H>(__byte_perm(w[2 * u], 0u, 0x3120), a[0], a[1]);
-        to_halves<H>(__byte_perm(w[2 * u + 1], 0u, 0x3120), a[2], a[3]);
+      for (int j = 0; j < D / 16; j += 2) {
+        const int chunk = j + (lane >> 4);
+        uint32_t w[4];
+        ldsm_x4_trans(v_at + t * 2 * C::kTile + (D == 128 ? chunk ^ (v_row & 7) : chunk ^ ((v_row >> 1) & 3)) * 16, w);
 #pragma unroll
-        for (int n = 0; n < kN; ++n) mma16816(o[n][j + u], a, pb[n]);
+        for (int u = 0; u < 2; ++u) {
+          uint32_t a[4];   // columns 2 g (a pair of keys) and 2 g + 1, keys 0-7; the same, keys 8-15
+          to_halves<H>(__byte_perm(w[2 * u], 0u, 0x3120), a[0], a[1]);
+          to_halves<H>(__byte_perm(w[2 * u + 1], 0u, 0x3120), a[2], a[3]);
+#pragma unroll
+          for (int n = 0; n < kN; ++n) mma16816(o[n][j + u], a, pb[t][n]);
+        }
       }
-    }
     __syncwarp();   // the stage is free
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -371,8 +413,8 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   const long long group = static_cast<long long>(blockIdx.x) * gridDim.z + blockIdx.z;
   auto store = [&](int r, int col, float4 v) {
     if (col >= p.dqk) return;
-    const int row = r_first + r;
-    T* to = static_cast<T*>(p.out) + ((s.q0 + row / ratio) * p.hq + hk * ratio + row % ratio) * p.dqk + col;
+    const int row = r_first + r, i_row = over(row, d.by_ratio);
+    T* to = static_cast<T*>(p.out) + ((s.q0 + i_row) * p.hq + hk * ratio + row - i_row * ratio) * p.dqk + col;
     *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * p.scale, v.y * p.scale), pack2<T>(v.z * p.scale, v.w * p.scale));
   };
   for (int i = tid; i < valid * (D / 4); i += kDecThreads) {
@@ -429,11 +471,13 @@ DecPlan plan(const KParams& p) {
     if (seen < most) most = seen;
     if (seen * p.batch < all) all = seen * p.batch;
   }
-  // Some twelve CTAs per SM, so that sequences of different lengths even out; a CTA of fewer than 8 tiles (two per warp) is
-  // mostly set-up.
-  long long tiles = all * p.hk * d.row_blocks / (12ll * 148);
+  // Some six CTAs per SM (three fit): fewer, and sequences of different lengths do not even out; more, and set-up and partial
+  // sums - a thousand instructions a warp, where a tile takes 300 - are what the SMs do.  Attention alone, us, at 4 / 6 / 8 /
+  // 12: 128 users of 200 - 2048 rows and 8 heads 64 / 66 / 70 / 75, 4 users of 14000 - 20000 44 / 39 / 45 / 50.
+  long long tiles = all * p.hk * d.row_blocks / (6ll * 148);
   tiles = tiles < 8 ? 8 : tiles > kDecMostTiles ? kDecMostTiles : tiles;
-  d.tiles = static_cast<int>((tiles + kDecWarps - 1) / kDecWarps * kDecWarps);
+  constexpr int kRound = kDecWarps * kPair;
+  d.tiles = static_cast<int>((tiles + kRound - 1) / kRound * kRound);
   d.splits = static_cast<int>((most + d.tiles - 1) / d.tiles);
   if (d.splits < 1) d.splits = 1;
   return d;
@@ -497,6 +541,12 @@ cudaError_t launch_decode8(const KParams& p, int dtype, void* workspace, cudaStr
   d.splits = pl.splits;
   d.tiles = pl.tiles;
   d.rows = pl.rows;
+  // (at most 2^20 heads of sequences by 16, 64 rows by 16, 20480 keys by a page of any size; of 1: 0)
+  auto inverse = [](int n) { return n == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + n - 1) / n); };
+  d.by_hk = inverse(p.hk);
+  d.by_ratio = inverse(p.gqa_ratio);
+  d.by_page = inverse(p.page_size);
+  d.by_block = inverse(p.scale_block);
   d.block_shift = 4;
   while (d.block_shift > 0 && (1 << d.block_shift) > p.scale_block) --d.block_shift;
   const long long n = pl.splits > 1 ? static_cast<long long>(p.batch) * p.hk * pl.row_blocks : 0;
