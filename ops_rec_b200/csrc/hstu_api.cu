@@ -40,6 +40,9 @@ cudaError_t launch_paged_gather(const KParams& p, const void* kv_cache, const vo
 bool decode8_supported(const KParams& p, int dtype);
 uint64_t decode8_workspace(const KParams& p);
 cudaError_t launch_decode8(const KParams& p, int dtype, void* workspace, cudaStream_t stream);
+bool rows8_supported(const KParams& p, int dtype);
+uint64_t rows8_workspace(const KParams& p);
+cudaError_t launch_rows8(const KParams& p, int dtype, void* workspace, cudaStream_t stream);
 cudaError_t launch_append(const HstuCacheAppendArgs& a, cudaStream_t stream);
 }  // namespace hstu
 
@@ -485,7 +488,9 @@ static hstu::KParams paged8_params(const HstuPaged8Args* args, const PagedPlan& 
   return p;
 }
 static uint64_t paged8_workspace(const hstu::KParams& p, const PagedPlan& pl) {
-  return hstu::decode8_supported(p, pl.fwd.dtype) ? hstu::decode8_workspace(p) : pl.fwd_bytes + 2 * pl.stage_bytes;
+  if (hstu::decode8_supported(p, pl.fwd.dtype)) return hstu::decode8_workspace(p);
+  if (hstu::rows8_supported(p, pl.fwd.dtype)) return hstu::rows8_workspace(p);
+  return pl.fwd_bytes + 2 * pl.stage_bytes;
 }
 
 int hstu_paged_8bit_fwd_get_workspace_size(const HstuPaged8Args* args, uint64_t* workspace_bytes) {
@@ -518,12 +523,13 @@ int hstu_paged_8bit_fwd(const HstuPaged8Args* args, void* workspace, uint64_t wo
     return fail(HSTU_E_WORKSPACE, "workspace has %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
                 (unsigned long long)need);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  if (hstu::decode8_supported(p, pl.fwd.dtype)) {
+  const bool few = hstu::decode8_supported(p, pl.fwd.dtype);
+  if (few || hstu::rows8_supported(p, pl.fwd.dtype)) {
     DeviceInfo dev;
     rc = device_info(&dev);
     if (rc) return rc;
     if (dev.major != 10) return fail(HSTU_E_ARCH, "this library is built for sm_100a only; device has compute capability %d.x", dev.major);
-    const cudaError_t e = hstu::launch_decode8(p, pl.fwd.dtype, workspace, stream);
+    const cudaError_t e = few ? hstu::launch_decode8(p, pl.fwd.dtype, workspace, stream) : hstu::launch_rows8(p, pl.fwd.dtype, workspace, stream);
     return e == cudaSuccess ? HSTU_OK : fail(HSTU_E_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   }
   char* base = static_cast<char*>(workspace);

@@ -10,14 +10,12 @@
 // sequence has more keys than a CTA takes - over CTAs: each leaves its partial sums in the workspace, and the last one to arrive
 // adds them in the order of the keys (the same bits every time).
 //
-// The rows of a call are (query, head of the group) pairs of one key head, 8 kN at a time: grouped heads share the cache's reads.
-// Both products have the cache as their A operand (16 keys, 16 columns of the head) and the rows as the 8 columns of B, so that
-// a number is converted once for all rows and one row does not cost what sixteen do.  All operands are fp16, whatever the call's
-// type: e4m3 and int8 numbers are exact there, one conversion per pair (bf16 has no such instruction, and five integer
-// operations per pair made the kernel issue-bound: 875 instructions a tile and 104 us above), and P has three bits more.
-//   S^T = K.Q^T    bf16 queries are divided by a power of two per row (their largest element to [1, 2)), which keeps all 8 bits
-//                  of every element that counts.  A thread's 16 bytes of a key are contiguous; the same permutation of the
-//                  contraction is applied to Q.  The key's scale, alpha and the row's power of two multiply the 32-bit score.
+// The rows of a call are (query, head of the group) pairs of one key head: grouped heads share the cache's reads.  Both products
+// have the cache as their A operand (16 keys, 16 columns of the head) and the rows as the eight columns of B, so that one row
+// does not cost what sixteen do.
+//   S^T = K.Q^T    bf16 queries are divided by a power of two per row, which keeps all 8 bits of every element that counts.  A
+//                  thread's 16 bytes of a key are contiguous; the same permutation of the contraction is applied to Q.  The
+//                  key's scale, alpha and the row's power of two multiply the 32-bit score.
 //   P              silu(x) * (scale of the value's block), rounded once, divided by a power of two per row that follows the
 //                  largest P so far (raised, and the output rescaled, when P outgrows 2^14), since neither scores nor scales
 //                  keep P inside fp16's narrow range
@@ -25,10 +23,7 @@
 //                  ones the rows 8-15.  P changes from accumulator to operand with movmatrix.
 // tcgen05 would need M = 128 rows and its operands in shared memory in 16 bits: the conversion would go through shared memory
 // twice for a tile of which one row counts.
-#include <type_traits>
-
-#include "hstu_held.cuh"
-#include "ptx_sm100.cuh"
+#include "hstu_mma8.cuh"
 
 namespace hstu {
 
@@ -39,8 +34,8 @@ constexpr int kDecKeys = 16;      // keys of a tile
 constexpr int kPair = 2;          // tiles a warp works on at a time: their chains of dependent steps overlap
 constexpr int kDecMostTiles = 128;   // of a CTA
 
-template <int D, int kN> struct DecCfg {
-  static constexpr int kRows = 8 * kN;                          // rows of a CTA
+template <int D> struct DecCfg {
+  static constexpr int kRows = 8;                               // rows of a CTA
   static constexpr int kStages = 2;                             // of kPair tiles each
   static constexpr int kTile = kDecKeys * D;                    // bytes of K (V) of a tile
   static constexpr int kStage = kPair * 2 * kTile;
@@ -52,9 +47,9 @@ template <int D, int kN> struct DecCfg {
 
 struct DecParams {
   KParams f;
-  uint32_t* counters;   // [batch * hk * row blocks], of CTAs that have left their sums
-  float* partial;       // [batch * hk * row blocks][splits][rows][D]
-  int splits, tiles, rows;   // CTAs along the keys, tiles of a CTA, rows of a partial block
+  uint32_t* counters;   // [batch * hk], of CTAs that have left their sums
+  float* partial;       // [batch * hk][splits][rows][D]
+  int splits, tiles, rows;   // CTAs along the keys, tiles of a CTA, rows of a partial sum
   int block_shift;      // log2 of a scale's block, 4 at most (a tile has one scale from there on)
   // ceil(2^32 / n): x / n is the upper half of the product, exactly, while x n < 2^32 (a warp with 20 tiles to do feels a
   // handful of divisions)
@@ -67,65 +62,9 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr)
-               : "memory");
-}
-// An 8 x 8 matrix of halves, a row's pair per thread -> its transpose.
-__device__ __forceinline__ uint32_t transposed(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-
-// The four numbers of w as two pairs of halves.
-template <typename H> __device__ __forceinline__ void to_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (std::is_same<H, E4m3>::value) {
-    asm("{\n\t.reg .b16 l, h;\n\t"
-        "mov.b32 {l, h}, %2;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(lo), "=r"(hi)
-        : "r"(w));
-  } else {
-    // 0x6400 + (v + 128) is 1024 + 128 + v
-    const uint32_t u = w ^ 0x80808080u, ul = __byte_perm(u, 0x64646464u, 0x4140), uh = __byte_perm(u, 0x64646464u, 0x4342);
-    const __half2 off = __floats2half2_rn(1152.f, 1152.f);
-    const __half2 l = __hsub2(*reinterpret_cast<const __half2*>(&ul), off), h = __hsub2(*reinterpret_cast<const __half2*>(&uh), off);
-    lo = *reinterpret_cast<const uint32_t*>(&l);
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-}
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
-
-// Clears the status word and the counters; the attention kernel, launched with programmatic stream serialization, streams
-// keys meanwhile and waits before it touches either.
-__global__ void hstu_decode8_init_kernel(uint32_t* header, uint32_t* counters, long long n) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i == 0) header[0] = 0;
-  if (i < n) counters[i] = 0;
-}
-
-template <int D, int kN, typename T, typename H, bool kWin>
+template <int D, typename T, typename H, bool kWin, bool kTanh>
 __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecParams d) {
-  using C = DecCfg<D, kN>;
+  using C = DecCfg<D>;
   using Mask = MaskOf<kWin>;
   const KParams& p = d.f;
   extern __shared__ __align__(128) uint8_t ring_of_all[];
@@ -133,30 +72,16 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   __shared__ long long s_scale[kDecMostTiles];   // where its scales start
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
-  auto over = [](int x, uint32_t inverse) { return static_cast<int>(inverse ? __umulhi(static_cast<uint32_t>(x), inverse) : static_cast<uint32_t>(x)); };
-  const int b = over(blockIdx.x, d.by_hk), hk = blockIdx.x - b * p.hk, split = blockIdx.y, r_first = blockIdx.z * C::kRows;
+  const int b = over(blockIdx.x, d.by_hk), hk = blockIdx.x - b * p.hk, split = blockIdx.y;
 
   const SeqInfo s = load_seq(p, b);
-  const int ratio = p.gqa_ratio, rows = s.lq * ratio - r_first;   // rows of this block, the group's heads inside a query
+  const int ratio = p.gqa_ratio, rows = min(s.lq * ratio, C::kRows);   // the group's heads inside a query
   long long pg0 = load_index(p.page_offsets, p.index_bytes, b), pg1 = load_index(p.page_offsets, p.index_bytes, b + 1);
   if (pg0 < 0) pg0 = 0;
   if (pg1 > p.num_page_ids) pg1 = p.num_page_ids;
-  // What a call's index tensors say wrongly goes into the status word, once per sequence.
-  if (hk == 0 && split == 0 && blockIdx.z == 0) {
-    unsigned st = 0;
-    if (tid == 0) st = check_seq(p, read_seq(p, b)) | check_page_count(p, b);
-    for (long long i = pg0 + tid; i < pg1; i += kDecThreads) {
-      const long long pid = load_index(p.page_ids, p.index_bytes, i);
-      if (pid < 0 || pid >= p.num_pages) st |= HSTU_ST_BAD_PAGES;
-    }
-    if (st) {
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      atomicOr(p.ws_header, st);
-    }
-  }
-  const int q_lo = over(r_first, d.by_ratio), q_n = over(min(rows, C::kRows) + r_first + ratio - 1, d.by_ratio) - q_lo;   // the block's queries
-  const KeyTiles tiles = rows > 0 ? Mask::tiles(p, s, q_lo, q_n, kDecKeys) : KeyTiles{0, 0, 0};
-  // CTAs that share this block's keys, evenly, in whole rounds of the four warps' pairs
+  if (hk == 0 && split == 0) report_sequence<kDecThreads>(p, b, pg0, pg1);
+  const KeyTiles tiles = rows > 0 ? Mask::tiles(p, s, 0, s.lq, kDecKeys) : KeyTiles{0, 0, 0};
+  // CTAs that share the keys, evenly, in whole rounds of the four warps' pairs
   int active = 1;
   while (active * d.tiles < tiles.n) ++active;
   constexpr int kRound = kDecWarps * kPair;
@@ -223,63 +148,42 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
-  // Q: this thread's row of each eight, of each 64 columns the 16 from 16 c on.
-  uint32_t qb[kN][D / 16][2];
-  float factor[kN][2];   // of the rows 2 c and 2 c + 1: alpha and the power of two a row was divided by
-  int query[kN][2];      // and their queries
-#pragma unroll
-  for (int n = 0; n < kN; ++n) {
-    const int r = 8 * n + g;
-    const bool on = r < rows;
-    const int row = on ? r_first + r : 0;
-    const int i_row = over(row, d.by_ratio);
+  // Q: row g, of each 64 columns the 16 from 16 c on.
+  uint32_t qb[D / 16][2];
+  float factor[2];   // of the rows 2 c and 2 c + 1: alpha and the power of two a row was divided by
+  int query[2];      // and their queries
+  {
+    const int row = g < rows ? g : 0, i_row = over(row, d.by_ratio);
     const T* from = static_cast<const T*>(p.q) + ((s.q0 + i_row) * p.hq + hk * ratio + row - i_row * ratio) * p.dqk;
     uint32_t w[D / 8];   // pairs in memory's order
 #pragma unroll
     for (int blk = 0; blk < D / 64; ++blk) {
-      const bool in = on && blk * 64 + 16 * c < p.dqk;
+      const bool in = g < rows && blk * 64 + 16 * c < p.dqk;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const uint4 v = in ? *reinterpret_cast<const uint4*>(from + blk * 64 + 16 * c + 8 * u) : make_uint4(0, 0, 0, 0);
         w[blk * 8 + 4 * u] = v.x, w[blk * 8 + 4 * u + 1] = v.y, w[blk * 8 + 4 * u + 2] = v.z, w[blk * 8 + 4 * u + 3] = v.w;
       }
     }
-    float f = p.alpha;
-    if constexpr (!std::is_same<T, __half>::value) {
-      uint32_t top = 0;   // the largest exponent of the row; an infinity or NaN leaves the row as it is
-#pragma unroll
-      for (int u = 0; u < D / 8; ++u) top = max(top, max(w[u] & 0x7f80u, (w[u] >> 16) & 0x7f80u));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = top == 0x7f80u || top == 0 ? 0 : static_cast<int>(top >> 7) - 127;
-      const float d1 = power_of_two(-(e / 2)), d2 = power_of_two(-(e - e / 2));   // (2^-e itself may lie outside of fp32's normal range)
-      f = p.alpha * power_of_two(e / 2) * power_of_two(e - e / 2);
-#pragma unroll
-      for (int u = 0; u < D / 8; ++u)
-        w[u] = pack2<__half>(__uint_as_float(w[u] << 16) * d1 * d2, __uint_as_float(w[u] & 0xffff0000u) * d1 * d2);
-    }
+    const float f = to_fp16_row<T>(w, p.alpha);
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      factor[n][e] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + e));
-      query[n][e] = over(r_first + min(8 * n + 2 * c + e, rows - 1), d.by_ratio);
+      factor[e] = __shfl_sync(0xffffffffu, f, 4 * (2 * c + e));
+      query[e] = over(min(2 * c + e, rows - 1), d.by_ratio);
     }
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      qb[n][k][0] = w[(k >> 2) * 8 + (k & 3) * 2];
-      qb[n][k][1] = w[(k >> 2) * 8 + (k & 3) * 2 + 1];
+      qb[k][0] = w[(k >> 2) * 8 + (k & 3) * 2];
+      qb[k][1] = w[(k >> 2) * 8 + (k & 3) * 2 + 1];
     }
   }
-  // Tiles that every row of the block sees whole (tile_is_full's rule).
-  const int full_end = min(s.lk, q_lo + (s.lk - s.lq) + 1), full_from = kWin ? win_anchor(s, q_lo + q_n - 1, 0) - p.window : 0;
+  // Tiles that every row sees whole (tile_is_full's rule).
+  const int full_end = min(s.lk, s.lk - s.lq + 1), full_from = kWin ? win_anchor(s, s.lq - 1, 0) - p.window : 0;
 
-  float o[kN][D / 16][4];   // column 2 g of 16 in rows 2 c, 2 c + 1; column 2 g + 1
-  float down[kN][2];        // what P of a row is multiplied by, a power of two
+  float o[D / 16][4];   // column 2 g of 16 in rows 2 c, 2 c + 1; column 2 g + 1
+  float down[2] = {0x1p126f, 0x1p126f};   // what P of a row is multiplied by, a power of two
 #pragma unroll
-  for (int n = 0; n < kN; ++n) {
-    down[n][0] = down[n][1] = 0x1p126f;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
-  }
+  for (int j = 0; j < D / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
   // this thread's places in a stage: K row g and g + 8, V for ldmatrix (lanes 0-7 and 16-23 name keys 0-7, the others 8-15)
   const int v_row = (lane & 7) + ((lane >> 3) & 1) * 8;
 
@@ -291,11 +195,9 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
     const uint32_t at = (i % C::kStages) * C::kStage;
     const uint8_t* const stage = ring_of_all + warp * C::kRing + at;
     const float* const scales = scales_of_mine + (i % C::kStages) * kPair * 2 * kDecKeys;
-    float sc[kPair][kN][4];   // keys g and g + 8, rows 2 c and 2 c + 1
+    float sc[kPair][4];   // keys g and g + 8, rows 2 c and 2 c + 1
 #pragma unroll
-    for (int t = 0; t < kPair; ++t)
-#pragma unroll
-      for (int n = 0; n < kN; ++n) sc[t][n][0] = sc[t][n][1] = sc[t][n][2] = sc[t][n][3] = 0.f;
+    for (int t = 0; t < kPair; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
 #pragma unroll
     for (int blk = 0; blk < D / 64; ++blk) {
       const int ch = D == 128 ? (4 * blk + c) ^ ((g & 1) << 2) : c;
@@ -312,68 +214,55 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
           uint32_t a[4];
           to_halves<H>(reinterpret_cast<const uint32_t*>(&w[t][0])[k], a[0], a[2]);
           to_halves<H>(reinterpret_cast<const uint32_t*>(&w[t][1])[k], a[1], a[3]);
-#pragma unroll
-          for (int n = 0; n < kN; ++n) mma16816(sc[t][n], a, qb[n][4 * blk + k]);
+          mma16816(sc[t], a, qb[4 * blk + k]);
         }
     }
     // P
-    uint32_t pb[kPair][kN][2];
-    float ks[kPair][2], vs[kPair][2];
+    float pv[kPair][4], m[2] = {0.f, 0.f};
     int key[kPair];
     bool full = true;
 #pragma unroll
     for (int t = 0; t < kPair; ++t) {
       const float* at_scales = scales + t * 2 * kDecKeys;
-      ks[t][0] = at_scales[g], ks[t][1] = at_scales[g + 8];
-      vs[t][0] = at_scales[kDecKeys + g], vs[t][1] = at_scales[kDecKeys + g + 8];
+      const float ks[2] = {at_scales[g], at_scales[g + 8]}, vs[2] = {at_scales[kDecKeys + g], at_scales[kDecKeys + g + 8]};
       key[t] = key_of_tile(tiles, t0 + warp + (i * kPair + t) * kDecWarps, kDecKeys);
       full &= key[t] + kDecKeys <= full_end && (!kWin || key[t] > full_from || key[t] + kDecKeys <= p.sink);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) pv[t][e] = silu_of<kTanh>(sc[t][e] * (ks[e >> 1] * factor[e & 1])) * vs[e >> 1];
+    }
+    if (!full) {   // (a select, not a multiply: a masked score may be anything; a tile behind the last one has scales of zero)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const typename Mask::Bounds rb = Mask::bounds(p, s, query[e]);
+#pragma unroll
+        for (int t = 0; t < kPair; ++t) {
+          if (!allowed(rb, key[t] + g)) pv[t][e] = 0.f;
+          if (!allowed(rb, key[t] + g + 8)) pv[t][2 + e] = 0.f;
+        }
+      }
     }
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      float pv[kPair][4];
-      float m[2] = {0.f, 0.f};
+    for (int t = 0; t < kPair; ++t) {
+      m[0] = fmaxf(m[0], fmaxf(fabsf(pv[t][0]), fabsf(pv[t][2])));
+      m[1] = fmaxf(m[1], fmaxf(fabsf(pv[t][1]), fabsf(pv[t][3])));
+    }
+    if (__any_sync(0xffffffffu, m[0] * down[0] > 16384.f || m[1] * down[1] > 16384.f)) {
 #pragma unroll
-      for (int t = 0; t < kPair; ++t)
+      for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = sc[t][n][e] * (ks[t][e >> 1] * factor[n][e & 1]);
-          pv[t][e] = x * ptx::rcp_approx(1.f + ptx::ex2_approx(x * -1.4426950408889634f)) * vs[t][e >> 1];
-        }
-      if (!full) {   // (a select, not a multiply: a masked score may be anything; a tile behind the last one is all masked)
+        for (int x = 4; x < 32; x <<= 1) m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], x));
+        if (!(m[e] * down[e] > 16384.f) || m[e] > 3.402823466e38f) continue;
+        const float next = down_to_one(m[e]), ratio2 = next / down[e];
+        down[e] = next;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const typename Mask::Bounds rb = Mask::bounds(p, s, query[n][e]);
-#pragma unroll
-          for (int t = 0; t < kPair; ++t) {
-            if (!allowed(rb, key[t] + g)) pv[t][e] = 0.f;
-            if (!allowed(rb, key[t] + g + 8)) pv[t][2 + e] = 0.f;
-          }
-        }
+        for (int j = 0; j < D / 16; ++j) o[j][e] *= ratio2, o[j][2 + e] *= ratio2;
       }
+    }
+    uint32_t pb[kPair][2];
 #pragma unroll
-      for (int t = 0; t < kPair; ++t) {
-        m[0] = fmaxf(m[0], fmaxf(fabsf(pv[t][0]), fabsf(pv[t][2])));
-        m[1] = fmaxf(m[1], fmaxf(fabsf(pv[t][1]), fabsf(pv[t][3])));
-      }
-      if (__any_sync(0xffffffffu, m[0] * down[n][0] > 16384.f || m[1] * down[n][1] > 16384.f)) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], x));
-          if (!(m[e] * down[n][e] > 16384.f) || m[e] > 3.402823466e38f) continue;
-          // the row's largest P to [1, 2)
-          const float next = __uint_as_float((254u - min(__float_as_uint(m[e]) >> 23, 253u)) << 23), ratio2 = next / down[n][e];
-          down[n][e] = next;
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) o[n][j][e] *= ratio2, o[n][j][2 + e] *= ratio2;
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < kPair; ++t) {
-        pb[t][n][0] = transposed(pack2<__half>(pv[t][0] * down[n][0], pv[t][1] * down[n][1]));
-        pb[t][n][1] = transposed(pack2<__half>(pv[t][2] * down[n][0], pv[t][3] * down[n][1]));
-      }
+    for (int t = 0; t < kPair; ++t) {
+      pb[t][0] = transposed(pack2<__half>(pv[t][0] * down[0], pv[t][1] * down[1]));
+      pb[t][1] = transposed(pack2<__half>(pv[t][2] * down[0], pv[t][3] * down[1]));
     }
     // O^T += V^T.P^T
     const uint32_t v_at = ring_at + at + C::kTile + v_row * D;
@@ -389,8 +278,7 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
           uint32_t a[4];   // columns 2 g (a pair of keys) and 2 g + 1, keys 0-7; the same, keys 8-15
           to_halves<H>(__byte_perm(w[2 * u], 0u, 0x3120), a[0], a[1]);
           to_halves<H>(__byte_perm(w[2 * u + 1], 0u, 0x3120), a[2], a[3]);
-#pragma unroll
-          for (int n = 0; n < kN; ++n) mma16816(o[n][j + u], a, pb[t][n]);
+          mma16816(o[j + u], a, pb[t]);
         }
       }
     __syncwarp();   // the stage is free
@@ -400,24 +288,21 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   // The warps' outputs, added in order.
   float* all = reinterpret_cast<float*>(ring_of_all);   // [warps][rows][D]
 #pragma unroll
-  for (int n = 0; n < kN; ++n)
+  for (int e = 0; e < 2; ++e) {
+    const float f = 1.f / down[e];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float f = 1.f / down[n][e];
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j)
-        *reinterpret_cast<float2*>(all + (warp * C::kRows + 8 * n + 2 * c + e) * D + 16 * j + 2 * g) = make_float2(o[n][j][e] * f, o[n][j][2 + e] * f);
-    }
+    for (int j = 0; j < D / 16; ++j)
+      *reinterpret_cast<float2*>(all + (warp * C::kRows + 2 * c + e) * D + 16 * j + 2 * g) = make_float2(o[j][e] * f, o[j][2 + e] * f);
+  }
   __syncthreads();
-  const int valid = min(rows, C::kRows);
-  const long long group = static_cast<long long>(blockIdx.x) * gridDim.z + blockIdx.z;
+  const long long group = blockIdx.x;
   auto store = [&](int r, int col, float4 v) {
     if (col >= p.dqk) return;
-    const int row = r_first + r, i_row = over(row, d.by_ratio);
-    T* to = static_cast<T*>(p.out) + ((s.q0 + i_row) * p.hq + hk * ratio + row - i_row * ratio) * p.dqk + col;
+    const int i_row = over(r, d.by_ratio);
+    T* to = static_cast<T*>(p.out) + ((s.q0 + i_row) * p.hq + hk * ratio + r - i_row * ratio) * p.dqk + col;
     *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * p.scale, v.y * p.scale), pack2<T>(v.z * p.scale, v.w * p.scale));
   };
-  for (int i = tid; i < valid * (D / 4); i += kDecThreads) {
+  for (int i = tid; i < rows * (D / 4); i += kDecThreads) {
     const int r = i / (D / 4), col = i % (D / 4) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -436,7 +321,7 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  for (int i = tid; i < valid * (D / 4); i += kDecThreads) {
+  for (int i = tid; i < rows * (D / 4); i += kDecThreads) {
     const int r = i / (D / 4), col = i % (D / 4) * 4;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -448,22 +333,15 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   }
 }
 
-// How a call is split: tiles of a CTA, CTAs along the keys, blocks of rows.
-struct DecPlan {
-  int tiles, splits, row_blocks, rows;
-};
 int tile_width(const KParams& p) { return p.dqk <= 64 ? 64 : 128; }
-// Rows of a CTA: as many groups of eight as its registers hold (1, 2; 4 at width 64).
-int row_groups(const KParams& p) {
-  const long long rows = static_cast<long long>(p.maxq) * p.gqa_ratio;
-  return rows <= 8 ? 1 : rows <= 16 || tile_width(p) == 128 ? 2 : 4;
-}
+
+// How a call is split: tiles of a CTA, CTAs along the keys.
+struct DecPlan {
+  int tiles, splits, rows;
+};
 DecPlan plan(const KParams& p) {
   DecPlan d;
-  const long long rows = static_cast<long long>(p.maxq) * p.gqa_ratio;
-  const int at_once = 8 * row_groups(p);
-  d.row_blocks = static_cast<int>((rows + at_once - 1) / at_once);
-  d.rows = rows < at_once ? static_cast<int>(rows) : at_once;
+  d.rows = p.maxq * p.gqa_ratio;
   long long most = (p.maxk + kDecKeys - 1) / kDecKeys;   // tiles of the longest sequence
   long long all = p.num_page_ids * p.page_size / kDecKeys;   // and of all of them together, at most
   if (p.window) {
@@ -474,7 +352,7 @@ DecPlan plan(const KParams& p) {
   // Some six CTAs per SM (three fit): fewer, and sequences of different lengths do not even out; more, and set-up and partial
   // sums - a thousand instructions a warp, where a tile takes 300 - are what the SMs do.  Attention alone, us, at 4 / 6 / 8 /
   // 12: 128 users of 200 - 2048 rows and 8 heads 64 / 66 / 70 / 75, 4 users of 14000 - 20000 44 / 39 / 45 / 50.
-  long long tiles = all * p.hk * d.row_blocks / (6ll * 148);
+  long long tiles = all * p.hk / (6ll * 148);
   tiles = tiles < 8 ? 8 : tiles > kDecMostTiles ? kDecMostTiles : tiles;
   constexpr int kRound = kDecWarps * kPair;
   d.tiles = static_cast<int>((tiles + kRound - 1) / kRound * kRound);
@@ -482,18 +360,20 @@ DecPlan plan(const KParams& p) {
   if (d.splits < 1) d.splits = 1;
   return d;
 }
-uint64_t counters_bytes(const KParams& p, const DecPlan& d) {
-  return (static_cast<uint64_t>(p.batch) * p.hk * d.row_blocks * 4 + 255) & ~static_cast<uint64_t>(255);
+uint64_t counters_bytes(const KParams& p) {
+  return (static_cast<uint64_t>(p.batch) * p.hk * 4 + 255) & ~static_cast<uint64_t>(255);
 }
 
-template <int D, int kN, typename T, typename H>
-cudaError_t launch_dec_of(const DecParams& d, const DecPlan& pl, cudaStream_t stream) {
-  using C = DecCfg<D, kN>;
-  auto kern = d.f.window ? hstu_decode8_kernel<D, kN, T, H, true> : hstu_decode8_kernel<D, kN, T, H, false>;
+template <int D, typename T, typename H>
+cudaError_t launch_dec(const DecParams& d, const DecPlan& pl, cudaStream_t stream) {
+  using C = DecCfg<D>;
+  constexpr bool kBf16 = !std::is_same<T, __half>::value;
+  auto kern = kBf16 && tanh_silu(d.f) ? (d.f.window ? hstu_decode8_kernel<D, T, H, true, kBf16> : hstu_decode8_kernel<D, T, H, false, kBf16>)
+                                      : (d.f.window ? hstu_decode8_kernel<D, T, H, true, false> : hstu_decode8_kernel<D, T, H, false, false>);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(d.f.batch) * d.f.hk, pl.splits, pl.row_blocks);
+  cfg.gridDim = dim3(static_cast<unsigned>(d.f.batch) * d.f.hk, pl.splits, 1);
   cfg.blockDim = dim3(kDecThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
@@ -504,15 +384,6 @@ cudaError_t launch_dec_of(const DecParams& d, const DecPlan& pl, cudaStream_t st
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, d);
 }
-template <int D, typename T, typename H>
-cudaError_t launch_dec(const DecParams& d, const DecPlan& pl, cudaStream_t stream) {
-  switch (row_groups(d.f)) {
-    case 1: return launch_dec_of<D, 1, T, H>(d, pl, stream);
-    case 2: return launch_dec_of<D, 2, T, H>(d, pl, stream);
-    default: return launch_dec_of<64, 4, T, H>(d, pl, stream);   // (of width 64 only)
-  }
-}
-
 }  // namespace
 
 // Whether a call runs here.  The pointers count: rows are read in pieces of 16 bytes.
@@ -521,13 +392,13 @@ bool decode8_supported(const KParams& p, int dtype) {
   const bool blocks = p.scale_block % kDecKeys == 0 || kDecKeys % p.scale_block == 0;
   return (dtype == HSTU_DTYPE_BF16 || dtype == HSTU_DTYPE_FP16) && p.dqk % 16 == 0 && p.dqk <= 128 && !p.tgt && blocks &&
          p.page_size % kDecKeys == 0 && (align & 15u) == 0 && !(p.flags & HSTU_FLAG_FORCE_GENERIC) &&
-         static_cast<long long>(p.maxq) * p.gqa_ratio <= 64;
+         static_cast<long long>(p.maxq) * p.gqa_ratio <= DecCfg<64>::kRows;
 }
 
 uint64_t decode8_workspace(const KParams& p) {
   const DecPlan d = plan(p);
-  const uint64_t partial = d.splits > 1 ? static_cast<uint64_t>(p.batch) * p.hk * d.row_blocks * d.splits * d.rows * tile_width(p) * 4 : 0;
-  return kWsHeaderBytes + counters_bytes(p, d) + partial;
+  const uint64_t partial = d.splits > 1 ? static_cast<uint64_t>(p.batch) * p.hk * d.splits * d.rows * tile_width(p) * 4 : 0;
+  return kWsHeaderBytes + counters_bytes(p) + partial;
 }
 
 cudaError_t launch_decode8(const KParams& p, int dtype, void* workspace, cudaStream_t stream) {
@@ -537,20 +408,19 @@ cudaError_t launch_decode8(const KParams& p, int dtype, void* workspace, cudaStr
   d.f.ws_header = static_cast<uint32_t*>(workspace);
   char* base = static_cast<char*>(workspace) + kWsHeaderBytes;
   d.counters = reinterpret_cast<uint32_t*>(base);
-  d.partial = reinterpret_cast<float*>(base + counters_bytes(p, pl));
+  d.partial = reinterpret_cast<float*>(base + counters_bytes(p));
   d.splits = pl.splits;
   d.tiles = pl.tiles;
   d.rows = pl.rows;
-  // (at most 2^20 heads of sequences by 16, 64 rows by 16, 20480 keys by a page of any size; of 1: 0)
-  auto inverse = [](int n) { return n == 1 ? 0u : static_cast<uint32_t>(((1ull << 32) + n - 1) / n); };
-  d.by_hk = inverse(p.hk);
-  d.by_ratio = inverse(p.gqa_ratio);
-  d.by_page = inverse(p.page_size);
-  d.by_block = inverse(p.scale_block);
+  // (at most 2^20 heads of sequences by 16, 8 rows by 8, 20480 keys by a page of any size)
+  d.by_hk = inverse_of(p.hk);
+  d.by_ratio = inverse_of(p.gqa_ratio);
+  d.by_page = inverse_of(p.page_size);
+  d.by_block = inverse_of(p.scale_block);
   d.block_shift = 4;
   while (d.block_shift > 0 && (1 << d.block_shift) > p.scale_block) --d.block_shift;
-  const long long n = pl.splits > 1 ? static_cast<long long>(p.batch) * p.hk * pl.row_blocks : 0;
-  hstu_decode8_init_kernel<<<static_cast<unsigned>(n / 256 + 1), 256, 0, stream>>>(d.f.ws_header, d.counters, n);
+  const long long n = pl.splits > 1 ? static_cast<long long>(p.batch) * p.hk : 0;
+  clear_kernel<<<static_cast<unsigned>(n / 256 + 1), 256, 0, stream>>>(d.f.ws_header, d.counters, n);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.total_q == 0) return e;
   const bool wide = tile_width(p) == 128, held = p.held == HSTU_HELD_E4M3;
