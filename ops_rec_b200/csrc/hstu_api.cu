@@ -37,6 +37,8 @@ cudaError_t launch_in_linear_silu_bwd(const LinSiluParams& shape, const void* x,
 cudaError_t launch_paged_gather(const KParams& p, const void* kv_cache, const void* k_in, const void* v_in,
                                 void* k_out, void* v_out, long long capacity, long long num_pages,
                                 long long num_page_ids, int dtype, cudaStream_t stream);
+bool unpack_supported(const KParams& p, int dtype);
+cudaError_t launch_unpack(const KParams& p, void* out, void* table, int dtype, cudaStream_t stream);
 bool decode8_supported(const KParams& p, int dtype);
 uint64_t decode8_workspace(const KParams& p);
 cudaError_t launch_decode8(const KParams& p, int dtype, void* workspace, cudaStream_t stream);
@@ -487,10 +489,37 @@ static hstu::KParams paged8_params(const HstuPaged8Args* args, const PagedPlan& 
   p.v_new = a->base.v;
   return p;
 }
-static uint64_t paged8_workspace(const hstu::KParams& p, const PagedPlan& pl) {
-  if (hstu::decode8_supported(p, pl.fwd.dtype)) return hstu::decode8_workspace(p);
-  if (hstu::rows8_supported(p, pl.fwd.dtype)) return hstu::rows8_workspace(p);
-  return pl.fwd_bytes + 2 * pl.stage_bytes;
+// How a call runs: on one of the two kernels that read the cache as it lies, or on the kernels of hstu_paged - those that read
+// pages in place from unpacked copies of the pages, the others from staging tensors.
+enum Paged8Path { kDecode8, kRows8, kUnpacked, kStaged };
+// Where more than eight rows can also be unpacked for tcgen05, the kernel that reads the cache in place is the better one for
+// few rows, or for few problems (its CTAs are chains of small steps, and a problem's beginning and end weigh as much as its
+// tiles).  us in place / unpacked: 512 users of 50 - 1000 rows, 4 heads of 64, 11 rows 150 / 172, 26 rows 160 / 174, 80 rows
+// 212 / 168; of 128: 245 / 307, 264 / 309, 342 / 297; 64 such users, 80 rows: 43 / 74, 68 / 118.  Where it cannot be unpacked,
+// beside the staging tensors: 128 users of 200 - 2048 rows, 8 heads of 128, 9 / 64 rows 250 / 664, 323 / 732; 4 users of
+// 14000 - 20000, 64 rows 234 / 532.
+static Paged8Path paged8_path(const HstuPaged8Args* args, const PagedPlan& pl, const hstu::KParams& p) {
+  if (hstu::decode8_supported(p, pl.fwd.dtype)) return kDecode8;
+  hstu::KParams u = p;
+  u.k = pl.fwd.k;
+  u.v = pl.fwd.v;
+  u.num_pages = p.num_page_ids;
+  const bool unpacked = wants_tc(&args->paged.base, u) && hstu::unpack_supported(p, pl.fwd.dtype) && hstu::short_paged_split(u);
+  const long long rows = static_cast<long long>(p.maxq) * p.gqa_ratio;
+  const bool few = rows <= 32 || static_cast<long long>(p.batch) * p.hk * ((rows + 63) / 64) <= 512;
+  if (hstu::rows8_supported(p, pl.fwd.dtype) && (few || !unpacked)) return kRows8;
+  return unpacked ? kUnpacked : kStaged;
+}
+static uint64_t unpacked_bytes(const hstu::KParams& p) {   // of the pages; their table follows
+  return (static_cast<uint64_t>(p.num_page_ids) * 2 * p.page_size * p.hk * p.dqk * 2 + 255) & ~static_cast<uint64_t>(255);
+}
+static uint64_t paged8_workspace(Paged8Path path, const hstu::KParams& p, const PagedPlan& pl) {
+  switch (path) {
+    case kDecode8: return hstu::decode8_workspace(p);
+    case kRows8: return hstu::rows8_workspace(p);
+    case kUnpacked: return pl.fwd_bytes + unpacked_bytes(p) + static_cast<uint64_t>(p.num_page_ids) * p.index_bytes;
+    default: return pl.fwd_bytes + 2 * pl.stage_bytes;
+  }
 }
 
 int hstu_paged_8bit_fwd_get_workspace_size(const HstuPaged8Args* args, uint64_t* workspace_bytes) {
@@ -499,7 +528,8 @@ int hstu_paged_8bit_fwd_get_workspace_size(const HstuPaged8Args* args, uint64_t*
   PagedPlan pl;
   const int rc = plan_paged8(args, &pl);
   if (rc) return rc;
-  *workspace_bytes = paged8_workspace(paged8_params(args, pl), pl);
+  const hstu::KParams p = paged8_params(args, pl);
+  *workspace_bytes = paged8_workspace(paged8_path(args, pl, p), p, pl);
   return HSTU_OK;
 }
 
@@ -516,20 +546,20 @@ int hstu_paged_8bit_fwd(const HstuPaged8Args* args, void* workspace, uint64_t wo
   if (reinterpret_cast<uintptr_t>(args->kv_scale) & 3u) return fail(HSTU_E_PARAM, "kv_scale must be 4-byte aligned");
   if (b->total_q > 0 && (!b->q || !b->out || !b->k || !b->v)) return fail(HSTU_E_NULL, "q / k / v / out is null");
   hstu::KParams p = paged8_params(args, pl);
-  const uint64_t need = paged8_workspace(p, pl);
+  const Paged8Path path = paged8_path(args, pl, p);
+  const uint64_t need = paged8_workspace(path, p, pl);
   if (!workspace) return fail(HSTU_E_WORKSPACE, "workspace is null (%llu bytes needed)", (unsigned long long)need);
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(HSTU_E_WORKSPACE, "workspace must be 256-byte aligned");
   if (workspace_bytes < need)
     return fail(HSTU_E_WORKSPACE, "workspace has %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
                 (unsigned long long)need);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  const bool few = hstu::decode8_supported(p, pl.fwd.dtype);
-  if (few || hstu::rows8_supported(p, pl.fwd.dtype)) {
+  if (path == kDecode8 || path == kRows8) {
     DeviceInfo dev;
     rc = device_info(&dev);
     if (rc) return rc;
     if (dev.major != 10) return fail(HSTU_E_ARCH, "this library is built for sm_100a only; device has compute capability %d.x", dev.major);
-    const cudaError_t e = few ? hstu::launch_decode8(p, pl.fwd.dtype, workspace, stream) : hstu::launch_rows8(p, pl.fwd.dtype, workspace, stream);
+    const cudaError_t e = path == kDecode8 ? hstu::launch_decode8(p, pl.fwd.dtype, workspace, stream) : hstu::launch_rows8(p, pl.fwd.dtype, workspace, stream);
     return e == cudaSuccess ? HSTU_OK : fail(HSTU_E_CUDA, "kernel launch: %s", cudaGetErrorString(e));
   }
   char* base = static_cast<char*>(workspace);
@@ -537,6 +567,18 @@ int hstu_paged_8bit_fwd(const HstuPaged8Args* args, void* workspace, uint64_t wo
   pl.fwd.out = b->out;
   pl.fwd.k = base + pl.fwd_bytes;
   pl.fwd.v = base + pl.fwd_bytes + pl.stage_bytes;
+  if (path == kUnpacked) {
+    void* pages = base + pl.fwd_bytes;
+    void* table = base + pl.fwd_bytes + unpacked_bytes(p);
+    pl.fwd.k = pl.fwd.v = pages;   // (not read: keys and values are the pages and the call's own rows)
+    const cudaError_t e = hstu::launch_unpack(p, pages, table, pl.fwd.dtype, stream);
+    if (e != cudaSuccess) return fail(HSTU_E_CUDA, "unpack launch: %s", cudaGetErrorString(e));
+    p.kv_cache = pages;
+    p.page_ids = table;
+    p.num_pages = p.num_page_ids;
+    p.paged_split = 1;
+    return jagged_fwd_impl(&pl.fwd, workspace, pl.fwd_bytes, stream_v, &p);
+  }
   const cudaError_t e = hstu::launch_paged_gather(p, a->kv_cache, b->k, b->v, base + pl.fwd_bytes, base + pl.fwd_bytes + pl.stage_bytes,
                                                   pl.capacity, a->num_pages, a->num_page_ids, pl.fwd.dtype, stream);
   if (e != cudaSuccess) return fail(HSTU_E_CUDA, "gather launch: %s", cudaGetErrorString(e));

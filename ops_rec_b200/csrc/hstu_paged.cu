@@ -19,7 +19,7 @@
 // with the cached rows turned into the call's type, number * scale rounded once, on the way.
 #include <type_traits>
 
-#include "hstu_held.cuh"
+#include "hstu_mma8.cuh"
 #include "hstu_simt.cuh"
 
 namespace hstu {
@@ -239,7 +239,151 @@ __global__ void __launch_bounds__(kGatherThreads) hstu_paged_gather_kernel(const
   }
 }
 
+// hstu_paged_8bit, calls that the kernel for short sequences then reads in place: the pages of the table, slot by slot, in the
+// call's type - a cache of its own whose page i is slot i, with the table of its pages.  Rows nobody reads (behind a sequence's
+// last one, and a whole tile of 64 keys away from what a window or its sinks show) stay unwritten.  HBM-bound: one byte in, two
+// out (10 600 pages of 128 rows, 4 heads of 64: 1.0 GB).
+constexpr int kUnpackThreads = 256;
+
+struct UnpackParams {
+  const unsigned char* cache;   // [pages, 2, page_size, heads, dim]
+  const float* scale;
+  void* out;                    // [num_page_ids, 2, page_size, heads, dim]
+  void* table;                  // [num_page_ids]: 0, 1, 2, .. (-1: not a page of the cache)
+  const void* offq;
+  const void* offk;
+  const void* tgt;
+  const void* page_offsets;
+  const void* page_ids;
+  long long num_pages, num_page_ids;
+  int index_bytes, batch, page_size, block, heads, dim, window, sink;
+  uint32_t by_row, by_head, by_block;   // over(): chunks of a row, chunks of a head, rows of a block
+};
+
+template <typename T, typename H>
+__global__ void __launch_bounds__(kUnpackThreads) hstu_unpack_kernel(const UnpackParams p) {
+  __shared__ int s_b;
+  const long long slot = blockIdx.x;
+  if (threadIdx.x < 32) {   // the last sequence whose first slot is <= slot, by a 32-way search
+    const int lane = threadIdx.x;
+    int lo = 0, hi = p.batch - 1;
+    while (hi > lo) {
+      const int stride = (hi - lo + 31) >> 5;
+      auto probe = [&](int l) { const int at = lo + (l + 1) * stride; return at < hi ? at : hi; };
+      const bool le = load_index(p.page_offsets, p.index_bytes, probe(lane)) <= slot;
+      const int c = __popc(__ballot_sync(0xffffffffu, le));
+      if (c == 0) {
+        hi = probe(0) - 1;
+      } else {
+        const int nlo = probe(c - 1);
+        if (c < 32) hi = probe(c) - 1 > nlo ? probe(c) - 1 : nlo;
+        lo = nlo;
+      }
+    }
+    if (lane == 0) s_b = lo;
+  }
+  __syncthreads();
+  const int b = s_b;
+  const long long pid = load_index(p.page_ids, p.index_bytes, slot);
+  const bool ok = pid >= 0 && pid < p.num_pages;
+  if (threadIdx.x == 0) {   // (a page outside of the cache stays one, for the pre-pass's check)
+    if (p.index_bytes == 8) static_cast<long long*>(p.table)[slot] = ok ? slot : -1;
+    else static_cast<int*>(p.table)[slot] = ok ? static_cast<int>(slot) : -1;
+  }
+  const long long first = (slot - load_index(p.page_offsets, p.index_bytes, b)) * p.page_size;   // the page's first key
+  const long long lk = load_index(p.offk, p.index_bytes, b + 1) - load_index(p.offk, p.index_bytes, b);
+  const long long lq = load_index(p.offq, p.index_bytes, b + 1) - load_index(p.offq, p.index_bytes, b);
+  long long t = p.tgt ? load_index(p.tgt, p.index_bytes, b) : 0;
+  if (t < 0) t = 0;
+  const long long cached = lk - t;
+  // rows [0, n) of the page are read; with a window, those below `skip_from` and from `skip_to` on
+  long long n = cached - first;
+  n = n < 0 ? 0 : n > p.page_size ? p.page_size : n;
+  long long skip_from = n, skip_to = n;
+  if (p.window) {
+    long long lo = lk - lq - p.window + 1;
+    lo = lo < 0 ? 0 : lo / 64 * 64;
+    const long long sinks = (p.sink + 63ll) / 64 * 64;
+    skip_from = sinks - first < 0 ? 0 : sinks - first;
+    skip_to = lo - first < skip_from ? skip_from : lo - first;
+  }
+  const int row_len = p.heads * p.dim, per_page = p.page_size / p.block;
+  const long long page_len = static_cast<long long>(p.page_size) * row_len;
+  const uint4* from = reinterpret_cast<const uint4*>(p.cache + (ok ? pid : 0) * 2 * page_len);
+  const float* scale = p.scale + (ok ? pid : 0) * 2 * per_page * static_cast<long long>(p.heads);
+  uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + slot * 2 * page_len);
+  const int chunks = static_cast<int>(n) * (row_len / 16);   // of 16 numbers, of the keys; as many of the values
+  constexpr int kFly = 4;
+  for (int i0 = threadIdx.x; i0 < 2 * chunks; i0 += kFly * kUnpackThreads) {
+    uint4 w[kFly];
+    float f[kFly];
+    long long at[kFly];   // of the chunk in the page, -1: nothing to do
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      const int both = i0 + u * kUnpackThreads, kv = both >= chunks ? 1 : 0, i = both - kv * chunks;
+      const int row = over(i, p.by_row), head = over(i - row * (row_len / 16), p.by_head);
+      at[u] = i < chunks && (row < skip_from || row >= skip_to) ? kv * (page_len / 16) + i : -1;
+      w[u] = make_uint4(0, 0, 0, 0);
+      f[u] = 0.f;
+      if (at[u] >= 0 && ok) {
+        w[u] = __ldcs(from + at[u]);
+        f[u] = __ldg(scale + (kv * per_page + over(row, p.by_block)) * p.heads + head);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kFly; ++u) {
+      if (at[u] < 0) continue;
+      alignas(16) T x[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] = simt::from_float<T>(H::to_float(reinterpret_cast<const uint8_t*>(&w[u])[e]) * f[u]);
+      to[2 * at[u]] = reinterpret_cast<const uint4*>(x)[0];
+      to[2 * at[u] + 1] = reinterpret_cast<const uint4*>(x)[1];
+    }
+  }
+}
+
 }  // namespace
+
+// Whether a cache of 8-bit rows can be unpacked page by page: pieces of 16 numbers of one head.
+bool unpack_supported(const KParams& p, int dtype) {
+  return dtype != HSTU_DTYPE_FP32 && p.dqk % 16 == 0 && (reinterpret_cast<uintptr_t>(p.kv_cache) & 15u) == 0 &&
+         p.page_size <= 65536 && static_cast<long long>(p.page_size) * p.hk * p.dqk / 16 < (1ll << 21) &&
+         p.num_page_ids <= 0x7fffffffll;
+}
+cudaError_t launch_unpack(const KParams& p, void* out, void* table, int dtype, cudaStream_t stream) {
+  UnpackParams u;
+  u.cache = static_cast<const unsigned char*>(p.kv_cache);
+  u.scale = p.kv_scale;
+  u.out = out;
+  u.table = table;
+  u.offq = p.offq;
+  u.offk = p.offk;
+  u.tgt = p.tgt;
+  u.page_offsets = p.page_offsets;
+  u.page_ids = p.page_ids;
+  u.num_pages = p.num_pages;
+  u.num_page_ids = p.num_page_ids;
+  u.index_bytes = p.index_bytes;
+  u.batch = p.batch;
+  u.page_size = p.page_size;
+  u.block = p.scale_block;
+  u.heads = p.hk;
+  u.dim = p.dqk;
+  u.window = p.window;
+  u.sink = p.sink;
+  // (at most 2^22 chunks by 512 of a row, 512 by 32 of a head, 2^16 rows by as many of a block)
+  u.by_row = inverse_of(p.hk * p.dqk / 16);
+  u.by_head = inverse_of(p.dqk / 16);
+  u.by_block = inverse_of(p.scale_block);
+  const dim3 grid(static_cast<unsigned>(p.num_page_ids), 1, 1);
+#define HSTU_UNPACK(TT)                                                                                            \
+  if (p.held == HSTU_HELD_E4M3) hstu_unpack_kernel<TT, E4m3><<<grid, kUnpackThreads, 0, stream>>>(u);             \
+  else hstu_unpack_kernel<TT, Int8><<<grid, kUnpackThreads, 0, stream>>>(u)
+  if (dtype == HSTU_DTYPE_BF16) { HSTU_UNPACK(__nv_bfloat16); }
+  else { HSTU_UNPACK(__half); }
+#undef HSTU_UNPACK
+  return cudaGetLastError();
+}
 
 template <typename T, int kN>
 static void launch_held(const GatherParams& g, int held, dim3 grid, cudaStream_t stream) {

@@ -5,8 +5,8 @@
 // 128 us of bytes, 28 us of products on the tcgen05 pipe, but 260 million scores, 59 us of SFU) and the latency of a problem this
 // small: a (user, head) has 17 tiles of 16 keys.  So as in the decode kernel nothing is staged in memory, and the matrix
 // instructions have the cache as their A operand; but here a warp owns rows - two groups of eight - and all four warps of a CTA
-// share the tiles: each 32 keys are fetched into registers while the 32 before are worked on, turned into fp16 once, and put
-// into one of two buffers in shared memory, one barrier per 32 keys.
+// share the tiles: 32 keys at a time arrive in a ring of raw numbers (cp.async, three stages ahead; each thread reads back only
+// what it fetched itself), are turned into fp16 once, and put into one of two buffers, one barrier per 32 keys.
 //   S^T = K.Q^T, O^T += V^T.P^T   ldmatrix, for V with .trans; P changes from accumulator to operand with movmatrix
 //   P    SiLU(x) times the value's scale and the row's power of two (see hstu_decode8.cu), rounded once; the products around SiLU
 //        on pairs of scores (tanh on two halves at once is no faster, and 1 + tanh from halves is 2^-12 off where it is small)
@@ -18,20 +18,22 @@ namespace hstu {
 
 namespace {
 
-constexpr int kRwWarps = 4, kRwThreads = 32 * kRwWarps;
 constexpr int kRwKeys = 16;        // keys of a tile
 constexpr int kRwStage = 32;       // keys of a stage: two tiles
-constexpr int kRwGroups = 2;       // groups of eight rows of a warp
-constexpr int kRwRows = 8 * kRwGroups * kRwWarps;
+constexpr int kRwRows = 64;        // of a CTA
 constexpr int kRwMostTiles = 128;  // of a CTA
 constexpr int kRwMostGroup = 4;    // targets of a group
 constexpr int kRwMostRows = 256;   // of a sequence and key head
 
 template <int D> struct RwCfg {
+  static constexpr int kGroups = 2, kWarps = kRwRows / 8 / kGroups, kThreads = 32 * kWarps;   // groups of eight rows of a warp
   static constexpr int kTile = kRwStage * D * 2;       // bytes of a stage's K (V) in fp16
   static constexpr int kPitch = D + 4;                 // of the output's rows in floats: eight columns of four rows, 32 banks
   static constexpr int kOut = kRwRows * kPitch * 4;
-  static constexpr int kSmem = 4 * kTile > kOut ? 4 * kTile : kOut;
+  static constexpr int kDepth = 4;                     // stages of the ring of raw numbers
+  static constexpr int kRaw = kRwStage * D * 2;        // bytes of a stage: K and V
+  static constexpr int kBuffers = 4 * kTile > kOut ? 4 * kTile : kOut;
+  static constexpr int kSmem = kBuffers + kDepth * (kRaw + 2 * kRwStage * 4);
 };
 
 struct RwParams {
@@ -44,6 +46,12 @@ struct RwParams {
 };
 
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {   // (off: zeros)
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
 template <bool kTanh> __device__ __forceinline__ float2 silu_pair(float2 x) {
   if (kTanh) {
     const float2 h = __fmul2_rn(x, make_float2(0.5f, 0.5f));
@@ -53,11 +61,12 @@ template <bool kTanh> __device__ __forceinline__ float2 silu_pair(float2 x) {
 }
 
 template <int D, typename T, typename H, bool kWin, bool kTanh>
-__global__ void __launch_bounds__(kRwThreads) hstu_rows8_kernel(const RwParams d) {
+__global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const RwParams d) {
   using C = RwCfg<D>;
+  constexpr int kRwGroups = C::kGroups, kRwWarps = C::kWarps, kRwThreads = C::kThreads;
   using Mask = MaskOf<kWin>;
   const KParams& p = d.f;
-  extern __shared__ __align__(128) uint8_t smem[];   // [2][K, V][32][D] halves; at the end the output
+  extern __shared__ __align__(256) uint8_t smem[];   // [2][K, V][32][D] halves; at the end the output
   __shared__ long long s_row[kRwMostTiles];          // where the tile's keys start in the cache, -1: no such page
   __shared__ long long s_scale[kRwMostTiles];        // and its scales
   __shared__ float s_factor[2][2][kRwStage];         // scales of a stage's keys and values
@@ -101,43 +110,45 @@ __global__ void __launch_bounds__(kRwThreads) hstu_rows8_kernel(const RwParams d
   }
   __syncthreads();
 
-  // This thread's 16 numbers of a stage: row my_row (and, 128 wide, my_row + 16), chunk my_chunk; and, of 64 threads, a scale.
-  constexpr int kChunks = D / 16, kPer = D / 64, kStep = kRwStage / kPer;
+  // This thread's numbers of a stage: chunk my_chunk of the rows my_row, my_row + 16; and, of 64 threads, a scale.
+  constexpr int kChunks = D / 16, kStep = kRwThreads / kChunks, kPer = kRwStage / kStep;
   const int my_row = tid / kChunks, my_chunk = tid % kChunks;
   const bool in_row = my_chunk * 16 < p.dqk;
   const long long to_v = static_cast<long long>(p.page_size) * row_bytes;
   const uint8_t* const from = static_cast<const uint8_t*>(p.kv_cache) + hk * p.dqk + my_chunk * 16;
-  uint4 raw_k[kPer], raw_v[kPer];
-  float raw_scale = 0.f;
+  uint8_t* const raw = smem + C::kBuffers + tid * 16;                                               // [kDepth][kPer][K, V][threads]
+  float* const raw_scale = reinterpret_cast<float*>(smem + C::kBuffers + C::kDepth * C::kRaw) + tid;   // [kDepth][2 * 32]
   // Rows behind the last cached one, chunks behind the head and tiles behind the last read as zeros.
   auto fetch = [&](int stage) {
+    const int slot = stage % C::kDepth;
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const int r = my_row + u * kStep, tile = 2 * stage + (r >> 4);
-      raw_k[u] = raw_v[u] = make_uint4(0, 0, 0, 0);
-      if (tile < nt && in_row && s_row[tile] >= 0 && key_of_tile(tiles, t0 + tile, kRwKeys) + (r & 15) < cached) {
-        const uint8_t* at = from + s_row[tile] + (r & 15) * row_bytes;
-        raw_k[u] = __ldg(reinterpret_cast<const uint4*>(at));
-        raw_v[u] = __ldg(reinterpret_cast<const uint4*>(at + to_v));
-      }
+      const bool on = tile < nt && in_row && s_row[tile] >= 0 && key_of_tile(tiles, t0 + tile, kRwKeys) + (r & 15) < cached;
+      const uint8_t* at = on ? from + s_row[tile] + (r & 15) * row_bytes : static_cast<const uint8_t*>(p.kv_cache);
+      const uint32_t to = ptx::smem_u32(raw + slot * C::kRaw + u * 2 * kRwThreads * 16);
+      cp16(to, at, on);
+      cp16(to + kRwThreads * 16, on ? at + to_v : at, on);
     }
     if (tid < 2 * kRwStage) {
       const int r = tid & (kRwStage - 1), tile = 2 * stage + (r >> 4);
-      raw_scale = 0.f;
-      if (tile < nt && s_row[tile] >= 0 && key_of_tile(tiles, t0 + tile, kRwKeys) + (r & 15) < cached)
-        raw_scale = __ldg(p.kv_scale + s_scale[tile] + ((tid < kRwStage ? 0 : per_page) + ((r & 15) >> d.block_shift)) * static_cast<long long>(p.hk));
+      const bool on = tile < nt && s_row[tile] >= 0 && key_of_tile(tiles, t0 + tile, kRwKeys) + (r & 15) < cached;
+      const float* at = on ? p.kv_scale + s_scale[tile] + ((tid < kRwStage ? 0 : per_page) + ((r & 15) >> d.block_shift)) * static_cast<long long>(p.hk)
+                           : p.kv_scale;
+      cp4(ptx::smem_u32(raw_scale + slot * 2 * kRwStage), at, on);
     }
   };
   // a 16-byte chunk (eight halves) of row r: eight rows' chunks of one column lie in different banks
   auto place = [](int r, int chunk) { return r * D * 2 + (((chunk ^ r) & 7) | (chunk & 8)) * 16; };
-  auto convert = [&](int buf) {
+  auto convert = [&](int stage) {
+    const int buf = stage & 1, slot = stage % C::kDepth;
     uint8_t* to = smem + buf * 2 * C::kTile;
 #pragma unroll
     for (int u = 0; u < kPer; ++u) {
       const int r = my_row + u * kStep;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        const uint4 w = kv ? raw_v[u] : raw_k[u];
+        const uint4 w = *reinterpret_cast<const uint4*>(raw + slot * C::kRaw + (u * 2 + kv) * kRwThreads * 16);
         uint4 lo, hi;
         to_halves<H>(w.x, lo.x, lo.y);
         to_halves<H>(w.y, lo.z, lo.w);
@@ -147,9 +158,17 @@ __global__ void __launch_bounds__(kRwThreads) hstu_rows8_kernel(const RwParams d
         *reinterpret_cast<uint4*>(to + kv * C::kTile + place(r, 2 * my_chunk + 1)) = hi;
       }
     }
-    if (tid < 2 * kRwStage) s_factor[buf][tid / kRwStage][tid % kRwStage] = raw_scale;
+    if (tid < 2 * kRwStage) s_factor[buf][tid / kRwStage][tid % kRwStage] = raw_scale[slot * 2 * kRwStage];
   };
-  fetch(0);
+  auto commit = [] { asm volatile("cp.async.commit_group;" ::: "memory"); };
+  // (the stages up to the one that is converted next are complete)
+  auto arrived = [] { asm volatile("cp.async.wait_group %0;" ::"n"(C::kDepth - 2) : "memory"); };
+  const int stages = (nt + 1) / 2;
+#pragma unroll
+  for (int i = 0; i < C::kDepth - 1; ++i) {
+    if (i < stages) fetch(i);
+    commit();
+  }
 
   // Q: the warp's groups warp and warp + 4, row g of each.
   uint32_t qb[kRwGroups][D / 16][2];
@@ -181,25 +200,34 @@ __global__ void __launch_bounds__(kRwThreads) hstu_rows8_kernel(const RwParams d
     constexpr int kLanes = D / 8;
     const int part = tid % kLanes;
     const bool in = part * 8 < p.dqk;
-    for (int r0 = 0; r0 < rows; r0 += kRwThreads / kLanes) {   // (uniform: the lanes of a row reduce together)
-      const int r = r0 + tid / kLanes, row = min(r_first + r, r_first + rows - 1), i_row = over(row, d.by_ratio);
-      const int nth = i_row - hist_rows, first = nth < 0 ? 0 : over(nth, d.by_group) * p.group;
-      uint4 q4 = make_uint4(0, 0, 0, 0);
-      if (in && nth >= 0)
-        q4 = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + ((s.q0 + i_row) * p.hq + hk * ratio + row - i_row * ratio) * p.dqk + part * 8));
-      for (int j = 0; j < p.group; ++j) {   // (up to four, the same for all)
-        uint4 k4 = make_uint4(0, 0, 0, 0);
-        const bool on = nth >= 0 && first + j <= nth;
-        if (in && on) k4 = __ldg(reinterpret_cast<const uint4*>(k_new + static_cast<long long>(first + j) * row_bytes + part * 8));
-        float x = 0.f;
+    constexpr int kAtOnce = kRwThreads / kLanes, kPasses = kRwRows / kAtOnce, kFly = 4;
+    for (int pass = 0; pass < kPasses && pass * kAtOnce < rows; pass += kFly) {
+      for (int j = 0; j < p.group; ++j) {
+        uint4 q4[kFly], k4[kFly];
+        bool on[kFly];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 qf = unpack2<T>(reinterpret_cast<const uint32_t*>(&q4)[e]), kf = unpack2<T>(reinterpret_cast<const uint32_t*>(&k4)[e]);
-          x = fmaf(qf.x, kf.x, fmaf(qf.y, kf.y, x));
+        for (int f = 0; f < kFly; ++f) {
+          const int r = (pass + f) * kAtOnce + tid / kLanes, row = r_first + min(r, rows - 1), i_row = over(row, d.by_ratio);
+          const int nth = i_row - hist_rows, first = nth < 0 ? 0 : over(nth, d.by_group) * p.group;
+          on[f] = r < rows && nth >= 0 && first + j <= nth;
+          q4[f] = k4[f] = make_uint4(0, 0, 0, 0);
+          if (on[f] && in) {
+            q4[f] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + ((s.q0 + i_row) * p.hq + hk * ratio + row - i_row * ratio) * p.dqk + part * 8));
+            k4[f] = __ldg(reinterpret_cast<const uint4*>(k_new + static_cast<long long>(first + j) * row_bytes + part * 8));
+          }
         }
 #pragma unroll
-        for (int o2 = kLanes / 2; o2 > 0; o2 >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o2);
-        if (part == 0 && r < rows && on) s_own[r][j] = silu_of<kTanh>(x * p.alpha);
+        for (int f = 0; f < kFly; ++f) {
+          float x = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 qf = unpack2<T>(reinterpret_cast<const uint32_t*>(&q4[f])[e]), kf = unpack2<T>(reinterpret_cast<const uint32_t*>(&k4[f])[e]);
+            x = fmaf(qf.x, kf.x, fmaf(qf.y, kf.y, x));
+          }
+#pragma unroll
+          for (int o2 = kLanes / 2; o2 > 0; o2 >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o2);
+          if (part == 0 && on[f]) s_own[(pass + f) * kAtOnce + tid / kLanes][j] = silu_of<kTanh>(x * p.alpha);
+        }
       }
     }
   }
@@ -215,32 +243,31 @@ __global__ void __launch_bounds__(kRwThreads) hstu_rows8_kernel(const RwParams d
     for (int j = 0; j < D / 16; ++j) o[u][j][0] = o[u][j][1] = o[u][j][2] = o[u][j][3] = 0.f;
   }
   // ldmatrix: the keys and the column half of 16 this lane names, for K as it lies and for V transposed
-  const int k_key = (lane & 7) + ((lane >> 3) & 1) * 8, k_half = lane >> 4;
-  const int v_key = (lane & 7) + (lane >> 4) * 8, v_half = (lane >> 3) & 1;
-  const uint32_t smem_at = ptx::smem_u32(smem);
+  // (place() of chunk 2 k + half is this lane's address for k = 0 with the bits of 32 k flipped: rows are multiples of 128 bytes)
+  const uint32_t k_lane = ptx::smem_u32(smem) + place((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
+  const uint32_t v_lane = ptx::smem_u32(smem) + C::kTile + place((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1);
 
-  const int stages = (nt + 1) / 2;
+  arrived();
   convert(0);
-  if (stages > 1) fetch(1);
   __syncthreads();
   for (int i = 0; i < stages; ++i) {
     const int buf = i & 1;
-    if (i + 1 < stages) {
-      convert(buf ^ 1);   // (its readers are behind the barrier of the stage before)
-      if (i + 2 < stages) fetch(i + 2);
-    }
+    if (i + C::kDepth - 1 < stages) fetch(i + C::kDepth - 1);   // (into the slot of the stage before, converted two stages ago)
+    commit();
+    arrived();
+    if (i + 1 < stages) convert(i + 1);   // (the buffer's readers are behind the barrier of the stage before)
 #pragma unroll 1
     for (int t = 0; t < 2; ++t) {
       if (groups == 0 || 2 * i + t >= nt) break;
       const int key = key_of_tile(tiles, t0 + 2 * i + t, kRwKeys);
-      const uint32_t k_tile = smem_at + buf * 2 * C::kTile, v_tile = k_tile + C::kTile;
+      const uint32_t tile_at = buf * 2 * C::kTile + t * 16 * D * 2;
       float sc[kRwGroups][4];   // keys g and g + 8: rows 2 c, 2 c + 1 of the first, of the second
 #pragma unroll
       for (int u = 0; u < kRwGroups; ++u) sc[u][0] = sc[u][1] = sc[u][2] = sc[u][3] = 0.f;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         uint32_t a[4];
-        ldsm_x4(k_tile + place(t * 16 + k_key, 2 * k + k_half), a);
+        ldsm_x4((k_lane + tile_at) ^ (32 * k), a);
 #pragma unroll
         for (int u = 0; u < kRwGroups; ++u)
           if (u < groups) mma16816(sc[u], a, qb[u][k]);
@@ -271,14 +298,12 @@ __global__ void __launch_bounds__(kRwThreads) hstu_rows8_kernel(const RwParams d
         // P times the row's power of two (a select of the bits: a masked score may be anything), and whether fp16 holds it with
         // room to spare
         auto form = [&]() {
-          bool fits = true;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float2 w = __fmul2_rn(y[h], down[u]);
             pb[u][h] = pack2<__half>(w.x, w.y) & see[h];
-            fits &= __hble2(__habs2(as_half2(pb[u][h])), __floats2half2_rn(16384.f, 16384.f));
           }
-          return fits;
+          return __hble2(__hmax2_nan(__habs2(as_half2(pb[u][0])), __habs2(as_half2(pb[u][1]))), __floats2half2_rn(16384.f, 16384.f));
         };
         if (!__all_sync(0xffffffffu, form())) {   // (NaN too, to no avail)
           float top[2] = {0.f, 0.f};
@@ -306,7 +331,7 @@ __global__ void __launch_bounds__(kRwThreads) hstu_rows8_kernel(const RwParams d
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
         uint32_t a[4];
-        ldsm_x4_trans(v_tile + place(t * 16 + v_key, 2 * j + v_half), a);
+        ldsm_x4_trans((v_lane + tile_at) ^ (32 * j), a);
 #pragma unroll
         for (int u = 0; u < kRwGroups; ++u)
           if (u < groups) mma16816(o[u][j], a, pb[u]);
@@ -334,23 +359,44 @@ __global__ void __launch_bounds__(kRwThreads) hstu_rows8_kernel(const RwParams d
     T* to = static_cast<T*>(p.out) + ((s.q0 + i_row) * p.hq + hk * ratio + row - i_row * ratio) * p.dqk + col;
     *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(v.x * p.scale, v.y * p.scale), pack2<T>(v.z * p.scale, v.w * p.scale));
   };
-  for (int i = tid; i < rows * (D / 4); i += kRwThreads) {
-    const int r = i / (D / 4), col = i % (D / 4) * 4;
-    float4 v = *reinterpret_cast<const float4*>(out + r * C::kPitch + col);
-    if (owns && col < p.dqk) {
-      const int nth = over(r_first + r, d.by_ratio) - hist_rows;
-      if (nth >= 0) {
-        const int first = over(nth, d.by_group) * p.group;
-        for (int j = first; j <= nth; ++j) {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(v_new + static_cast<long long>(j) * row_bytes + col));
-          const float2 lo = unpack2<T>(w.x), hi = unpack2<T>(w.y);
-          const float pj = s_own[r][j - first];
-          v.x = fmaf(pj, lo.x, v.x), v.y = fmaf(pj, lo.y, v.y), v.z = fmaf(pj, hi.x, v.z), v.w = fmaf(pj, hi.y, v.w);
+  constexpr int kFly = 4;
+  for (int i0 = tid; i0 < rows * (D / 4); i0 += kFly * kRwThreads) {
+    float4 v[kFly];
+#pragma unroll
+    for (int f = 0; f < kFly; ++f) {
+      const int i = min(i0 + f * kRwThreads, rows * (D / 4) - 1), r = i / (D / 4), col = i % (D / 4) * 4;
+      v[f] = *reinterpret_cast<const float4*>(out + r * C::kPitch + col);
+    }
+    if (owns) {
+      for (int j = 0; j < p.group; ++j) {
+        uint2 w[kFly];
+        float pj[kFly];
+#pragma unroll
+        for (int f = 0; f < kFly; ++f) {
+          const int i = min(i0 + f * kRwThreads, rows * (D / 4) - 1), r = i / (D / 4), col = i % (D / 4) * 4;
+          const int nth = over(r_first + r, d.by_ratio) - hist_rows, first = nth < 0 ? 0 : over(nth, d.by_group) * p.group;
+          w[f] = make_uint2(0, 0);
+          pj[f] = 0.f;
+          if (nth >= 0 && first + j <= nth && col < p.dqk) {
+            w[f] = __ldg(reinterpret_cast<const uint2*>(v_new + static_cast<long long>(first + j) * row_bytes + col));
+            pj[f] = s_own[r][j];
+          }
+        }
+#pragma unroll
+        for (int f = 0; f < kFly; ++f) {
+          const float2 lo = unpack2<T>(w[f].x), hi = unpack2<T>(w[f].y);
+          v[f].x = fmaf(pj[f], lo.x, v[f].x), v[f].y = fmaf(pj[f], lo.y, v[f].y);
+          v[f].z = fmaf(pj[f], hi.x, v[f].z), v[f].w = fmaf(pj[f], hi.y, v[f].w);
         }
       }
     }
-    if (active == 1) store(r, col, v);
-    else *reinterpret_cast<float4*>(d.partial + ((group * d.splits + split) * d.rows + r) * D + col) = v;
+#pragma unroll
+    for (int f = 0; f < kFly; ++f) {
+      const int i = i0 + f * kRwThreads, r = i / (D / 4), col = i % (D / 4) * 4;
+      if (i >= rows * (D / 4)) continue;
+      if (active == 1) store(r, col, v[f]);
+      else *reinterpret_cast<float4*>(d.partial + ((group * d.splits + split) * d.rows + r) * D + col) = v[f];
+    }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the counters are cleared (and this grid ends after that one)
   if (active == 1) return;
@@ -412,7 +458,7 @@ cudaError_t launch_rows(const RwParams& d, const RwPlan& pl, cudaStream_t stream
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(d.f.batch) * d.f.hk, pl.splits, pl.row_blocks);
-  cfg.blockDim = dim3(kRwThreads);
+  cfg.blockDim = dim3(C::kThreads);
   cfg.dynamicSmemBytes = C::kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

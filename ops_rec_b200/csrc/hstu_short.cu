@@ -314,10 +314,16 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
             int row = static_cast<int>(t.s.k0) + key, in_page = 0;
             if (from_cache) {
               in_page = key % p.page_size;
-              if (in_page == 0) {
-                pid = pid_next;   // (an id outside the cache reads as zeros: the coordinate lies past the tensor)
+              // (an id outside the cache reads as zeros: the coordinate lies past the tensor)
+              if (kWin) {
+                if (in_page == 0 || j == t.n_sink) {   // (a window starts anywhere in a page)
+                  pid = page(t, key / p.page_size);
+                  if (pid < 0 || pid >= p.num_pages) pid = p.num_pages;
+                }
+              } else if (in_page == 0) {
+                pid = pid_next;
                 if (pid < 0 || pid >= p.num_pages) pid = p.num_pages;
-                pid_next = page(t, (j * kShKeys) / p.page_size + 1);
+                pid_next = page(t, key / p.page_size + 1);
               }
             } else if (p.paged_split) {
               row = static_cast<int>(t.s.q0) + t.s.lq - t.s.tgt + (key - t.split);
@@ -638,6 +644,7 @@ bool short_paged_split(const KParams& p) {
   if (p.batch <= 0 || p.mask_type == HSTU_MASK_CUSTOM || p.bias || p.page_size % kShKeys != 0 || (align & 15u) != 0 ||
       p.num_pages > 0x7fffff00ll / 2 / p.page_size)
     return false;
+  if (p.window) return true;   // (no other kernel knows windows)
   // (the cached keys are not known here: all pages, each sequence's last one half full)
   return short_rule(p, (p.num_page_ids * p.page_size + p.total_q) / p.batch - p.page_size / 2, true);
 }
