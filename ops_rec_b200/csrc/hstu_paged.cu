@@ -257,7 +257,7 @@ struct UnpackParams {
   const void* page_ids;
   long long num_pages, num_page_ids;
   int index_bytes, batch, page_size, block, heads, dim, window, sink;
-  uint32_t by_row, by_head, by_block;   // over(): chunks of a row, chunks of a head, rows of a block
+  uint32_t by_row, by_head, by_block;   // over(): pieces of a row, pieces of a head, rows of a block
 };
 
 template <typename T, typename H>
@@ -309,21 +309,21 @@ __global__ void __launch_bounds__(kUnpackThreads) hstu_unpack_kernel(const Unpac
   }
   const int row_len = p.heads * p.dim, per_page = p.page_size / p.block;
   const long long page_len = static_cast<long long>(p.page_size) * row_len;
-  const uint4* from = reinterpret_cast<const uint4*>(p.cache + (ok ? pid : 0) * 2 * page_len);
+  const uint2* from = reinterpret_cast<const uint2*>(p.cache + (ok ? pid : 0) * 2 * page_len);
   const float* scale = p.scale + (ok ? pid : 0) * 2 * per_page * static_cast<long long>(p.heads);
   uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + slot * 2 * page_len);
-  const int chunks = static_cast<int>(n) * (row_len / 16);   // of 16 numbers, of the keys; as many of the values
-  constexpr int kFly = 4;
-  for (int i0 = threadIdx.x; i0 < 2 * chunks; i0 += kFly * kUnpackThreads) {
-    uint4 w[kFly];
+  const int per_row = row_len / 8, pieces = static_cast<int>(n) * per_row;   // of 8 numbers (a warp's stores are 512 bytes in a row)
+  constexpr int kFly = 8;
+  for (int i0 = threadIdx.x; i0 < 2 * pieces; i0 += kFly * kUnpackThreads) {
+    uint2 w[kFly];
     float f[kFly];
-    long long at[kFly];   // of the chunk in the page, -1: nothing to do
+    int at[kFly];   // of the piece in the page, -1: nothing to do
 #pragma unroll
     for (int u = 0; u < kFly; ++u) {
-      const int both = i0 + u * kUnpackThreads, kv = both >= chunks ? 1 : 0, i = both - kv * chunks;
-      const int row = over(i, p.by_row), head = over(i - row * (row_len / 16), p.by_head);
-      at[u] = i < chunks && (row < skip_from || row >= skip_to) ? kv * (page_len / 16) + i : -1;
-      w[u] = make_uint4(0, 0, 0, 0);
+      const int both = i0 + u * kUnpackThreads, kv = both >= pieces ? 1 : 0, i = both - kv * pieces;
+      const int row = over(i, p.by_row), head = over(i - row * per_row, p.by_head);
+      at[u] = i < pieces && (row < skip_from || row >= skip_to) ? kv * (p.page_size * per_row) + i : -1;
+      w[u] = make_uint2(0, 0);
       f[u] = 0.f;
       if (at[u] >= 0 && ok) {
         w[u] = __ldcs(from + at[u]);
@@ -333,21 +333,25 @@ __global__ void __launch_bounds__(kUnpackThreads) hstu_unpack_kernel(const Unpac
 #pragma unroll
     for (int u = 0; u < kFly; ++u) {
       if (at[u] < 0) continue;
-      alignas(16) T x[16];
+      uint32_t h[4], x[4];
+      to_halves<H>(w[u].x, h[0], h[1]);
+      to_halves<H>(w[u].y, h[2], h[3]);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[e] = simt::from_float<T>(H::to_float(reinterpret_cast<const uint8_t*>(&w[u])[e]) * f[u]);
-      to[2 * at[u]] = reinterpret_cast<const uint4*>(x)[0];
-      to[2 * at[u] + 1] = reinterpret_cast<const uint4*>(x)[1];
+      for (int e = 0; e < 4; ++e) {
+        const float2 v = unpack2<__half>(h[e]);
+        x[e] = pack2<T>(v.x * f[u], v.y * f[u]);
+      }
+      to[at[u]] = make_uint4(x[0], x[1], x[2], x[3]);
     }
   }
 }
 
 }  // namespace
 
-// Whether a cache of 8-bit rows can be unpacked page by page: pieces of 16 numbers of one head.
+// Whether a cache of 8-bit rows can be unpacked page by page: pieces of 8 numbers of one head.
 bool unpack_supported(const KParams& p, int dtype) {
-  return dtype != HSTU_DTYPE_FP32 && p.dqk % 16 == 0 && (reinterpret_cast<uintptr_t>(p.kv_cache) & 15u) == 0 &&
-         p.page_size <= 65536 && static_cast<long long>(p.page_size) * p.hk * p.dqk / 16 < (1ll << 21) &&
+  return dtype != HSTU_DTYPE_FP32 && p.dqk % 8 == 0 && (reinterpret_cast<uintptr_t>(p.kv_cache) & 7u) == 0 &&
+         p.page_size <= 65536 && static_cast<long long>(p.page_size) * p.hk * p.dqk / 8 < (1ll << 21) &&
          p.num_page_ids <= 0x7fffffffll;
 }
 cudaError_t launch_unpack(const KParams& p, void* out, void* table, int dtype, cudaStream_t stream) {
@@ -371,9 +375,9 @@ cudaError_t launch_unpack(const KParams& p, void* out, void* table, int dtype, c
   u.dim = p.dqk;
   u.window = p.window;
   u.sink = p.sink;
-  // (at most 2^22 chunks by 512 of a row, 512 by 32 of a head, 2^16 rows by as many of a block)
-  u.by_row = inverse_of(p.hk * p.dqk / 16);
-  u.by_head = inverse_of(p.dqk / 16);
+  // (at most 2^21 pieces - and as many again - by 1024 of a row, 1024 by 64 of a head, 2^16 rows by as many of a block)
+  u.by_row = inverse_of(p.hk * p.dqk / 8);
+  u.by_head = inverse_of(p.dqk / 8);
   u.by_block = inverse_of(p.scale_block);
   const dim3 grid(static_cast<unsigned>(p.num_page_ids), 1, 1);
 #define HSTU_UNPACK(TT)                                                                                            \
