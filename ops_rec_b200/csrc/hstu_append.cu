@@ -4,7 +4,9 @@
 //           block and head; where the block holds rows already, no smaller than the scale they have
 //   row   = round(x / scale); the rows a block holds already are rounded anew to round(number * old / scale) when it grew
 //
-// A warp does one (block of tokens, keys or values, head): two passes over at most `block` rows, the second out of the L1 / L2.
+// A warp does one block of tokens, of the keys or of the values: two passes over at most `block` rows, the second out of the
+// L1 / L2.  Where a head is 8, 16, .. 256 wide it takes 256 columns, whichever heads they belong to - a piece of 8 columns per
+// lane, whole lines per row, and the look-ups in front shared by all of the heads - elsewhere one head.
 // Which blocks there are is known to the device only; sequence b owns the slots [seq_offset[b] / block + 2 b, ..) of the grid,
 // which are never fewer than the blocks its rows touch (n rows touch at most n / block + 2), and finds them by a 32-way search.
 // HBM-bound for histories (3 bytes per 16-bit element), a chain of six dependent reads for single rows.
@@ -64,20 +66,58 @@ template <typename T> struct Piece<T, 8> {
   }
 };
 
-template <typename T, typename H, int kN>
-__global__ void __launch_bounds__(kAppendThreads) hstu_append_kernel(const AppendParams p) {
+// (a 64-bit division is some hundred instructions)
+__device__ __forceinline__ long long quotient(long long a, int b) {
+  return (a >> 32) == 0 ? static_cast<long long>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b)) : a / b;
+}
+
+// The largest magnitude of eight (the call's type): NaN take no part, infinities do.
+template <typename T> struct Largest;
+template <> struct Largest<float> {
+  float m = 0.f;
+  __device__ __forceinline__ void take(const float* from) {
+    float x[8];
+    Piece<float, 8>::load(from, x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(x[e]));
+  }
+  __device__ __forceinline__ float get() const { return m; }
+};
+template <> struct Largest<__nv_bfloat16> {
+  __nv_bfloat162 m = __floats2bfloat162_rn(0.f, 0.f);
+  __device__ __forceinline__ void take(const __nv_bfloat16* from) {
+    const uint4 u = *reinterpret_cast<const uint4*>(from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __hmax2(m, __habs2(reinterpret_cast<const __nv_bfloat162*>(&u)[e]));
+  }
+  __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+template <> struct Largest<__half> {
+  __half2 m = __floats2half2_rn(0.f, 0.f);
+  __device__ __forceinline__ void take(const __half* from) {
+    const uint4 u = *reinterpret_cast<const uint4*>(from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = __hmax2(m, __habs2(reinterpret_cast<const __half2*>(&u)[e]));
+  }
+  __device__ __forceinline__ float get() const { return fmaxf(__low2float(m), __high2float(m)); }
+};
+
+// What a warp's slot stands for: rows [r0, r1) of sequence b, in block `base / block` of its cache.
+struct AppendWork {
+  long long first;    // of the rows, in k and v
+  long long place;    // of the block's first row in the cache, counted in rows of the keys' half of its page
+  long long scale;    // of its scales: of the keys of head 0
+  int held, count;    // rows the block holds already, new rows; 0 new rows: nothing to do
+};
+__device__ __forceinline__ AppendWork find_work(const AppendParams& p, long long slot) {
   const int lane = threadIdx.x & 31;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
-  const int per_slot = 2 * p.heads;
-  const long long slot = unit / per_slot;
-  if (slot >= p.total / p.block + 2ll * p.batch) return;
-  const int kv = static_cast<int>(unit - slot * per_slot) / p.heads, head = static_cast<int>(unit - slot * per_slot) % p.heads;
+  AppendWork w = {0, 0, 0, 0, 0};
   // the last sequence whose first slot is <= slot
   auto first_slot = [&](int b) {
     long long o = load_index(p.offset, p.index_bytes, b);
     if (o < 0) o = 0;
     if (o > p.total) o = p.total;
-    return o / p.block + 2ll * b;
+    return quotient(o, p.block) + 2ll * b;
   };
   int lo = 0, hi = p.batch - 1;
   while (hi > lo) {
@@ -110,23 +150,112 @@ __global__ void __launch_bounds__(kAppendThreads) hstu_append_kernel(const Appen
   if (!bad && start < 0) bad |= HSTU_ST_BAD_PAGES;
   if (bad) {
     if (lane == 0 && p.status) atomicOr(p.status, bad);
-    return;
+    return w;
   }
-  const long long blk = start / p.block + (slot - first_slot(b));
+  const long long blk = quotient(start, p.block) + (slot - first_slot(b));
   const long long base = blk * p.block;
   const long long r0 = base > start ? base : start, r1 = base + p.block < cached ? base + p.block : cached;
-  if (fresh == 0 || r0 >= r1) return;
-  const long long pid = load_index(p.page_ids, p.index_bytes, pg0 + base / p.page_size);
+  if (fresh == 0 || r0 >= r1) return w;
+  const long long pid = load_index(p.page_ids, p.index_bytes, pg0 + quotient(base, p.page_size));
   if (pid < 0 || pid >= p.num_pages) {
     if (lane == 0 && p.status) atomicOr(p.status, static_cast<unsigned>(HSTU_ST_BAD_PAGES));
-    return;
+    return w;
   }
-  const int in_page = static_cast<int>(base % p.page_size);
+  const int in_page = static_cast<int>(base - quotient(base, p.page_size) * p.page_size);
+  w.first = q0 + (r0 - start);
+  w.place = pid * 2 * p.page_size + in_page;
+  w.scale = (pid * 2 * (p.page_size / p.block) + in_page / p.block) * p.heads;
+  w.held = static_cast<int>(r0 - base);
+  w.count = static_cast<int>(r1 - r0);
+  return w;
+}
+
+// 256 columns a warp: see the top.
+template <typename T, typename H>
+__global__ void __launch_bounds__(kAppendThreads) hstu_append_columns_kernel(const AppendParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long unit = static_cast<long long>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  const int row_len = p.heads * p.dim, spans = (row_len + 255) / 256;
+  const long long slot = unit / (2 * spans);
+  if (slot >= p.total / p.block + 2ll * p.batch) return;
+  const int rest = static_cast<int>(unit - slot * (2 * spans)), kv = rest / spans, col = (rest - kv * spans) * 256 + lane * 8;
+  const AppendWork w = find_work(p, slot);
+  if (w.count == 0) return;
+  const bool on = col < row_len;
+  const int head = on ? col / p.dim : 0;
+  const T* src = static_cast<const T*>(kv ? p.v : p.k) + w.first * row_len + (on ? col : 0);
+  uint8_t* dst = p.cache + (w.place + kv * static_cast<long long>(p.page_size)) * row_len + (on ? col : 0);
+  float* scale_at = p.scale + w.scale + kv * static_cast<long long>(p.page_size / p.block) * p.heads + head;
+  const float old = on && w.held > 0 ? *scale_at : 0.f;
+  Largest<T> most;
+#pragma unroll 8
+  for (int r = 0; r < w.count; ++r) most.take(src + static_cast<long long>(r) * row_len);
+  float amax = most.get();
+  if (__any_sync(0xffffffffu, amax > 3.402823466e38f)) {   // infinities among them: over the finite values alone
+    amax = 0.f;
+    for (int r = 0; r < w.count; ++r) {
+      float x[8];
+      Piece<T, 8>::load(src + static_cast<long long>(r) * row_len, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(x[e]);
+        amax = a <= 3.402823466e38f && a > amax ? a : amax;
+      }
+    }
+  }
+  // over the lanes of the head (dim / 8 of them, a power of two; all of a warp hold parts of whole heads or of one)
+  for (int o = p.dim / 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  float scale = block_scale<H>(amax);
+  if (w.held > 0) {
+    if (scale > old) {
+      if (on)
+        for (int r = 0; r < w.held; ++r) {
+          uint8_t* at = dst + static_cast<long long>(r) * row_len;
+          uint8_t v[8];
+          Piece<T, 8>::load_held(at, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = H::from_float(H::to_float(v[e]) * (old / scale));
+          Piece<T, 8>::store(at, v);
+        }
+    } else {
+      scale = old;
+    }
+    __syncwarp();   // (every lane has read the scale before one writes it)
+  }
+  if (!on) return;
+  if (col % p.dim == 0) *scale_at = scale;
+  dst += static_cast<long long>(w.held) * row_len;
+  auto write = [&](auto divide) {
+#pragma unroll 8
+    for (int r = 0; r < w.count; ++r) {
+      float x[8];
+      Piece<T, 8>::load(src + static_cast<long long>(r) * row_len, x);
+      const uint32_t lo = H::from_floats(divide(x[0]), divide(x[1])) | (H::from_floats(divide(x[2]), divide(x[3])) << 16);
+      const uint32_t hi = H::from_floats(divide(x[4]), divide(x[5])) | (H::from_floats(divide(x[6]), divide(x[7])) << 16);
+      *reinterpret_cast<uint2*>(dst + static_cast<long long>(r) * row_len) = make_uint2(lo, hi);
+    }
+  };
+  // the product with the reciprocal is the quotient wherever the scale is a power of two; another one was not written here
+  const float inverse = 1.f / scale;
+  if ((__float_as_uint(scale) & 0x7fffffu) == 0) write([&](float x) { return x * inverse; });
+  else write([&](float x) { return x / scale; });
+}
+
+template <typename T, typename H, int kN>
+__global__ void __launch_bounds__(kAppendThreads) hstu_append_kernel(const AppendParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long unit = static_cast<long long>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  const int per_slot = 2 * p.heads;
+  const long long slot = unit / per_slot;
+  if (slot >= p.total / p.block + 2ll * p.batch) return;
+  const int kv = static_cast<int>(unit - slot * per_slot) / p.heads, head = static_cast<int>(unit - slot * per_slot) % p.heads;
+  const AppendWork w = find_work(p, slot);
+  if (w.count == 0) return;
   const long long row_len = static_cast<long long>(p.heads) * p.dim;
-  const T* src = static_cast<const T*>(kv ? p.v : p.k) + (q0 + (r0 - start)) * row_len + static_cast<long long>(head) * p.dim;
-  uint8_t* dst = p.cache + ((pid * 2 + kv) * p.page_size + in_page) * row_len + static_cast<long long>(head) * p.dim;
-  float* scale_at = p.scale + ((pid * 2 + kv) * (p.page_size / p.block) + in_page / p.block) * p.heads + head;
-  const int held = static_cast<int>(r0 - base), count = static_cast<int>(r1 - r0);   // rows it holds already, new rows
+  const T* src = static_cast<const T*>(kv ? p.v : p.k) + w.first * row_len + static_cast<long long>(head) * p.dim;
+  uint8_t* dst = p.cache + (w.place + kv * static_cast<long long>(p.page_size)) * row_len + static_cast<long long>(head) * p.dim;
+  float* scale_at = p.scale + w.scale + kv * static_cast<long long>(p.page_size / p.block) * p.heads + head;
+  const int held = w.held, count = w.count;
   const int per_row = p.dim / kN;
   const int step_row = 32 / per_row, step_piece = 32 % per_row;
 
@@ -191,7 +320,10 @@ cudaError_t launch_append_t(const AppendParams& p, cudaStream_t stream) {
   const unsigned grid = static_cast<unsigned>((units + kAppendThreads / 32 - 1) / (kAppendThreads / 32));
   const bool vec = p.dim % 8 == 0 && ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15u) == 0 &&
                    (reinterpret_cast<uintptr_t>(p.cache) & 7u) == 0;
-  if (vec) hstu_append_kernel<T, H, 8><<<grid, kAppendThreads, 0, stream>>>(p);
+  if (vec && p.dim <= 256 && (p.dim & (p.dim - 1)) == 0) {
+    const long long columns = (p.total / p.block + 2ll * p.batch) * 2 * ((p.heads * p.dim + 255) / 256);
+    hstu_append_columns_kernel<T, H><<<static_cast<unsigned>((columns + kAppendThreads / 32 - 1) / (kAppendThreads / 32)), kAppendThreads, 0, stream>>>(p);
+  } else if (vec) hstu_append_kernel<T, H, 8><<<grid, kAppendThreads, 0, stream>>>(p);
   else hstu_append_kernel<T, H, 1><<<grid, kAppendThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }

@@ -17,6 +17,9 @@ struct E4m3 {
   static __device__ __forceinline__ uint8_t from_float(float x) {   // round to nearest even, +-448 beyond, NaN stays NaN
     return static_cast<uint8_t>(__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3));
   }
+  static __device__ __forceinline__ uint32_t from_floats(float a, float b) {   // two of them, the first in the low byte
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  }
   static __device__ __forceinline__ float to_float(uint8_t v) {
     return __half2float(__half(__nv_cvt_fp8_to_halfraw(v, __NV_E4M3)));
   }
@@ -29,6 +32,9 @@ struct Int8 {
     int v = __float2int_rn(x);
     v = v > 127 ? 127 : v < -127 ? -127 : v;
     return static_cast<uint8_t>(static_cast<int8_t>(v));
+  }
+  static __device__ __forceinline__ uint32_t from_floats(float a, float b) {
+    return static_cast<uint32_t>(from_float(a)) | (static_cast<uint32_t>(from_float(b)) << 8);
   }
   static __device__ __forceinline__ float to_float(uint8_t v) { return static_cast<float>(static_cast<int8_t>(v)); }
 };
