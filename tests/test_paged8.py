@@ -434,3 +434,109 @@ def test_paged_keeps_what_is_not_finite(dtype, new):
     out[:new, 0, 5], out[:new, 1] = 0, 0
     want[:new, 0, 5], want[:new, 1] = 0, 0
     assert ((out.double() - want).abs() <= tol + 1e-9).all()
+
+
+MANY = 140        # users of 4 heads and more than 32 rows: their pages are unpacked for the kernel that many rows share
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,held", [(BF16, E4M3), (FP16, INT8), (BF16, INT8), (FP16, E4M3)])
+@pytest.mark.parametrize("d,page,block", [(64, 64, 16), (64, 128, 128), (128, 64, 64)])
+@pytest.mark.parametrize("window,sink", [(0, 0), (70, 5)])
+def test_paged_many_users_of_many_rows(dtype, held, d, page, block, window, sink):
+    rng = np.random.default_rng(21)
+    cached = rng.integers(1, 400, MANY)
+    cached[:4] = 1, 64, 65, 128
+    new = np.minimum(cached, rng.integers(0, 50, MANY))
+    new[5], cached[5] = 49, 399
+    check_paged(make(cached, new, None, 4, 4, d, dtype, held, page, block, seed=22), window, sink)
+    check_paged(make(cached, new, rng.integers(0, 40, MANY), 8, 4, d, dtype, held, page, block, seed=23, index=torch.int32), window, sink)
+
+
+@pytest.mark.gpu
+def test_paged_many_users_reads_nothing_behind_a_row_and_flags_bad_pages():
+    rng = np.random.default_rng(24)
+    cached = rng.integers(60, 300, MANY)
+    args = make(cached, np.full(MANY, 40), rng.integers(0, 9, MANY), 4, 4, 64, page=64, block=32, seed=25)
+    a, w = check_paged(args), check_paged(args, 50, 3)
+    nan = CO.numbers(torch.tensor(float("nan")), E4M3).view(torch.uint8)
+    dirty = args | dict(kv_cache=args["kv_cache"].clone(), kv_scale=args["kv_scale"].clone())
+    raw, used = dirty["kv_cache"].view(torch.uint8), torch.zeros(dirty["kv_cache"].shape[0], 64, dtype=torch.bool)
+    for b, n in enumerate(cached):
+        for j in range(0, int(n), 64):
+            used[int(args["page_ids"][int(args["page_offsets"][b]) + j // 64]), :int(n) - j] = True
+    raw.permute(0, 2, 1, 3, 4)[~used] = nan
+    dirty["kv_scale"].permute(0, 2, 1, 3)[~used.unflatten(1, (-1, 32)).any(2)] = float("nan")
+    assert torch.equal(cabi.hstu_paged_8bit_forward(**on_gpu(dirty), workspace_fill=0xFF), a)
+    assert torch.equal(cabi.hstu_paged_8bit_forward(**on_gpu(dirty), window=50, num_sink=3, workspace_fill=0xFF), w)
+    # a page that is not there: flagged, and every other user's rows as they were
+    for bad in (10 ** 6, -1, -2 ** 40):
+        ids = args["page_ids"].clone()
+        ids[int(args["page_offsets"][7])] = bad
+        for window, good in ((0, a), (50, w)):
+            out, st = cabi.hstu_paged_8bit_forward(**on_gpu(args | dict(page_ids=ids)), window=window, num_sink=3 if window else 0, return_status=True)
+            assert st & cabi.ST_BAD_PAGES
+            here = torch.ones(out.shape[0], dtype=torch.bool, device="cuda")
+            here[int(args["seq_offset"][7]):int(args["seq_offset"][8])] = False
+            assert torch.equal(out[here], good[here])
+    for name, change in (("last_page_len", 70), ("page_offsets", 1)):
+        wrong = args[name].clone()
+        wrong[3] += change
+        _, st = cabi.hstu_paged_8bit_forward(**on_gpu(args | {name: wrong}), return_status=True)
+        assert st & cabi.ST_BAD_PAGES, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [1, 2, 3, 4, 5, 16])
+@pytest.mark.parametrize("d,hq,hk", [(64, 4, 2), (128, 2, 2), (96, 3, 3)])
+def test_paged_groups_of_targets(group, d, hq, hk):
+    args = make([700, 77, 0, 1300], [20, 1, 0, 0], [30, 7, 5, 64], hq, hk, d, page=64, block=32, seed=26) | dict(target_group_size=group)
+    check_paged(args)
+    check_paged(args, 100, 17)
+    rng = np.random.default_rng(27)
+    cached = rng.integers(1, 200, MANY)
+    args = make(cached, np.minimum(cached, 30), rng.integers(1, 40, MANY), 4, 4, d, FP16, INT8, 64, 32, seed=28) | dict(target_group_size=group)
+    check_paged(args)
+    check_paged(args, 33, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("window,sink", [(0, 0), (5000, 64), (1, 0)])
+def test_paged_long_histories_of_few_users_with_targets(window, sink):
+    """Split over the keys, and over the rows."""
+    check_paged(make([15000, 130], [200, 3], [150, 9], 2, 1, 128, BF16, E4M3, 128, 64, seed=29), window, sink)
+    check_paged(make([15000], [0], [300], 1, 1, 64, FP16, INT8, 32, 16, seed=30), window, sink)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("users,new", [(3, 1), (3, 20), (MANY, 40)])
+def test_paged_on_two_streams_and_captured(users, new):
+    """Two calls at once on streams of their own; a captured step of both operators, replayed with other contents."""
+    rng = np.random.default_rng(31)
+    cached = rng.integers(new, 500, users)
+    args = on_gpu(make(cached, np.full(users, new), None, 4, 4, 64, page=64, block=32, seed=32))
+    other = on_gpu(make(cached + 1, np.full(users, new), None, 4, 4, 64, page=64, block=32, seed=33))
+    names = ["q", "k", "v", "kv_cache", "kv_scale", "max_seq_len", "max_seq_len_k", "seq_offset", "seq_offset_k", "page_offsets", "page_ids",
+             "last_page_len", "alpha"]
+    call = lambda a: paged_op(**{n: a[n] for n in names}, window=99, num_sink=4)   # noqa: E731
+    want, want_other = call(args), call(other)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        with torch.cuda.stream(s1):
+            got.append((call(args), want))
+        with torch.cuda.stream(s2):
+            got.append((call(other), want_other))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in got)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        append_op(**{n: args[n] for n in TABLE})
+        out = call(args)
+    args["k"].mul_(1.5), args["q"].mul_(0.5)
+    twin = args | {n: args[n].clone() for n in ("kv_cache", "kv_scale")}
+    append_op(**{n: twin[n] for n in TABLE})
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(args["kv_cache"].view(torch.uint8), twin["kv_cache"].view(torch.uint8)) and torch.equal(out, call(twin))
