@@ -80,7 +80,8 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   if (pg0 < 0) pg0 = 0;
   if (pg1 > p.num_page_ids) pg1 = p.num_page_ids;
   if (hk == 0 && split == 0) report_sequence<kDecThreads>(p, b, pg0, pg1);
-  const KeyTiles tiles = rows > 0 ? Mask::tiles(p, s, 0, s.lq, kDecKeys) : KeyTiles{0, 0, 0};
+  KeyTiles tiles = rows > 0 ? Mask::tiles(p, s, 0, s.lq, kDecKeys) : KeyTiles{0, 0, 0};
+  tiles.n = min(tiles.n, d.splits * d.tiles);   // (lengths beyond the table's pages: flagged)
   // CTAs that share the keys, evenly, in whole rounds of the four warps' pairs
   int active = 1;
   while (active * d.tiles < tiles.n) ++active;
@@ -344,6 +345,7 @@ DecPlan plan(const KParams& p) {
   d.rows = p.maxq * p.gqa_ratio;
   long long most = (p.maxk + kDecKeys - 1) / kDecKeys;   // tiles of the longest sequence
   long long all = p.num_page_ids * p.page_size / kDecKeys;   // and of all of them together, at most
+  if (all < most) most = all;
   if (p.window) {
     const long long seen = (static_cast<long long>(p.window) + p.maxq) / kDecKeys + 2 + (p.sink + kDecKeys - 1) / kDecKeys;
     if (seen < most) most = seen;
@@ -353,6 +355,10 @@ DecPlan plan(const KParams& p) {
   // sums - a thousand instructions a warp, where a tile takes 300 - are what the SMs do.  Attention alone, us, at 4 / 6 / 8 /
   // 12: 128 users of 200 - 2048 rows and 8 heads 64 / 66 / 70 / 75, 4 users of 14000 - 20000 44 / 39 / 45 / 50.
   long long tiles = all * p.hk / (6ll * 148);
+  // Of a bound that is far above the lengths most CTAs find nothing to do: at most some 32 per SM (1000 users of 60 - 128 rows,
+  // one head, max_seq_len_k 128 / 20480: 14 / 21 us; without it 14 / 169).
+  const long long busy = most * p.batch * p.hk / (32ll * 148);
+  if (tiles < busy) tiles = busy;
   tiles = tiles < 8 ? 8 : tiles > kDecMostTiles ? kDecMostTiles : tiles;
   constexpr int kRound = kDecWarps * kPair;
   d.tiles = static_cast<int>((tiles + kRound - 1) / kRound * kRound);

@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
   const int v_lo = min(q_lo, hist_rows), v_n = min(q_lo + q_n - 1, hist_rows) - v_lo + 1;
   KeyTiles tiles = rows > 0 ? Mask::tiles(p, s, v_lo, v_n, kRwKeys) : KeyTiles{0, 0, 0};
   if (tiles.n > 0 && key_of_tile(tiles, tiles.n - 1, kRwKeys) >= cached) tiles.n -= 1;   // (the targets' own place)
+  tiles.n = min(tiles.n, d.splits * d.tiles);   // (lengths beyond the table's pages: flagged)
   // CTAs that share this block's keys, evenly, in whole stages
   int active = 1;
   while (active * d.tiles < tiles.n) ++active;
@@ -431,6 +432,7 @@ RwPlan plan(const KParams& p) {
   d.rows = rows < kRwRows ? rows : kRwRows;
   long long most = (p.maxk + kRwKeys - 1) / kRwKeys;         // tiles of the longest sequence
   long long all = p.num_page_ids * p.page_size / kRwKeys;    // and of all of them together, at most
+  if (all < most) most = all;
   if (p.window) {
     const long long seen = (static_cast<long long>(p.window) + p.maxq) / kRwKeys + 2 + (p.sink + kRwKeys - 1) / kRwKeys;
     if (seen < most) most = seen;
@@ -438,6 +440,10 @@ RwPlan plan(const KParams& p) {
   }
   // some eight CTAs per SM, of at least 16 tiles: less is mostly set-up
   long long tiles = all * p.hk * d.row_blocks / (8ll * 148);
+  // Of a bound that is far above the lengths most CTAs find nothing to do: at most some 32 per SM (1000 users of 60 - 128 rows,
+  // one head, 9 rows and 20 targets, max_seq_len_k 148 / 20480: 35 / 45 us; without it 35 / 166).
+  const long long busy = most * p.batch * p.hk * d.row_blocks / (32ll * 148);
+  if (tiles < busy) tiles = busy;
   tiles = tiles < 16 ? 16 : tiles > kRwMostTiles ? kRwMostTiles : tiles;
   d.tiles = static_cast<int>((tiles + 1) / 2 * 2);
   d.splits = static_cast<int>((most + d.tiles - 1) / d.tiles);

@@ -540,3 +540,13 @@ def test_paged_on_two_streams_and_captured(users, new):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(args["kv_cache"].view(torch.uint8), twin["kv_cache"].view(torch.uint8)) and torch.equal(out, call(twin))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("users,new,targets", [(3, 1, None), (300, 1, None), (3, 20, None), (300, 5, 9)])
+def test_paged_a_loose_bound_of_the_lengths(users, new, targets):
+    rng = np.random.default_rng(34)
+    cached = rng.integers(new, 150, users)
+    args = make(cached, np.full(users, new), None if targets is None else np.full(users, targets), 2, 1, 64, seed=35)
+    check_paged(args | dict(max_seq_len_k=20480))
+    check_paged(args | dict(max_seq_len_k=20480), 20, 1)
