@@ -248,14 +248,15 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dkv_kernel(const BwdParams 
 }
 
 // ------------------------------------------------------------------------------------ register-tiled form
-// Rows of the streamed tile: 64, or 32 at width 128 (two CTAs on an SM instead of one).
-template <int kDim> constexpr int kStream = kDim > 64 ? 32 : 64;
+// Rows of the streamed tile: 64, or 32 at width 128 (two CTAs on an SM instead of one) and with a window, where shorter tiles
+// leave less of what nobody sees (128 sequences of 50 - 500 rows, window 100, 4 sinks, 4 heads of 64, fp32: 760 us, 900 with 64).
+template <int kDim, bool kWin> constexpr int kStream = kDim > 64 || (kWin && kDim > 32) ? 32 : 64;
 
 template <typename T, int kDim, bool kWin>
 __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const BwdParams bp) {
   using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
-  constexpr int kN = kStream<kDim>, kCols = kN / 16, kPer = simt::OutCols<kDim>::kPer;
+  constexpr int kN = kStream<kDim, kWin>, kCols = kN / 16, kPer = simt::OutCols<kDim>::kPer;
   constexpr int ld = kDim + 4, ldp = kN + 4;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const KParams& p = bp.f;
@@ -347,16 +348,18 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const 
   asm volatile("griddepcontrol.wait;" ::: "memory");   // (the pre-pass: nothing here reads what it wrote)
 }
 
-template <typename T, int kDim, bool kWin>
-__global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const BwdParams bp) {
+template <typename T, int kDim, bool kWin, int kSplit>
+__global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const BwdParams bp, int first_tile) {
   using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
-  constexpr int kN = kStream<kDim>, kCols = kN / 16, kPer = simt::OutCols<kDim>::kPer;
+  constexpr int kN = kStream<kDim, kWin>, kCols = kN / 16, kPer = simt::OutCols<kDim>::kPer;
   constexpr int ld = kDim + 4, ldp = kN + 4;
   const KParams& p = bp.f;
   const int b = blockIdx.x / p.hk, hk = blockIdx.x - b * p.hk;
-  const int c0 = blockIdx.y * simt::kRows;   // (the first keys are seen by the most queries)
+  const int c0 = (first_tile + blockIdx.y) * simt::kRows;   // (the first keys are seen by the most queries)
+  const int rank = kSplit > 1 ? blockIdx.z : 0;             // (see simt::lay_down)
   const SeqInfo s = load_seq(p, b);
+  if (kSplit > 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the other key tiles)
   if (c0 < s.lk) {
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const int dq = p.dqk, dv = p.dv;
@@ -379,7 +382,13 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
     for (int r = 0; r < 4; ++r)
 #pragma unroll
       for (int c = 0; c < kPer; ++c) acc_k[r][c] = acc_v[r][c] = 0.f;
+    auto after = [&](int u) {   // the tile that follows u here
+#pragma unroll 1
+      for (int n = 0; n < kSplit; ++n) u = next(u + 1);
+      return u;
+    };
     int u = next(0);
+    for (int n = 0; n < rank; ++n) u = next(u + 1);
     if (u < count) {
       const int h = hk * p.gqa_ratio + u / per_head, r0 = (u % per_head) * kN;
       simt::load_rows<T, simt::kRows, kDim>(Ks, ld, static_cast<const T*>(p.k), s.k0, c0, s.lk, p.hk, hk, dq);
@@ -390,7 +399,7 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
     }
     while (u < count) {
       const int h = hk * p.gqa_ratio + u / per_head, r0 = (u % per_head) * kN;
-      const int un = next(u + 1);
+      const int un = after(u);
       const int hn = hk * p.gqa_ratio + un / per_head, rn = (un % per_head) * kN;
       typename Mask::Bounds rb[kCols];
       float bv[4][kCols];
@@ -431,12 +440,25 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
       u = un;
     }
     simt::cp_async_wait<0>();
+    auto store = [&](int j, const float (&ak)[kPer], const float (&av)[kPer]) {
+      if (j >= s.lk) return;
+      simt::store_row<T, kDim>(static_cast<T*>(bp.dk) + ((s.k0 + j) * p.hk + hk) * dq, dq, tx, ak);
+      simt::store_row<T, kDim>(static_cast<T*>(bp.dv) + ((s.k0 + j) * p.hk + hk) * dv, dv, tx, av);
+    };
+    if constexpr (kSplit > 1) {
+      __syncthreads();   // (every copy has landed and every tile is consumed)
+      simt::lay_down<kDim>(smem, acc_k);
+      simt::lay_down<kDim>(smem + simt::kRows * kDim, acc_v);
+      simt::cluster_arrive();
+      simt::cluster_wait();
+      simt::add_up<kDim>(smem, rank, acc_k[0]);
+      simt::add_up<kDim>(smem + simt::kRows * kDim, rank, acc_v[0]);
+      store(c0 + 4 * ty + rank, acc_k[0], acc_v[0]);
+      simt::cluster_arrive();
+      simt::cluster_wait();   // (the others have read this one's sums)
+    } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = c0 + 4 * ty + r;
-      if (j >= s.lk) continue;
-      simt::store_row<T, kDim>(static_cast<T*>(bp.dk) + ((s.k0 + j) * p.hk + hk) * dq, dq, tx, acc_k[r]);
-      simt::store_row<T, kDim>(static_cast<T*>(bp.dv) + ((s.k0 + j) * p.hk + hk) * dv, dv, tx, acc_v[r]);
+      for (int r = 0; r < 4; ++r) store(c0 + 4 * ty + r, acc_k[r], acc_v[r]);
     }
   }
   // the dQ pass wrote nothing this one reads; the wait makes the stream's next operation find both complete
@@ -444,25 +466,51 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
 }
 
 template <typename T, int kDim, bool kWin>
-cudaError_t launch_simt_bwd_of(const BwdParams& bp, cudaStream_t stream) {
+cudaError_t launch_simt_dq(const BwdParams& bp, cudaStream_t stream) {
   const KParams& p = bp.f;
-  constexpr int kN = kStream<kDim>;
-  constexpr int tiles = 2 * (simt::kRows + kN) * (kDim + 4), part = simt::kRows * (kN + 4);
-  constexpr int smem_q = 4 * (tiles + part), smem_kv = 4 * (tiles + 2 * part);
-  cudaError_t e = cudaFuncSetAttribute(hstu_simt_bwd_dq_kernel<T, kDim, kWin>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(hstu_simt_bwd_dkv_kernel<T, kDim, kWin>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_kv);
+  constexpr int kN = kStream<kDim, kWin>, smem = 4 * (2 * (simt::kRows + kN) * (kDim + 4) + simt::kRows * (kN + 4));
+  auto kern = hstu_simt_bwd_dq_kernel<T, kDim, kWin>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid_q(static_cast<unsigned>(p.batch) * p.hq, (p.maxq + simt::kRows - 1) / simt::kRows, 1);
-  e = simt::launch(hstu_simt_bwd_dq_kernel<T, kDim, kWin>, grid_q, smem_q, stream, bp);
+  return simt::launch(kern, dim3(static_cast<unsigned>(p.batch) * p.hq, (p.maxq + simt::kRows - 1) / simt::kRows, 1), smem, stream, bp);
+}
+
+template <typename T, int kDim, bool kWin, int kSplit>
+cudaError_t launch_simt_dkv(const BwdParams& bp, int first, int tiles, cudaStream_t stream) {
+  const KParams& p = bp.f;
+  if (tiles == 0) return cudaSuccess;
+  constexpr int kN = kStream<kDim, kWin>, smem = 4 * (2 * (simt::kRows + kN) * (kDim + 4) + 2 * simt::kRows * (kN + 4));
+  auto kern = hstu_simt_bwd_dkv_kernel<T, kDim, kWin, kSplit>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid_k(static_cast<unsigned>(p.batch) * p.hk, (p.maxk + simt::kRows - 1) / simt::kRows, 1);
-  return simt::launch(hstu_simt_bwd_dkv_kernel<T, kDim, kWin>, grid_k, smem_kv, stream, bp);
+  return simt::launch(kern, dim3(static_cast<unsigned>(p.batch) * p.hk, tiles, kSplit), smem, stream, bp, first);
+}
+
+// Windows leave a key tile a few tiles of queries, and those of the sinks all of them: chains that the rest of a call waits for.
+// Four CTAs share one of 8 tiles or more where the call is small: of the sinks up to 8 CTAs per SM, of all keys up to 2.  (fp32,
+// 50 - 500 rows, 2 / 1 heads of 64, window 100, 4 sinks, us of the whole backward pass with all / the sinks' / no chains shared:
+// 4 sequences 50 / 72 / 132, 16 78 / 108 / 169, 32 135 / 139 / 233; 48 - / 192 / 240; 64 of 2 / 2 heads - / 229 / 212; 2 of
+// 4000 rows, window 1000, 500 CTAs: 642 / 592 / 834.)
+int shared_key_tiles(const KParams& p, int tile) {
+  const int tiles = (p.maxk + simt::kRows - 1) / simt::kRows;
+  const long long ctas = static_cast<long long>(p.batch) * p.hk * tiles;
+  auto is_long = [&](long long rows) { return ((rows < p.maxq ? rows : p.maxq) + tile - 1) / tile * p.gqa_ratio >= 8; };
+  if (is_long(static_cast<long long>(p.window) + simt::kRows) && ctas <= 2 * 148) return tiles;
+  if (p.sink == 0 || ctas > 8 * 148 || !is_long(p.maxq)) return 0;
+  return p.sink < p.maxk ? (p.sink + simt::kRows - 1) / simt::kRows : tiles;
 }
 
 template <typename T, int kDim>
 cudaError_t launch_simt_bwd(const BwdParams& bp, cudaStream_t stream) {
-  return bp.f.window ? launch_simt_bwd_of<T, kDim, true>(bp, stream) : launch_simt_bwd_of<T, kDim, false>(bp, stream);
+  const int tiles = (bp.f.maxk + simt::kRows - 1) / simt::kRows;
+  if (!bp.f.window) {
+    const cudaError_t e = launch_simt_dq<T, kDim, false>(bp, stream);
+    return e != cudaSuccess ? e : launch_simt_dkv<T, kDim, false, 1>(bp, 0, tiles, stream);
+  }
+  const int shared = shared_key_tiles(bp.f, kStream<kDim, true>);
+  cudaError_t e = launch_simt_dq<T, kDim, true>(bp, stream);
+  if (e == cudaSuccess) e = launch_simt_dkv<T, kDim, true, simt::kSplitCtas>(bp, 0, shared, stream);
+  return e != cudaSuccess ? e : launch_simt_dkv<T, kDim, true, 1>(bp, shared, tiles - shared, stream);
 }
 
 // The register-tiled kernels wherever their loads are possible.  (16 sequences of 50-500 rows, 2 heads of 64, fp32, forward

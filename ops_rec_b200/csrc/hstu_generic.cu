@@ -30,7 +30,10 @@ constexpr int GMAXC = 16;    // dv <= 512 -> at most 16 output columns per threa
 template <typename T> __device__ __forceinline__ float to_f(T x) { return simt::to_float<T>(x); }
 template <typename T> __device__ __forceinline__ T from_f(float x) { return simt::from_float<T>(x); }
 
-constexpr int kFwdKeys = 64;   // keys per tile of the register-tiled kernel
+// Keys per tile of the register-tiled kernel.  With a window, shorter tiles leave less of what no row sees in the first and the
+// last one (128 sequences of 50 - 500 rows, window 100, 4 sinks, 4 heads, fp32, us of 32 / 64: heads of 64 213 / 262, of 128
+// 363 / 446; one of 32 numbers, window 400: 45 / 33).
+template <int kDim, bool kWin> constexpr int kFwdTile = kWin && kDim > 32 ? 32 : 64;
 
 // See hstu_simt.cuh for the tile shape and what bounds it.  K_t is read by the scores only and V_t by the output only,
 // so each is fetched again while the other's products run.
@@ -38,7 +41,7 @@ template <typename T, int kDim, bool kWin>
 __global__ void __launch_bounds__(simt::kThreads) hstu_simt_fwd_kernel(const KParams p) {
   using Mask = MaskOf<kWin>;
   extern __shared__ float smem[];
-  constexpr int kCols = kFwdKeys / 16;
+  constexpr int kFwdKeys = kFwdTile<kDim, kWin>, kCols = kFwdKeys / 16;
   constexpr int kPer = simt::OutCols<kDim>::kPer;
   constexpr int ldq = kDim + 4, ldp = kFwdKeys + 4;
   const int b = blockIdx.x / p.hq, h = blockIdx.x - b * p.hq;
@@ -48,8 +51,8 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_fwd_kernel(const KPa
   if (r0 < s.lq) {
     const int dq = p.dqk, dv = p.dv;
     float* Qs = smem;                        // [32][ldq]
-    float* Ks = Qs + simt::kRows * ldq;      // [64][ldq]
-    float* Vs = Ks + kFwdKeys * ldq;         // [64][kDim]
+    float* Ks = Qs + simt::kRows * ldq;      // [kFwdKeys][ldq]
+    float* Vs = Ks + kFwdKeys * ldq;         // [kFwdKeys][kDim]
     float* Ps = Vs + kFwdKeys * kDim;        // [32][ldp]
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const T* k = static_cast<const T*>(p.k);
@@ -272,6 +275,7 @@ size_t generic_smem_bytes(const KParams& p) {
 
 template <typename T, int kDim, bool kWin>
 cudaError_t launch_simt_of(const KParams& p, cudaStream_t stream) {
+  constexpr int kFwdKeys = kFwdTile<kDim, kWin>;
   constexpr int smem = 4 * (simt::kRows * (kDim + 4) + kFwdKeys * (kDim + 4) + kFwdKeys * kDim + simt::kRows * (kFwdKeys + 4));
   cudaError_t e = cudaFuncSetAttribute(hstu_simt_fwd_kernel<T, kDim, kWin>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;

@@ -174,6 +174,40 @@ __device__ __forceinline__ void store_row(T* row, int dim, int tx, const float (
   }
 }
 
+// A result whose tiles the CTAs of a cluster share (along z, one CTA per row that a thread holds; each takes every fourth tile):
+// each lays its sums down in shared memory, and adds up and stores one row per thread, in the order of the ranks - the same
+// bits every time.
+constexpr int kSplitCtas = 4;
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// This thread's sums -> `area`, 32 * kDim floats.
+template <int kDim>
+__device__ __forceinline__ void lay_down(float* area, const float (&acc)[4][OutCols<kDim>::kPer]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int c = 0; c < OutCols<kDim>::kPer; ++c) area[(r * OutCols<kDim>::kPer + c) * kThreads + threadIdx.x] = acc[r][c];
+}
+// Row 4 ty + r of the cluster's sums.
+template <int kDim>
+__device__ __forceinline__ void add_up(const float* area, int r, float (&sum)[OutCols<kDim>::kPer]) {
+  const uint32_t here = static_cast<uint32_t>(__cvta_generic_to_shared(area));
+#pragma unroll
+  for (int c = 0; c < OutCols<kDim>::kPer; ++c) sum[c] = 0.f;
+#pragma unroll
+  for (int n = 0; n < kSplitCtas; ++n) {
+    uint32_t there;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(n));
+#pragma unroll
+    for (int c = 0; c < OutCols<kDim>::kPer; ++c) {
+      float x;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];"
+                   : "=f"(x) : "r"(there + 4u * static_cast<uint32_t>((r * OutCols<kDim>::kPer + c) * kThreads + threadIdx.x)) : "memory");
+      sum[c] += x;
+    }
+  }
+}
+
 // Head dims and alignment these kernels take: whole 4-element pieces, at most kMaxDim wide.
 inline bool dims_ok(const KParams& p) {
   return p.dqk % 4 == 0 && p.dv % 4 == 0 && p.dqk >= 4 && p.dv >= 4 && p.dqk <= kMaxDim && p.dv <= kMaxDim;
@@ -188,6 +222,7 @@ inline int tile_dim(const KParams& p) {
 
 // Launched with programmatic stream serialization: the pre-pass in front only checks the inputs (its status word), so
 // the kernel need not wait for it before its end; nor the second backward kernel for the first.
+// A grid with a z dimension is one of clusters along it.
 template <typename... P, typename... A>
 cudaError_t launch(void (*kern)(P...), dim3 grid, int smem, cudaStream_t stream, const A&... args) {
   cudaLaunchConfig_t cfg = {};
@@ -195,11 +230,14 @@ cudaError_t launch(void (*kern)(P...), dim3 grid, int smem, cudaStream_t stream,
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = grid.z;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = grid.z > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 
