@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dq_kernel(const BwdParams b
 #pragma unroll
     for (int c = 0; c < BMAXC; ++c) {
       const int col = tx + BT * c;
-      if (c < ncol && col < dq) row[col] = cvt_f<T>(acc[c]);
+      if (c < ncol && col < dq) row[col] = cvt_f<T>(kWin ? acc[c] * p.out_scale : acc[c]);
     }
   }
 }
@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dkv_kernel(const BwdParams 
 #pragma unroll
     for (int c = 0; c < BMAXC; ++c) {
       const int col = tx + BT * c;
-      if (c < ncol_k && col < dq) krow[col] = cvt_f<T>(acc_k[c]);
-      if (c < ncol_v && col < dv) vrow[col] = cvt_f<T>(acc_v[c]);
+      if (c < ncol_k && col < dq) krow[col] = cvt_f<T>(kWin ? acc_k[c] * p.out_scale : acc_k[c]);
+      if (c < ncol_v && col < dv) vrow[col] = cvt_f<T>(kWin ? acc_v[c] * p.out_scale : acc_v[c]);
     }
   }
 }
@@ -342,6 +342,7 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const 
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = r0 + 4 * ty + r;
+      if (kWin) simt::times<kPer>(acc[r], p.out_scale);
       if (i < s.lq) simt::store_row<T, kDim>(static_cast<T*>(bp.dq) + ((s.q0 + i) * p.hq + h) * dq, dq, tx, acc[r]);
     }
   }
@@ -440,8 +441,9 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
       u = un;
     }
     simt::cp_async_wait<0>();
-    auto store = [&](int j, const float (&ak)[kPer], const float (&av)[kPer]) {
+    auto store = [&](int j, float (&ak)[kPer], float (&av)[kPer]) {
       if (j >= s.lk) return;
+      if (kWin) simt::times<kPer>(ak, p.out_scale), simt::times<kPer>(av, p.out_scale);
       simt::store_row<T, kDim>(static_cast<T*>(bp.dk) + ((s.k0 + j) * p.hk + hk) * dq, dq, tx, ak);
       simt::store_row<T, kDim>(static_cast<T*>(bp.dv) + ((s.k0 + j) * p.hk + hk) * dv, dv, tx, av);
     };

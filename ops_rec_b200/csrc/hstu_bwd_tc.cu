@@ -813,6 +813,10 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
 #pragma unroll
           for (int e = 0; e < 32; ++e) acc[e] = 0u;   // nothing visible: zero gradient
         }
+        if (kWin && std::is_same<T, __half>::value) {   // (see KParams)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * p.out_scale);
+        }
         if (mine_ok) {
           uint4* dst = reinterpret_cast<uint4*>((which == 0 ? out1 : out2) + ch * 32);
 #pragma unroll

@@ -54,6 +54,7 @@ struct KParams {
   int maxq, maxk;
   int group;
   float scale;
+  float out_scale;      // of the sums (with windows and 8-bit caches): 1, or the call's scale where P and dS are formed without it
   float alpha;
   unsigned flags;
   uint32_t* ws_header;  // status, item count, counter

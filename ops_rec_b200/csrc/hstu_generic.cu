@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_fwd_kernel(const KPa
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int i = r0 + 4 * ty + r;
+      if (kWin) simt::times<kPer>(acc[r], p.out_scale);
       if (i < s.lq) simt::store_row<T, kDim>(out + ((s.q0 + i) * p.hq + h) * dv, dv, tx, acc[r]);
     }
   }
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(GTHREADS) hstu_generic_kernel(const KParams p)
 #pragma unroll
     for (int c = 0; c < GMAXC; ++c) {
       const int col = tx + 32 * c;
-      if (c < ncol && col < dv) orow[col] = from_f<T>(acc[r][c]);
+      if (c < ncol && col < dv) orow[col] = from_f<T>(kWin ? acc[r][c] * p.out_scale : acc[r][c]);
     }
   }
 }

@@ -546,6 +546,10 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
         uint32_t orr[32];
         ptx::tmem_ld32(t_s + kShColO + ch * 32, orr);
         ptx::tmem_wait_ld_dep(orr);
+        if (std::is_same<T, __half>::value) {   // (see KParams; elsewhere it is 1)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) orr[e] = __float_as_uint(__uint_as_float(orr[e]) * p.out_scale);
+        }
         if (row_ok) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {

@@ -157,6 +157,11 @@ __device__ __forceinline__ void outer_tile(const float* pm, int ldp, const float
   }
 }
 
+template <int kPer> __device__ __forceinline__ void times(float (&x)[kPer], float f) {
+#pragma unroll
+  for (int c = 0; c < kPer; ++c) x[c] *= f;
+}
+
 // The thread's columns of one output row; dim a multiple of 4, row aligned to four elements.
 template <typename T, int kDim>
 __device__ __forceinline__ void store_row(T* row, int dim, int tx, const float (&acc)[OutCols<kDim>::kPer]) {

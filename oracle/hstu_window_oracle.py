@@ -37,7 +37,7 @@ def window_mask(len_q, len_k, tgt, group, window, sink, device="cpu"):
     return see
 
 
-def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=False, unit=None):
+def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=False, unit=None, behind=False):
     """One sequence: q [lq, hq, d], k, v [lk, hk, .] -> {"out": (value, tolerance)} and with grad also dq, dk, dv.
     staged: k and v may have been rounded to the element type on their way, one rounding each: u relative, and below the type's
     normal range half of its smallest step.  Such a cache's blocks may differ by any power of two, and that shows how tensor
@@ -45,19 +45,21 @@ def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=F
     bits below it, and a P of zero has the exponent of one there.  So a masked value v costs the rows that do not see it up to
     2^-25 |v| for its group of 16 keys (seen as errors that are multiples of 2^-17 beside hidden values of 256).
     unit: [keys, hk], the scales of the values (value = number * scale).  A kernel may round P * scale instead of P, to fp16
-    relative to the row's largest: half a smallest step is then 2^-25 of that largest, for every number."""
+    relative to the row's largest: half a smallest step is then 2^-25 of that largest, for every number.
+    behind: P and dS are rounded without the scale, which the sums take: so is half a smallest step."""
     u = torch.finfo(dtype).eps / 2
     hq, hk = q.shape[1], k.shape[1]
     q, k, v = (t.double().transpose(0, 1) for t in (q, k, v))                     # [heads, rows, dim]
     kk, vv = (t.repeat_interleave(hq // hk, 0) for t in (k, v))
     f32, tiny = 2.0 ** -24, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    step = tiny * abs(scale) if behind else tiny
     x = alpha * q @ kk.transpose(1, 2)
     xerr = (q.shape[2] + 4) * f32 * abs(alpha) * (q.abs() @ kk.abs().transpose(1, 2))
     if staged:
         xerr = xerr + (u + f32) * abs(alpha) * (q.abs() @ kk.abs().transpose(1, 2)) + tiny * abs(alpha) * q.abs().sum(2, keepdim=True)
     sg = torch.sigmoid(x)
     approx = x.abs() * 2.0 ** -12 if tanh else (x * sg).abs() * 2.0 ** -20
-    perr = torch.where(see, scale * (1.1 * (xerr + approx) + (u + 4 * f32) * (x * sg).abs()) + tiny, 0.0)
+    perr = torch.where(see, scale * (1.1 * (xerr + approx) + (u + 4 * f32) * (x * sg).abs()) + step, 0.0)
     p = torch.where(see, x * sg * scale, 0.0)
     out = p @ vv
     n = k.shape[1] + 4
@@ -76,7 +78,7 @@ def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=F
         sgerr = 0.25 * xerr + (2.0 ** -12 if tanh else sg * 2.0 ** -20)
         ferr = abs(scale * alpha) * ((1 + x.abs()) * 1.1 * sgerr + xerr * 0.3) + 8 * f32 * f.abs()
         ds = torch.where(see, dp * f, 0.0)
-        dserr = torch.where(see, u * (dp * f).abs() + dp.abs() * ferr + dperr * f.abs() + dperr * ferr + tiny, 0.0)
+        dserr = torch.where(see, u * (dp * f).abs() + dp.abs() * ferr + dperr * f.abs() + dperr * ferr + step, 0.0)
         m = q.shape[1] * (hq // hk) + 4
         dq = ds @ kk
         got["dq"] = dq, u * dq.abs() + dserr @ kk.abs() + n * f32 * (ds.abs() @ kk.abs())
@@ -101,7 +103,8 @@ def hstu_window(q, k, v, window, sink=0, max_seq_len=0, max_seq_len_k=0, silu_sc
         rows, keys = slice(offq[b], offq[b + 1]), slice(offk[b], offk[b + 1])
         t = int(num_target[b]) if num_target is not None else 0
         see = window_mask(offq[b + 1] - offq[b], offk[b + 1] - offk[b], t, target_group_size, window, sink, q.device)
-        one = attention(q[rows], k[keys], v[keys], see, alpha, scale, q.dtype, grad[rows] if grad is not None else None, tanh)
+        one = attention(q[rows], k[keys], v[keys], see, alpha, scale, q.dtype, grad[rows] if grad is not None else None, tanh,
+                        behind=q.dtype == torch.float16)
         for name, pair in one.items():
             for full, part in zip(got[name], pair):
                 full[rows if name in ("out", "dq") else keys] = part

@@ -293,3 +293,35 @@ def test_inconsistent_offsets_are_flagged():
     _, st = cabi.hstu_window_backward(grad, window=10, return_status=True, **(args | dict(max_seq_len=64)))
     assert st & cabi.ST_LEN_GT_MAX
     check(args, grad, 10, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dq,dv", [(64, 64), (128, 128), (96, 96), (20, 16), (17, 32)])
+@pytest.mark.parametrize("delta", [None, 30])
+def test_half_precision_keeps_its_bits_under_a_small_scale(dq, dv, delta):
+    """fp16 with a scale of 1 / 4096: P and dS of the usual sizes times it would be below the type's normal range.  A value x that
+    is rounded once is u x / sqrt(3) off at most in the mean square (u: half a step), so a result y = sum(p w) of rounded p that
+    is rounded itself u / sqrt(3) sqrt(sum((p w)^2) + y^2), and 2^-25 / sqrt(3) where it is subnormal; a tenth on top for the sample
+    and what 32 bits add."""
+    args, grad = make([600, 300, 33], 2, 2, dq, dv, FP16, delta=delta, seed=41, max_seq_len=4096)
+    args["v"], grad, alpha, scale = args["v"] * 8, grad * 8, args["alpha"], 1 / 4096
+    out = cabi.hstu_window_forward(window=20, num_sink=2, **args)
+    got = dict(zip(("out", "dq", "dk", "dv"), (out, *cabi.hstu_window_backward(grad, window=20, num_sink=2, **args))))
+    want = {n: torch.zeros(t.shape, dtype=torch.float64, device="cuda") for n, t in got.items()}
+    square = {n: torch.zeros_like(t) for n, t in want.items()}
+    offq = args["seq_offset"].tolist()
+    offk = args["seq_offset_k"].tolist() if "seq_offset_k" in args else offq
+    for b in range(3):
+        rows, keys = slice(offq[b], offq[b + 1]), slice(offk[b], offk[b + 1])
+        q, g, k, v = (t.double().transpose(0, 1) for t in (args["q"][rows], grad[rows], args["k"][keys], args["v"][keys]))
+        see = WO.window_mask(rows.stop - rows.start, keys.stop - keys.start, 0, 0, 20, 2, "cuda")
+        x = alpha * q @ k.transpose(1, 2)
+        sg = torch.sigmoid(x)
+        p = torch.where(see, x * sg * scale, 0.0)
+        ds = torch.where(see, g @ v.transpose(1, 2) * scale * alpha * sg * (1 + x * (1 - sg)), 0.0)
+        for name, at, a, w in (("out", rows, p, v), ("dq", rows, ds, k), ("dk", keys, ds.transpose(1, 2), q), ("dv", keys, p.transpose(1, 2), g)):
+            want[name][at], square[name][at] = (a @ w).transpose(0, 1), (a ** 2 @ w ** 2).transpose(0, 1)
+    for name in got:
+        off = (got[name].double() - want[name]).square().mean().sqrt()
+        most = 1.1 * ((2.0 ** -22 * (square[name] + want[name] ** 2).mean() + 2.0 ** -50) / 3).sqrt()
+        assert off <= most, (name, (off / most).item())
