@@ -289,7 +289,8 @@ HSTU_API int hstu_cache_append(const HstuCacheAppendArgs* args, void* stream);
 
 /* hstu_paged over such a cache: the arguments of hstu_paged_fwd without mask, attn_bias and num_context (mask_type
  * HSTU_MASK_TRIL), paged.kv_cache in 8 bits.  window 0: every key up to the row's own; else the window and sinks of
- * hstu_window_fwd.  q, k, v, out in bf16, fp16 or fp32. */
+ * hstu_window_fwd.  q, k, v, out in bf16, fp16 or fp32.  The kernel, and with it the size of the workspace, follows types,
+ * sizes and the alignment of the pointers: ask for the size with the arguments of the call. */
 typedef struct HstuPaged8Args {
   uint32_t struct_bytes;  /* sizeof(HstuPaged8Args) */
   int32_t held;           /* HSTU_HELD_* */

@@ -3,7 +3,8 @@
   libhstu_b200.so   the C-ABI library: CUDA kernels for sm_100a + entry points (include/hstu_b200.h); nvcc only
   _torch_shim.so    registers the operators with torch under the reference's schema strings - ops_rec::hstu_jagged
                     (.equal / .delta), hstu_jagged_backward (.equal / .delta), hstu_dense, hstu_paged, ln_mul,
-                    distance_in_linear_silu - with their Meta implementations, and forwards to the C ABI
+                    distance_in_linear_silu; hstu_window (+ _backward), hstu_cache_append, hstu_paged_8bit, which the
+                    reference does not have - with their Meta implementations, and forwards to the C ABI
 
 Run `python ops_rec_b200/_build.py` (or call build_all()) after changing anything under csrc/.
 """

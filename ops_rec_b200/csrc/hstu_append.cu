@@ -5,11 +5,12 @@
 //   row   = round(x / scale); the rows a block holds already are rounded anew to round(number * old / scale) when it grew
 //
 // A warp does one block of tokens, of the keys or of the values: two passes over at most `block` rows, the second out of the
-// L1 / L2.  Where a head is 8, 16, .. 256 wide it takes 256 columns, whichever heads they belong to - a piece of 8 columns per
+// L1 / L2 (kept in registers between them, the rows leave an SM too few warps: 80 -> 140 us below).  Where a head is 8, 16, .. 256 wide it takes 256 columns, whichever heads they belong to - a piece of 8 columns per
 // lane, whole lines per row, and the look-ups in front shared by all of the heads - elsewhere one head.
 // Which blocks there are is known to the device only; sequence b owns the slots [seq_offset[b] / block + 2 b, ..) of the grid,
 // which are never fewer than the blocks its rows touch (n rows touch at most n / block + 2), and finds them by a 32-way search.
-// HBM-bound for histories (3 bytes per 16-bit element), a chain of six dependent reads for single rows.
+// HBM-bound for histories (3 bytes per 16-bit element: 256 of 680 rows on average, 4 heads of 64, 43 us of bytes, take 80), a chain
+// of six dependent reads for single rows (6 us of one row each of 128 users).
 #include "hstu_held.cuh"
 #include "hstu_simt.cuh"
 

@@ -2,10 +2,12 @@
 // head dims that are multiples of 16 up to 128, no targets, pages of whole 16-row tiles).
 //
 // HBM-bound: a decode step reads every visible cached row once, at one byte per element (128 users of 200 - 2048 rows, 8 heads
-// of 128: 294 MB, 46 us), and there is next to nothing to compute per byte.  So nothing is staged: a warp streams tiles of 16 keys
-// through a ring of its own in shared memory (cp.async, four stages, no barrier of the CTA in the loop; TMA boxes of 16 rows of 128
-// bytes, one for keys and one for values, came in at 3.4 TB/s at most, whatever the number of CTAs), turns the 8-bit numbers
-// into 16-bit ones in registers where the matrix instructions want them, and keeps its 16 rows of the output in registers.
+// of 128: 294 MB, 46 us; it takes 65, 4.5 TB/s), and there is little to compute per byte.  So nothing is staged: a warp streams
+// pairs of tiles of 16 keys through a ring of its own in shared memory (cp.async, two stages of a pair, no barrier of the CTA in
+// the loop; TMA boxes of 16 rows of 128 bytes, one for keys and one for values, came in at 3.4 TB/s at most, whatever the number
+// of CTAs), turns the 8-bit numbers into 16-bit ones in registers where the matrix instructions want them, and keeps its rows of
+// the output in registers.  What is left above the bytes is the set-up of a CTA, a thousand instructions a warp (4 users of 14000
+// - 20000 rows: 40 us of 22; 512 users with a window of 1024, 541 MB: 103 of 84).
 // There is no softmax: partial outputs of any split of the keys add up, first over the four warps of a CTA, then - where a
 // sequence has more keys than a CTA takes - over CTAs: each leaves its partial sums in the workspace, and the last one to arrive
 // adds them in the order of the keys (the same bits every time).

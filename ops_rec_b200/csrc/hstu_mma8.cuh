@@ -113,7 +113,7 @@ template <int kThreads> __device__ __forceinline__ void report_sequence(const KP
 }
 
 // Eight query rows as the B operands of S^T = K.Q^T: a bf16 row is divided by a power of two (its largest element to [1, 2)).
-// Returns alpha times that power.  w: pairs of one row, `lanes` bits of the four threads that hold the rest of it.
+// Returns alpha times that power.  w: this thread's pairs of one row; the four threads of a lane group hold the rest of it.
 template <typename T, int kPairs> __device__ __forceinline__ float to_fp16_row(uint32_t (&w)[kPairs], float alpha) {
   if constexpr (std::is_same<T, __half>::value) {
     return alpha;

@@ -6,7 +6,9 @@
 // small: a (user, head) has 17 tiles of 16 keys.  So as in the decode kernel nothing is staged in memory, and the matrix
 // instructions have the cache as their A operand; but here a warp owns rows - two groups of eight - and all four warps of a CTA
 // share the tiles: 32 keys at a time arrive in a ring of raw numbers (cp.async, three stages ahead; each thread reads back only
-// what it fetched itself), are turned into fp16 once, and put into one of two buffers, one barrier per 32 keys.
+// what it fetched itself), are turned into fp16 once, and put into one of two buffers, one barrier per 32 keys.  (64 users of 200 -
+// 2048 rows, 4 heads of 64, 80 rows: 43 us, where pages unpacked for the tcgen05 kernel take 74; 128 users, 8 heads of 128, 9
+// rows: 245 of 46 of bytes.  With many more problems than the SMs hold the set-up of each counts, and unpacking wins.)
 //   S^T = K.Q^T, O^T += V^T.P^T   ldmatrix, for V with .trans; P changes from accumulator to operand with movmatrix
 //   P    SiLU(x) times the value's scale and the row's power of two (see hstu_decode8.cu), rounded once; the products around SiLU
 //        on pairs of scores (tanh on two halves at once is no faster, and 1 + tanh from halves is 2^-12 off where it is small)

@@ -17,6 +17,11 @@
 //   warp 4     one thread: draws tiles (scheduler), requests Q, K / V ring and bias tiles by TMA
 //   warp 5     TMEM allocation; one thread issues the MMAs
 //
+// With a window (hstu_window, hstu_paged_8bit) a Q tile visits the tiles of the sinks and then those from the first key that one of
+// its rows sees, so a long sequence is many short chains too: bf16, 4 heads of 128, 32 sequences of 256 - 1024 rows, window 256,
+// 43 us (13 of bytes); 16 of 4096 - 8192, window 512 and 16 sinks, 220 us (62 of bytes, 70 of products), 1600 cycles per 64 keys
+// and SM; 8 of 20 - 200, heads of 64, 13 us.
+//
 // Element-wise stage, masks, work list and numerics are hstu_tc.cu's, except that a staged bias is added in registers
 // (which needs no identity products and no special case at the end of a sequence).  Every mbarrier wait is bounded.
 #include <cuda.h>
