@@ -209,8 +209,13 @@ int hstu_jagged_fwd_kernel_kind(const HstuJaggedArgs* args) {
 static void scale_behind(hstu::KParams* p, int dtype);
 
 // `paged` (hstu_paged, hstu_window): parameters that carry what HstuJaggedArgs has no place for - the page table, the window.
+// `unpacked` (hstu_paged_8bit): where the pages of `paged` go, in the call's type, before the attention, and their table.
+struct UnpackedPages {
+  void* pages;
+  void* table;
+};
 static int jagged_fwd_impl(const HstuJaggedArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v,
-                           const hstu::KParams* paged);
+                           const hstu::KParams* paged, const UnpackedPages* unpacked = nullptr);
 
 int hstu_jagged_fwd(const HstuJaggedArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v) {
   g_err[0] = 0;
@@ -218,7 +223,7 @@ int hstu_jagged_fwd(const HstuJaggedArgs* args, void* workspace, uint64_t worksp
 }
 
 static int jagged_fwd_impl(const HstuJaggedArgs* args, void* workspace, uint64_t workspace_bytes, void* stream_v,
-                           const hstu::KParams* paged) {
+                           const hstu::KParams* paged, const UnpackedPages* unpacked) {
   int rc = validate(args);
   if (rc) return rc;
   rc = validate_pointers(args);
@@ -254,10 +259,20 @@ static int jagged_fwd_impl(const HstuJaggedArgs* args, void* workspace, uint64_t
     p.sink = paged->sink;
     if (p.window || (p.paged_split && paged->kv_scale)) scale_behind(&p, args->dtype);
   }
+  const hstu::KParams as_called = p;   // (the pre-pass checks the page table as it came)
+  if (unpacked) {
+    p.kv_cache = unpacked->pages;
+    p.page_ids = unpacked->table;
+    p.num_pages = p.num_page_ids;
+  }
   const bool tc = wants_tc(args, p);
-  cudaError_t e = hstu::launch_prepass(p, tc, stream);
+  cudaError_t e = hstu::launch_prepass(as_called, tc, stream);
   if (e != cudaSuccess) return fail(HSTU_E_CUDA, "pre-pass launch: %s", cudaGetErrorString(e));
   if (args->total_q == 0) return HSTU_OK;
+  if (unpacked) {
+    e = hstu::launch_unpack(*paged, unpacked->pages, unpacked->table, args->dtype, stream);
+    if (e != cudaSuccess) return fail(HSTU_E_CUDA, "unpack launch: %s", cudaGetErrorString(e));
+  }
   if (tc) {
     e = hstu::launch_tc(p, args->dtype, dev.sms, stream);
     if (e == cudaErrorNotSupported) return fail(HSTU_E_CUDA, "cuTensorMapEncodeTiled failed or is unavailable");
@@ -585,13 +600,9 @@ int hstu_paged_8bit_fwd(const HstuPaged8Args* args, void* workspace, uint64_t wo
     void* pages = base + pl.fwd_bytes;
     void* table = base + pl.fwd_bytes + unpacked_bytes(p);
     pl.fwd.k = pl.fwd.v = pages;   // (not read: keys and values are the pages and the call's own rows)
-    const cudaError_t e = hstu::launch_unpack(p, pages, table, pl.fwd.dtype, stream);
-    if (e != cudaSuccess) return fail(HSTU_E_CUDA, "unpack launch: %s", cudaGetErrorString(e));
-    p.kv_cache = pages;
-    p.page_ids = table;
-    p.num_pages = p.num_page_ids;
     p.paged_split = 1;
-    return jagged_fwd_impl(&pl.fwd, workspace, pl.fwd_bytes, stream_v, &p);
+    const UnpackedPages unpacked = {pages, table};
+    return jagged_fwd_impl(&pl.fwd, workspace, pl.fwd_bytes, stream_v, &p, &unpacked);
   }
   const cudaError_t e = hstu::launch_paged_gather(p, a->kv_cache, b->k, b->v, base + pl.fwd_bytes, base + pl.fwd_bytes + pl.stage_bytes,
                                                   pl.capacity, a->num_pages, a->num_page_ids, pl.fwd.dtype, stream);

@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kGatherThreads) hstu_paged_gather_kernel(const
 // call's type - a cache of its own whose page i is slot i, with the table of its pages.  Rows nobody reads (behind a sequence's
 // last one, and a whole tile of 64 keys away from what a window or its sinks show) stay unwritten.  HBM-bound: one byte in, two
 // out (10 600 pages of 128 rows, 4 heads of 64, 80 % full: 1.5 GB, 244 us, 6.2 TB/s; in pieces of 16 numbers, whose stores do not
-// fill lines, 263).
+// fill lines, 263); the pre-pass runs beside it (15 us of 600 of such a call).
 constexpr int kUnpackThreads = 256;
 
 struct UnpackParams {
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(kUnpackThreads) hstu_unpack_kernel(const Unpac
   const int b = s_b;
   const long long pid = load_index(p.page_ids, p.index_bytes, slot);
   const bool ok = pid >= 0 && pid < p.num_pages;
-  if (threadIdx.x == 0) {   // (a page outside of the cache stays one, for the pre-pass's check)
+  if (threadIdx.x == 0) {   // (a page outside of the cache stays one)
     if (p.index_bytes == 8) static_cast<long long*>(p.table)[slot] = ok ? slot : -1;
     else static_cast<int*>(p.table)[slot] = ok ? static_cast<int>(slot) : -1;
   }
@@ -345,6 +345,8 @@ __global__ void __launch_bounds__(kUnpackThreads) hstu_unpack_kernel(const Unpac
       to[at[u]] = make_uint4(x[0], x[1], x[2], x[3]);
     }
   }
+  // Launched beside the pre-pass, which writes nothing this one reads; the kernel behind it finds both complete.
+  if (slot == p.num_page_ids - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace
@@ -380,14 +382,19 @@ cudaError_t launch_unpack(const KParams& p, void* out, void* table, int dtype, c
   u.by_row = inverse_of(p.hk * p.dqk / 8);
   u.by_head = inverse_of(p.dqk / 8);
   u.by_block = inverse_of(p.scale_block);
-  const dim3 grid(static_cast<unsigned>(p.num_page_ids), 1, 1);
-#define HSTU_UNPACK(TT)                                                                                            \
-  if (p.held == HSTU_HELD_E4M3) hstu_unpack_kernel<TT, E4m3><<<grid, kUnpackThreads, 0, stream>>>(u);             \
-  else hstu_unpack_kernel<TT, Int8><<<grid, kUnpackThreads, 0, stream>>>(u)
-  if (dtype == HSTU_DTYPE_BF16) { HSTU_UNPACK(__nv_bfloat16); }
-  else { HSTU_UNPACK(__half); }
-#undef HSTU_UNPACK
-  return cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.num_page_ids));
+  cfg.blockDim = dim3(kUnpackThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const bool held = p.held == HSTU_HELD_E4M3;
+  if (dtype == HSTU_DTYPE_BF16)
+    return cudaLaunchKernelEx(&cfg, held ? hstu_unpack_kernel<__nv_bfloat16, E4m3> : hstu_unpack_kernel<__nv_bfloat16, Int8>, u);
+  return cudaLaunchKernelEx(&cfg, held ? hstu_unpack_kernel<__half, E4m3> : hstu_unpack_kernel<__half, Int8>, u);
 }
 
 template <typename T, int kN>
