@@ -4,12 +4,14 @@
 //           block and head; where the block holds rows already, no smaller than the scale they have
 //   row   = round(x / scale); the rows a block holds already are rounded anew to round(number * old / scale) when it grew
 //
-// A warp does one block of tokens, of the keys or of the values: two passes over at most `block` rows, the second out of the
-// L1 / L2 (kept in registers between them, the rows leave an SM too few warps: 80 -> 140 us below).  Where a head is 8, 16, .. 256 wide it takes 256 columns, whichever heads they belong to - a piece of 8 columns per
-// lane, whole lines per row, and the look-ups in front shared by all of the heads - elsewhere one head.
+// A warp does one block of tokens, of the keys or of the values: two passes over at most `block` rows.  Where a head is 8, 16, ..
+// 256 wide it takes 256 columns, whichever heads they belong to - a piece of 8 columns per lane, whole lines per row, and the
+// look-ups in front shared by all of the heads - elsewhere one head.  Of 16-bit histories the rows arrive in shared memory, all
+// requested at once (cp.async), and stay there between the passes; read twice from memory instead, eight rows at a time, they come
+// out of the L2 the second time (80 us below), and kept in registers they leave an SM too few warps (140).
 // Which blocks there are is known to the device only; sequence b owns the slots [seq_offset[b] / block + 2 b, ..) of the grid,
 // which are never fewer than the blocks its rows touch (n rows touch at most n / block + 2), and finds them by a 32-way search.
-// HBM-bound for histories (3 bytes per 16-bit element: 256 of 680 rows on average, 4 heads of 64, 43 us of bytes, take 80), a chain
+// HBM-bound for histories (3 bytes per 16-bit element: 256 of 680 rows on average, 4 heads of 64, 43 us of bytes, take 53: 5 TB/s), a chain
 // of six dependent reads for single rows (6 us of one row each of 128 users).
 #include "hstu_held.cuh"
 #include "hstu_simt.cuh"
@@ -34,6 +36,8 @@ struct AppendParams {
 };
 
 constexpr int kAppendThreads = 256;
+constexpr int kStagedThreads = 32;
+constexpr int kStagedRows = 32;   // of a block, at most: 16 KB a warp, 13 warps on an SM
 
 // Eight elements (or one) of a row, as floats.
 template <typename T, int kN> struct Piece;
@@ -171,11 +175,13 @@ __device__ __forceinline__ AppendWork find_work(const AppendParams& p, long long
   return w;
 }
 
-// 256 columns a warp: see the top.
-template <typename T, typename H>
-__global__ void __launch_bounds__(kAppendThreads) hstu_append_columns_kernel(const AppendParams p) {
+// 256 columns a warp: see the top.  kStaged: the block's rows lie in shared memory between the passes, 512 bytes each.
+template <typename T, typename H, bool kStaged>
+__global__ void __launch_bounds__(kStaged ? kStagedThreads : kAppendThreads) hstu_append_columns_kernel(const AppendParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int kWarps = (kStaged ? kStagedThreads : kAppendThreads) / 32;
   const int lane = threadIdx.x & 31;
-  const long long unit = static_cast<long long>(blockIdx.x) * (kAppendThreads / 32) + (threadIdx.x >> 5);
+  const long long unit = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const int row_len = p.heads * p.dim, spans = (row_len + 255) / 256;
   const long long slot = unit / (2 * spans);
   if (slot >= p.total / p.block + 2ll * p.batch) return;
@@ -185,18 +191,28 @@ __global__ void __launch_bounds__(kAppendThreads) hstu_append_columns_kernel(con
   const bool on = col < row_len;
   const int head = on ? col / p.dim : 0;
   const T* src = static_cast<const T*>(kv ? p.v : p.k) + w.first * row_len + (on ? col : 0);
+  long long src_len = row_len;
+  if (kStaged) {   // (a lane reads back what it fetched itself)
+    uint8_t* const mine = smem + (threadIdx.x >> 5) * p.block * 512 + lane * 16;
+    for (int r = 0; r < w.count; ++r)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(mine + r * 512))),
+                   "l"(src + static_cast<long long>(r) * row_len) : "memory");
+    src = reinterpret_cast<const T*>(mine);
+    src_len = 512 / sizeof(T);
+  }
   uint8_t* dst = p.cache + (w.place + kv * static_cast<long long>(p.page_size)) * row_len + (on ? col : 0);
   float* scale_at = p.scale + w.scale + kv * static_cast<long long>(p.page_size / p.block) * p.heads + head;
   const float old = on && w.held > 0 ? *scale_at : 0.f;
+  if (kStaged) asm volatile("cp.async.wait_all;" ::: "memory");
   Largest<T> most;
 #pragma unroll 8
-  for (int r = 0; r < w.count; ++r) most.take(src + static_cast<long long>(r) * row_len);
+  for (int r = 0; r < w.count; ++r) most.take(src + r * src_len);
   float amax = most.get();
   if (__any_sync(0xffffffffu, amax > 3.402823466e38f)) {   // infinities among them: over the finite values alone
     amax = 0.f;
     for (int r = 0; r < w.count; ++r) {
       float x[8];
-      Piece<T, 8>::load(src + static_cast<long long>(r) * row_len, x);
+      Piece<T, 8>::load(src + r * src_len, x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float a = fabsf(x[e]);
@@ -230,7 +246,7 @@ __global__ void __launch_bounds__(kAppendThreads) hstu_append_columns_kernel(con
 #pragma unroll 8
     for (int r = 0; r < w.count; ++r) {
       float x[8];
-      Piece<T, 8>::load(src + static_cast<long long>(r) * row_len, x);
+      Piece<T, 8>::load(src + r * src_len, x);
       const uint32_t lo = H::from_floats(divide(x[0]), divide(x[1])) | (H::from_floats(divide(x[2]), divide(x[3])) << 16);
       const uint32_t hi = H::from_floats(divide(x[4]), divide(x[5])) | (H::from_floats(divide(x[6]), divide(x[7])) << 16);
       *reinterpret_cast<uint2*>(dst + static_cast<long long>(r) * row_len) = make_uint2(lo, hi);
@@ -323,7 +339,18 @@ cudaError_t launch_append_t(const AppendParams& p, cudaStream_t stream) {
                    (reinterpret_cast<uintptr_t>(p.cache) & 7u) == 0;
   if (vec && p.dim <= 256 && (p.dim & (p.dim - 1)) == 0) {
     const long long columns = (p.total / p.block + 2ll * p.batch) * 2 * ((p.heads * p.dim + 255) / 256);
-    hstu_append_columns_kernel<T, H><<<static_cast<unsigned>((columns + kAppendThreads / 32 - 1) / (kAppendThreads / 32)), kAppendThreads, 0, stream>>>(p);
+    // Staged where blocks are at least half full on average and rows fill a warp's columns.  us staged / not, 4 heads of 64, blocks
+    // of 32: 2000 users of 1 / 8 / 16 rows 16.6 / 14.5, 18.8 / 18.6, 22.7 / 24.7, 1000 of 64 27 / 41; blocks of 8, 2000 of 4 rows 14.5 /
+    // 16.6; 300 of 300 rows, 1 head of 32 37 / 29, 8 of 128 97 / 147.
+    if constexpr (sizeof(T) == 2) {
+      if (p.block <= kStagedRows && 2 * (p.total / p.batch) >= p.block && p.heads * p.dim >= 256) {
+        constexpr int kWarps = kStagedThreads / 32;
+        hstu_append_columns_kernel<T, H, true><<<static_cast<unsigned>((columns + kWarps - 1) / kWarps), kStagedThreads, kWarps * p.block * 512, stream>>>(p);
+        return cudaGetLastError();
+      }
+    }
+    constexpr int kWarps = kAppendThreads / 32;
+    hstu_append_columns_kernel<T, H, false><<<static_cast<unsigned>((columns + kWarps - 1) / kWarps), kAppendThreads, 0, stream>>>(p);
   } else if (vec) hstu_append_kernel<T, H, 8><<<grid, kAppendThreads, 0, stream>>>(p);
   else hstu_append_kernel<T, H, 1><<<grid, kAppendThreads, 0, stream>>>(p);
   return cudaGetLastError();

@@ -550,3 +550,22 @@ def test_paged_a_loose_bound_of_the_lengths(users, new, targets):
     args = make(cached, np.full(users, new), None if targets is None else np.full(users, targets), 2, 1, 64, seed=35)
     check_paged(args | dict(max_seq_len_k=20480))
     check_paged(args | dict(max_seq_len_k=20480), 20, 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,held", [(BF16, E4M3), (FP16, INT8), (FP16, E4M3)])
+@pytest.mark.parametrize("hk,d,page,block", [(4, 64, 64, 32), (5, 64, 32, 32), (1, 256, 24, 8), (16, 16, 10, 5), (3, 128, 16, 1), (4, 64, 64, 64)])
+def test_append_histories(dtype, held, hk, d, page, block):
+    """Rows that fill a warp's columns, blocks that are mostly full: with infinities, NaN and blocks that grow."""
+    args = make([300, 33, 1, 129, 64], [300, 20, 1, 100, 0], [7, 0, 2, 0, 3], hk=hk, hq=hk, d=d, dtype=dtype, held=held, page=page, block=block, seed=50 + d)
+    check_append(args)
+    args["k"], args["v"] = args["k"] * 37, args["v"] * 0.01
+    args["k"][3, 0, 5], args["v"][40, hk - 1, 7], args["v"][6, 0, 1], args["v"][70] = float("inf"), float("-inf"), float("nan"), float("nan")
+    check_append(args)
+    wide = {n: torch.zeros(args[n].shape[0], 2 * hk, d, dtype=dtype) for n in ("k", "v")}     # heads of a larger tensor
+    for n in wide:
+        wide[n][:, ::2] = args[n]
+    cache, scale = CO.append(**table(args, False))
+    t = table(args) | {n: x.cuda()[:, ::2] for n, x in wide.items()}
+    append_op(**t)
+    assert torch.equal(t["kv_cache"].cpu().view(torch.uint8), cache.view(torch.uint8)) and torch.equal(t["kv_scale"].cpu(), scale)
