@@ -569,3 +569,23 @@ def test_append_histories(dtype, held, hk, d, page, block):
     t = table(args) | {n: x.cuda()[:, ::2] for n, x in wide.items()}
     append_op(**t)
     assert torch.equal(t["kv_cache"].cpu().view(torch.uint8), cache.view(torch.uint8)) and torch.equal(t["kv_scale"].cpu(), scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("users,new,d", [(3, 1, 64), (3, 30, 64), (MANY, 40, 64), (3, 5, 320)])
+def test_offsets_beyond_32_bits(users, new, d):
+    """The same pages at the end of a cache of more than 4 GB: the same bits, from the attention and of the append."""
+    rng = np.random.default_rng(51)
+    cached = rng.integers(new, 300, users)
+    args = on_gpu(make(cached, np.full(users, new), None, 4, 4, d, page=64, block=32, seed=52))
+    small, shift = args["kv_cache"], (5 << 30) // (2 * 64 * 4 * d)
+    far = args | dict(page_ids=args["page_ids"] + shift)
+    far["kv_cache"] = torch.empty(shift + small.shape[0], *small.shape[1:], dtype=small.dtype, device="cuda")
+    far["kv_scale"] = torch.empty(shift + small.shape[0], *args["kv_scale"].shape[1:], device="cuda")
+    for n in ("kv_cache", "kv_scale"):
+        far[n][shift:] = args[n]
+    for window in (0, 70):
+        assert torch.equal(cabi.hstu_paged_8bit_forward(**far, window=window), cabi.hstu_paged_8bit_forward(**args, window=window))
+    for a in (args, far):
+        assert cabi.hstu_cache_append(**{n: a[n] for n in TABLE}, return_status=True) == 0
+    assert torch.equal(far["kv_cache"][shift:].view(torch.uint8), small.view(torch.uint8)) and torch.equal(far["kv_scale"][shift:], args["kv_scale"])
