@@ -68,6 +68,7 @@ template <int D, typename T, typename H, bool kWin, bool kTanh>
 __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecParams d) {
   using C = DecCfg<D>;
   using Mask = MaskOf<kWin>;
+  constexpr bool kFine = std::is_same<T, __half>::value;
   const KParams& p = d.f;
   extern __shared__ __align__(128) uint8_t ring_of_all[];
   __shared__ long long s_row[kDecMostTiles];     // where the tile's keys start in the cache, -1: no such page
@@ -249,11 +250,13 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
       m[0] = fmaxf(m[0], fmaxf(fabsf(pv[t][0]), fabsf(pv[t][2])));
       m[1] = fmaxf(m[1], fmaxf(fabsf(pv[t][1]), fabsf(pv[t][3])));
     }
+    bool finite = true;
     if (__any_sync(0xffffffffu, m[0] * down[0] > 16384.f || m[1] * down[1] > 16384.f)) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], x));
+        finite &= !(m[e] > 3.402823466e38f);
         if (!(m[e] * down[e] > 16384.f) || m[e] > 3.402823466e38f) continue;
         const float next = down_to_one(m[e]), ratio2 = next / down[e];
         down[e] = next;
@@ -261,12 +264,21 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
         for (int j = 0; j < D / 16; ++j) o[j][e] *= ratio2, o[j][2 + e] *= ratio2;
       }
     }
-    uint32_t pb[kPair][2];
+    // In fp16 calls P is two halves, the rounded one and what it leaves: rounded once it costs as much again as the output's own
+    // rounding (1.4 times the error; 3 bits less than fp16's, bf16's output does not notice).
+    uint32_t pb[kPair][2], pl[kPair][2];
 #pragma unroll
-    for (int t = 0; t < kPair; ++t) {
-      pb[t][0] = transposed(pack2<__half>(pv[t][0] * down[0], pv[t][1] * down[1]));
-      pb[t][1] = transposed(pack2<__half>(pv[t][2] * down[0], pv[t][3] * down[1]));
-    }
+    for (int t = 0; t < kPair; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = pv[t][2 * h] * down[0], y = pv[t][2 * h + 1] * down[1];
+        const uint32_t rounded = pack2<__half>(x, y);
+        pb[t][h] = transposed(rounded);
+        if (kFine) {   // (of an infinite P there is nothing left)
+          const float2 r = unpack2<__half>(rounded);
+          pl[t][h] = transposed(finite ? pack2<__half>(x - r.x, y - r.y) : 0u);
+        }
+      }
     // O^T += V^T.P^T
     const uint32_t v_at = ring_at + at + C::kTile + v_row * D;
 #pragma unroll
@@ -282,6 +294,7 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
           to_halves<H>(__byte_perm(w[2 * u], 0u, 0x3120), a[0], a[1]);
           to_halves<H>(__byte_perm(w[2 * u + 1], 0u, 0x3120), a[2], a[3]);
           mma16816(o[j + u], a, pb[t]);
+          if (kFine) mma16816(o[j + u], a, pl[t]);
         }
       }
     __syncwarp();   // the stage is free

@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
   using C = RwCfg<D>;
   constexpr int kRwGroups = C::kGroups, kRwWarps = C::kWarps, kRwThreads = C::kThreads;
   using Mask = MaskOf<kWin>;
+  constexpr bool kFine = std::is_same<T, __half>::value;
   const KParams& p = d.f;
   extern __shared__ __align__(256) uint8_t smem[];   // [2][K, V][32][D] halves; at the end the output
   __shared__ long long s_row[kRwMostTiles];          // where the tile's keys start in the cache, -1: no such page
@@ -278,7 +279,7 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
       const bool full = key + kRwKeys <= full_end && (!kWin || key > full_from || key + kRwKeys <= p.sink);
       const float ks[2] = {s_factor[buf][0][t * 16 + g], s_factor[buf][0][t * 16 + g + 8]};
       const float vs[2] = {s_factor[buf][1][t * 16 + g], s_factor[buf][1][t * 16 + g + 8]};
-      uint32_t pb[kRwGroups][2];
+      uint32_t pb[kRwGroups][2], pl[kRwGroups][2];   // pl: what the rounding of P leaves, in fp16 calls (see hstu_decode8.cu)
 #pragma unroll
       for (int u = 0; u < kRwGroups; ++u) {
         if (u >= groups) continue;
@@ -304,7 +305,12 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float2 w = __fmul2_rn(y[h], down[u]);
-            pb[u][h] = pack2<__half>(w.x, w.y) & see[h];
+            pb[u][h] = pack2<__half>(w.x, w.y);
+            if (kFine) {
+              const float2 r = unpack2<__half>(pb[u][h]);
+              pl[u][h] = pack2<__half>(w.x - r.x, w.y - r.y) & see[h];
+            }
+            pb[u][h] &= see[h];
           }
           return __hble2(__hmax2_nan(__habs2(as_half2(pb[u][0])), __habs2(as_half2(pb[u][1]))), __floats2half2_rn(16384.f, 16384.f));
         };
@@ -326,10 +332,11 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
 #pragma unroll
             for (int j = 0; j < D / 16; ++j) o[u][j][e] *= change, o[u][j][2 + e] *= change;
           }
-          form();
+          if (!form() && kFine) pl[u][0] = pl[u][1] = 0u;   // (nothing is left of an infinite P)
         }
         pb[u][0] = transposed(pb[u][0]);
         pb[u][1] = transposed(pb[u][1]);
+        if (kFine) pl[u][0] = transposed(pl[u][0]), pl[u][1] = transposed(pl[u][1]);
       }
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) {
@@ -337,7 +344,10 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
         ldsm_x4_trans((v_lane + tile_at) ^ (32 * j), a);
 #pragma unroll
         for (int u = 0; u < kRwGroups; ++u)
-          if (u < groups) mma16816(o[u][j], a, pb[u]);
+          if (u < groups) {
+            mma16816(o[u][j], a, pb[u]);
+            if (kFine) mma16816(o[u][j], a, pl[u]);
+          }
       }
     }
     __syncthreads();

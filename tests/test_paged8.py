@@ -589,3 +589,16 @@ def test_offsets_beyond_32_bits(users, new, d):
     for a in (args, far):
         assert cabi.hstu_cache_append(**{n: a[n] for n in TABLE}, return_status=True) == 0
     assert torch.equal(far["kv_cache"][shift:].view(torch.uint8), small.view(torch.uint8)) and torch.equal(far["kv_scale"][shift:], args["kv_scale"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("held", [E4M3, INT8])
+@pytest.mark.parametrize("new,d,targets", [(1, 64, None), (1, 128, None), (20, 64, None), (9, 128, [3, 8, 5, 1])])
+def test_half_precision_loses_nothing_but_its_own_rounding(held, new, d, targets):
+    """fp16 in place: P is held in two halves, 2^-22 of it off, so what the output is off is its own rounding - a tenth on top for
+    SiLU's 2^-20 and for sums of 32 bits."""
+    args = on_gpu(make([200, 77, 640, 31], [new] * 4, targets, 4, 2, d, FP16, held, 64, 16, seed=53))
+    want, _ = CO.paged(**args)
+    out = cabi.hstu_paged_8bit_forward(**args)
+    off, least = ((x.double() - want).square().mean().sqrt().item() for x in (out, want.half()))
+    assert off <= 1.1 * least, off / least
