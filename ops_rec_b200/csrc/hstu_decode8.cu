@@ -18,7 +18,7 @@
 //   S^T = K.Q^T    bf16 queries are divided by a power of two per row, which keeps all 8 bits of every element that counts.  A
 //                  thread's 16 bytes of a key are contiguous; the same permutation of the contraction is applied to Q.  The
 //                  key's scale, alpha and the row's power of two multiply the 32-bit score.
-//   P              silu(x) * (scale of the value's block), rounded once, divided by a power of two per row that follows the
+//   P              silu(x) * (scale of the value's block), rounded once (two halves in fp16 calls), divided by a power of two per row that follows the
 //                  largest P so far (raised, and the output rescaled, when P outgrows 2^14), since neither scores nor scales
 //                  keep P inside fp16's narrow range
 //   O^T += V^T.P^T V is read with ldmatrix.trans as pairs of bytes; the even columns of the head are the rows 0-7 of A, the odd

@@ -10,7 +10,7 @@
 // 2048 rows, 4 heads of 64, 80 rows: 43 us, where pages unpacked for the tcgen05 kernel take 74; 128 users, 8 heads of 128, 9
 // rows: 245 of 46 of bytes.  With many more problems than the SMs hold the set-up of each counts, and unpacking wins.)
 //   S^T = K.Q^T, O^T += V^T.P^T   ldmatrix, for V with .trans; P changes from accumulator to operand with movmatrix
-//   P    SiLU(x) times the value's scale and the row's power of two (see hstu_decode8.cu), rounded once; the products around SiLU
+//   P    SiLU(x) times the value's scale and the row's power of two (see hstu_decode8.cu: rounded once, in fp16 calls two halves); the products around SiLU
 //        on pairs of scores (tanh on two halves at once is no faster, and 1 + tanh from halves is 2^-12 off where it is small)
 // Targets see the cached keys as a row right behind the history would; what they see of each other - their own group, up to
 // themselves - is added at the end in 32 bits (groups of up to four; with one target per group a row's own key and value).
