@@ -286,9 +286,12 @@ static int jagged_fwd_impl(const HstuJaggedArgs* args, void* workspace, uint64_t
 // fp16 has five bits of exponent: P = SiLU(x) scale with its usual scale of 1 / max_seq_len is subnormal in long sequences (0.1 /
 // 2000 keeps 9 of 11 bits), dS more so.  Where results take the scale behind their sums instead - with a window, and over pages
 // in 8 bits - P and dS are formed without it.  (7 sequences of 95 - 1915 rows, window 71: error of the output against 64 bits
-// 3.5e-4 -> 2.9e-4, two roundings.)
+// 3.5e-4 -> 2.9e-4, two roundings.)  What then lies beyond fp16 - a score above 65504, dS of loss-scaled gradients - although the
+// scaled one does not, the tensor-core kernels do again with the scale inside (KParams::turn); those on CUDA cores hold P and dS in
+// 32 bits.
 static void scale_behind(hstu::KParams* p, int dtype) {
   if (dtype != HSTU_DTYPE_FP16) return;
+  p->turn = p->scale < 1.0f && p->scale > -1.0f ? 1 : 0;   // (otherwise the scale brings nothing into range)
   p->out_scale = p->scale;
   p->scale = 1.0f;
 }

@@ -56,7 +56,7 @@ __device__ __forceinline__ float bias_at(const KParams& p, int b, int h, int i, 
 // P (rounded) and dS (rounded) of element (i, j) from the raw dot products s = q_i.k_j and dp = dO_i.v_j.
 // d_bias gets dS for the reference's x = alpha (S + bias) and dX for the alpha-before-bias variant.
 // bv: bias_at(i, j) of a visible element (unused without a bias)
-template <typename T>
+template <typename T, bool kWin>
 __device__ __forceinline__ void score_grad(const KParams& p, int b, int h, int i, int j, bool visible, float s, float dp,
                                            float bv, float* p_out, float* ds_out, float* dbias_out) {
   // (selects, no branch around the arithmetic: a thread has up to sixteen elements in a row)
@@ -71,9 +71,10 @@ __device__ __forceinline__ void score_grad(const KParams& p, int b, int h, int i
   }
   const float sg = simt::divide(1.f, 1.f + expf(-x));
   const float dx = dp * p.scale * m * sg * (1.f + x * (1.f - sg));
-  const float pv = visible ? round_to<T>(x * sg * p.scale * m) : 0.f;
-  const float ds = visible ? round_to<T>(dx * p.alpha) : 0.f;
-  const float db = visible ? (alpha_first ? round_to<T>(dx) : round_to<T>(dx * p.alpha)) : 0.f;
+  using R = simt::HeldIn<T, kWin>;
+  const float pv = visible ? round_to<R>(x * sg * p.scale * m) : 0.f;
+  const float ds = visible ? round_to<R>(dx * p.alpha) : 0.f;
+  const float db = visible ? (alpha_first ? round_to<R>(dx) : round_to<R>(dx * p.alpha)) : 0.f;
   *p_out = pv;
   *ds_out = ds;
   *dbias_out = db;
@@ -146,7 +147,7 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dq_kernel(const BwdParams b
     const int j = c0 + tx;
     const bool visible = i < s.lq && j < s.lk && allowed(rb, j);
     float pv, ds, db;
-    score_grad<T>(p, b, h, i, j, visible, sc, dp, visible && p.bias ? bias_at<T>(p, b, h, i, j) : 0.f, &pv, &ds, &db);
+    score_grad<T, kWin>(p, b, h, i, j, visible, sc, dp, visible && p.bias ? bias_at<T>(p, b, h, i, j) : 0.f, &pv, &ds, &db);
     Ds[ty * BT + tx] = ds;
     if (dbias && i < p.maxq && j < p.maxk) dbias[(brow0 + i) * p.maxk + j] = cvt_f<T>(db);
     __syncthreads();
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(BTHREADS) hstu_bwd_dkv_kernel(const BwdParams 
       for (int d = 0; d < dv; ++d) dp = fmaf(Gs[ty * ldv + d], Vs[tx * ldv + d], dp);
       const bool visible = i < s.lq && j < s.lk && allowed(rb, j);
       float pv, ds, db;
-      score_grad<T>(p, b, h, i, j, visible, sc, dp, visible && p.bias ? bias_at<T>(p, b, h, i, j) : 0.f, &pv, &ds, &db);
+      score_grad<T, kWin>(p, b, h, i, j, visible, sc, dp, visible && p.bias ? bias_at<T>(p, b, h, i, j) : 0.f, &pv, &ds, &db);
       Ps[ty * BT + tx] = pv;
       Ds[ty * BT + tx] = ds;
       __syncthreads();
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dq_kernel(const 
         for (int c = 0; c < kCols; ++c) {
           const int i = r0 + 4 * ty + r, j = c0 + tx + 16 * c;
           float pv, ds, db;
-          score_grad<T>(p, b, h, i, j, allowed(rb[r], j), sc[r][c], dp[r][c], bv[r][c], &pv, &ds, &db);
+          score_grad<T, kWin>(p, b, h, i, j, allowed(rb[r], j), sc[r][c], dp[r][c], bv[r][c], &pv, &ds, &db);
           Ds[(4 * ty + r) * ldp + tx + 16 * c] = ds;
           if (dbias && i < p.maxq && j < p.maxk) dbias[(brow0 + i) * p.maxk + j] = cvt_f<T>(db);
         }
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_bwd_dkv_kernel(const
         for (int c = 0; c < kCols; ++c) {
           const int i = r0 + tx + 16 * c, j = c0 + 4 * ty + r;
           float pv, ds, db;
-          score_grad<T>(p, b, h, i, j, allowed(rb[c], j), sc[r][c], dp[r][c], bv[r][c], &pv, &ds, &db);
+          score_grad<T, kWin>(p, b, h, i, j, allowed(rb[c], j), sc[r][c], dp[r][c], bv[r][c], &pv, &ds, &db);
           Ps[(4 * ty + r) * ldp + tx + 16 * c] = pv;
           Ds[(4 * ty + r) * ldp + tx + 16 * c] = ds;
         }

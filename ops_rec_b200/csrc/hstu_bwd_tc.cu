@@ -35,6 +35,7 @@
 #include <type_traits>
 
 #include "hstu_common.cuh"
+#include "hstu_tc_common.cuh"
 #include "ptx_sm100.cuh"
 
 namespace hstu {
@@ -130,18 +131,6 @@ __device__ __forceinline__ void for_each_step(const KParams& p, const SeqInfo& s
   }
 }
 
-// Bit e set <=> column j0 + e is visible to the row described by rb (columns j0 .. j0 + 31).
-__device__ __forceinline__ uint32_t low_bits(int n) {  // n lowest bits set, n clamped to [0, 32]
-  return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : ((1u << n) - 1u));
-}
-__device__ __forceinline__ uint32_t visible_bits(const RowBounds& rb, int j0) {
-  return low_bits(rb.lim1 - j0) | (low_bits(rb.hi2 + 1 - j0) & ~low_bits(rb.lo2 - j0));
-}
-__device__ __forceinline__ uint32_t visible_bits(const WinBounds& rb, int j0) {
-  return low_bits(rb.lim1 - j0) | (low_bits(rb.hi2 + 1 - j0) & ~low_bits(rb.lo2 - j0)) |
-         (low_bits(rb.hi3 + 1 - j0) & ~low_bits(rb.lo3 - j0));
-}
-
 // Two neighbouring elements, the part that needs the scores only (vector_score.h:175-197), on the packed f32x2 pipe:
 //   x = alpha (s + bias),  sg = sigmoid(x),  P = x sg scale,  f = scale alpha sg (1 + x - x sg)   (dS = dP f)
 // With h = x / 2 and th = tanh h:  sg = (1 + th) / 2,  P = scale (h + h th),  f = (scale alpha / 2) (1 + th) (1 + h - h th).
@@ -224,6 +213,8 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
   constexpr bool staged = kStaged;
   BwdBars* bars = reinterpret_cast<BwdBars*>(base_ptr + (2 + kRing1 + kRing2) * kTileBytes + (staged ? 2 * kTileM * 128 : 0));
   const BwdWaiter w{&bars->abort_flag, p.ws_header};
+  constexpr bool kTurns = kWin && std::is_same<T, __half>::value;   // (see KParams)
+  if (kTurns && second_turn_idle(p)) return;
 
   // The two passes do not depend on each other, only on the pre-pass before them.  The dK/dV pass is launched with
   // programmatic stream serialization behind the dQ pass, which lets it go at once: its CTAs take the SMs as the dQ
@@ -278,7 +269,7 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
   // its last q-tile; dK/dV pass: its first keys).
   const int heads = kDKV ? p.hk : p.hq;
   const uint32_t* list = p.items + (kDKV ? 2 * p.bwd_cap_q : 0);
-  uint32_t* counter = p.ws_header + (kDKV ? 3 : 2);
+  uint32_t* counter = p.ws_header + (kDKV ? 3 : 2) + (kTurns && p.turn == 2 ? 4 : 0);
   uint32_t cnt = 0;          // steps so far (every role counts them alike): barrier phases run on across tiles
   uint32_t tiles_done = 0;   // tiles so far: phase of a_full / acc_full
   // Tiles are drawn by the producer thread, which runs ahead of the other warps across tile boundaries: when it has
@@ -801,6 +792,8 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
     const long long tok = (kDKV ? s.k0 : s.q0) + mine;
     T* out2 = static_cast<T*>(kDKV ? bp.dk : bp.dq) + (tok * heads + head) * p.dqk + col0;
     T* out1 = kDKV ? static_cast<T*>(bp.dv) + (tok * heads + head) * p.dv + col0 : nullptr;
+    const bool store2 = mine_ok && !(kTurns && p.turn == 2 && col0 < p.dqk && stored_finite(out2));
+    const bool store1 = kDKV && mine_ok && !(kTurns && p.turn == 2 && col0 < p.dv && stored_finite(out1));
 #pragma unroll 1
     for (int ch = 0; ch < D / 64; ++ch) {
 #pragma unroll 1
@@ -815,11 +808,12 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
 #pragma unroll
           for (int e = 0; e < 32; ++e) acc[e] = 0u;   // nothing visible: zero gradient
         }
-        if (kWin && std::is_same<T, __half>::value) {   // (see KParams)
+        if (kTurns) {
+          if (ch == 0 && mine_ok && p.turn == 1) note_not_finite(p, acc[0]);
 #pragma unroll
           for (int e = 0; e < 32; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * p.out_scale);
         }
-        if (mine_ok) {
+        if (which == 0 ? store1 : store2) {
           uint4* dst = reinterpret_cast<uint4*>((which == 0 ? out1 : out2) + ch * 32);
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
@@ -853,7 +847,7 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
 }
 
 template <int D, typename T>
-cudaError_t launch_bwd_tc_t(const BwdParams& bp, int dtype, int num_sms, cudaStream_t stream) {
+cudaError_t launch_bwd_tc_t(BwdParams bp, int dtype, int num_sms, cudaStream_t stream) {
   const KParams& p = bp.f;
   CUtensorMap mq, mg, mk, mv;
   if (!make_tile_map(&mq, p.q, p.total_q, p.hq, p.dqk, dtype) ||
@@ -892,16 +886,19 @@ cudaError_t launch_bwd_tc_t(const BwdParams& bp, int dtype, int num_sms, cudaStr
     return bias_staged ? go(hstu_bwd_tc_kernel<D, T, kDKV, true, false>, BwdRings<D, true, kDKV>::kSmem)
                        : go(hstu_bwd_tc_kernel<D, T, kDKV, false, false>, BwdRings<D, false, kDKV>::kSmem);
   };
-  cudaError_t e = cudaSuccess;
   overlap = p.total_q > 0;   // (a dQ pass is launched in front of the dK/dV pass)
-  if (p.total_q > 0)
-    e = launch(std::false_type{}, static_cast<long long>(p.batch) * p.hq * ((p.maxq + kTileM - 1) / kTileM), mq, mg,
-               mk, mv);
-  if (e != cudaSuccess) return e;
-  if (p.total_k > 0)
-    e = launch(std::true_type{}, static_cast<long long>(p.batch) * p.hk * ((p.maxk + kTileN - 1) / kTileN), mk, mv,
-               mq, mg);
-  return e;
+  for (;;) {
+    cudaError_t e = cudaSuccess;
+    if (p.total_q > 0)
+      e = launch(std::false_type{}, static_cast<long long>(p.batch) * p.hq * ((p.maxq + kTileM - 1) / kTileM), mq, mg,
+                 mk, mv);
+    if (e != cudaSuccess) return e;
+    if (p.total_k > 0)
+      e = launch(std::true_type{}, static_cast<long long>(p.batch) * p.hk * ((p.maxk + kTileN - 1) / kTileN), mk, mv,
+                 mq, mg);
+    if (e != cudaSuccess || p.turn != 1) return e;
+    bp.f = second_turn(p);
+  }
 }
 
 }  // namespace

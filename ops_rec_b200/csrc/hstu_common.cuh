@@ -26,6 +26,9 @@ constexpr int kTileN = 128;
 //   [4]   uint32 number of work items
 //   [8]   uint32 work counter (forward kernel; backward dQ pass)
 //   [12]  uint32 work counter (backward dK/dV pass)
+//   [16]  uint32 number of work items of the backward's dK/dV pass
+//   [20]  uint32 not 0: a sum came out infinite or NaN (see KParams::turn)
+//   [24]  uint32 work counters of the second turn, as at [8] and [12]
 //   [256] uint32 items[2 * capacity]   {sequence, head << 16 | q_pair}
 constexpr uint64_t kWsHeaderBytes = 256;
 // Below this many work items (tiles) in a call - eight per SM of a B200 - a list is ordered by the items' step counts,
@@ -89,7 +92,20 @@ struct KParams {
   // hstu_paged_8bit: kv_cache holds 8-bit numbers (HSTU_HELD_*), with a scale per scale_block rows and head
   const float* kv_scale;      // [num_pages, 2, page_size / scale_block, hk], null for a cache in the call's type
   int held, scale_block;
+  // Where P and dS are formed without the scale (out_scale; fp16 on the tensor cores), they may be beyond fp16 although the scaled
+  // ones are not.  Such a call takes two turns: 1 notes in the header that sums came out infinite or NaN; 2 ends at once when none
+  // did, and otherwise forms them again with the scale inside P and dS and stores those the first turn left infinite or NaN.  0:
+  // one turn.  (16 sequences of 1024 - 4096 rows, fp16, window 512: forward and backward 856 -> 863 us; 8 of 20 - 200, forward
+  // 14.5 -> 15.1.)
+  int turn;
 };
+
+inline KParams second_turn(KParams p) {
+  p.turn = 2;
+  p.scale = p.out_scale;
+  p.out_scale = 1.0f;
+  return p;
+}
 
 // Backward call: the forward's parameters plus the gradient tensors.
 struct BwdParams {

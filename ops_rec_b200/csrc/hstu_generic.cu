@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(simt::kThreads) hstu_simt_fwd_kernel(const KPa
           float pv = simt::divide(x, 1.f + expf(-x)) * p.scale;
           if (p.mask_type == HSTU_MASK_CUSTOM)
             pv *= on ? to_f<T>(cmask[((static_cast<long long>(b) * p.hq + h) * p.maxq + i) * p.maxk + j]) : 0.f;
-          pv = on ? simt::rounded<T>(pv) : 0.f;
+          pv = on ? simt::rounded<simt::HeldIn<T, kWin>>(pv) : 0.f;
           Ps[(4 * ty + r) * ldp + tx + 16 * c] = pv;
         }
       simt::cp_async_wait<0>();   // V_t
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(GTHREADS) hstu_generic_kernel(const KParams p)
           const long long moff = ((static_cast<long long>(b) * p.hq + h) * p.maxq + i) * p.maxk + j;
           pv *= to_f<T>(cmask[moff]);
         }
-        pv = to_f<T>(from_f<T>(pv));
+        pv = simt::rounded<simt::HeldIn<T, kWin>>(pv);
       }
       Ps[(ty * GROWS + r) * GN + tx] = pv;
     }

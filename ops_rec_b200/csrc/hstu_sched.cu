@@ -152,6 +152,8 @@ __global__ void __launch_bounds__(kPreThreads) hstu_prepass_kernel(const KParams
       p.ws_header[0] = s_status;
       p.ws_header[2] = 0;   // work counters (forward; backward dQ pass)
       p.ws_header[3] = 0;   // (backward dK/dV pass)
+      p.ws_header[5] = 0;   // (see KParams::turn)
+      p.ws_header[6] = 0;
       p.ws_header[1] = build_items ? total : 0u;
     }
   }
@@ -335,6 +337,8 @@ __global__ void __launch_bounds__(kPreThreads) hstu_bwd_prepass_kernel(const KPa
         if (static_cast<long long>(total) > cap) total = static_cast<unsigned>(cap);
         p.ws_header[which ? 4 : 1] = total;
         p.ws_header[2 + which] = 0;   // the pass's work counter
+        p.ws_header[5] = 0;           // (see KParams::turn)
+        p.ws_header[6 + which] = 0;
       }
     }
     __syncthreads();

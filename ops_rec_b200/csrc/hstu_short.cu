@@ -28,6 +28,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "hstu_common.cuh"
 #include "hstu_tc_common.cuh"
 #include "ptx_sm100.cuh"
@@ -145,6 +147,8 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
   const Waiter w{&bars->abort_flag, p.ws_header};
   const int halves_qk = C::kHalves == 1 ? 1 : (p.dqk + 63) >> 6;
   const int halves_v = C::kHalves == 1 ? 1 : (p.dv + 63) >> 6;
+  constexpr bool kTurns = std::is_same<T, __half>::value && !kBias;   // (see KParams)
+  if (kTurns && second_turn_idle(p)) return;
 
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&tm_q);
@@ -201,7 +205,7 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
       // (inline: the compiler's form of a one-lane atomicAdd waits for the result at once)
       auto draw = [&] {
         uint32_t u;
-        asm volatile("atom.global.add.u32 %0, [%1], 1;" : "=r"(u) : "l"(&p.ws_header[2]) : "memory");
+        asm volatile("atom.global.add.u32 %0, [%1], 1;" : "=r"(u) : "l"(&p.ws_header[kTurns && p.turn == 2 ? 6 : 2]) : "memory");
         return u;
       };
       auto read_entry = [&](uint32_t u) {
@@ -545,17 +549,19 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
       if (stopped()) break;
       ++o_uses;
       ptx::tc_fence_after();
+      const bool store = row_ok && !(kTurns && p.turn == 2 && stored_finite(orow));
 #pragma unroll
       for (int ch = 0; ch < D / 32; ++ch) {
         if (ch * 32 >= p.dv) continue;
         uint32_t orr[32];
         ptx::tmem_ld32(t_s + kShColO + ch * 32, orr);
         ptx::tmem_wait_ld_dep(orr);
-        if (std::is_same<T, __half>::value) {   // (see KParams; elsewhere it is 1)
+        if (kTurns) {   // (elsewhere the scale behind the sums is 1)
+          if (ch == 0 && store && p.turn == 1) note_not_finite(p, orr[0]);
 #pragma unroll
           for (int e = 0; e < 32; ++e) orr[e] = __float_as_uint(__uint_as_float(orr[e]) * p.out_scale);
         }
-        if (row_ok) {
+        if (store) {
 #pragma unroll
           for (int q4 = 0; q4 < 4; ++q4) {
             uint4 u;
@@ -598,7 +604,9 @@ cudaError_t launch_inst(const KParams& p, const CUtensorMap& mq, const CUtensorM
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p, mq, mk, mv, mb, mc);
+  e = cudaLaunchKernelEx(&cfg, kern, p, mq, mk, mv, mb, mc);
+  if (e != cudaSuccess || p.turn != 1) return e;
+  return cudaLaunchKernelEx(&cfg, kern, second_turn(p), mq, mk, mv, mb, mc);
 }
 
 }  // namespace

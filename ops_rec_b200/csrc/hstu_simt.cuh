@@ -14,6 +14,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "hstu_common.cuh"
 
 namespace hstu {
@@ -32,6 +34,10 @@ template <> __device__ __forceinline__ float from_float<float>(float x) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 template <typename T> __device__ __forceinline__ float rounded(float x) { return to_float<T>(from_float<T>(x)); }
+// The type P and dS are rounded to: fp16 calls with a window take the scale behind the sums, so theirs may be beyond fp16 and
+// stay in 32 bits.
+template <typename T, bool kWin>
+using HeldIn = typename std::conditional<kWin && std::is_same<T, __half>::value, float, T>::type;
 
 // a / b for b >= 1 with the remainder correction of Markstein ("Computation of elementary functions on the IBM RISC
 // System/6000 processor", 1990).  r = (1 + d) / b with |d| <= 2^-23 (the documented error of rcp.approx), so q = a r is

@@ -125,6 +125,23 @@ __device__ __forceinline__ uint32_t visible_bits(const WinBounds& rb, int j0) {
          (low_bits(rb.hi3 + 1 - j0) & ~low_bits(rb.lo3 - j0));
 }
 
+// KParams::turn.  The start of a kernel that has two, for every thread of the grid: the first lets the second go, which takes
+// SMs as they become free, waits for the first one's mark and results, and leaves (true) if there is none.
+__device__ __forceinline__ bool second_turn_idle(const KParams& p) {
+  if (p.turn == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (p.turn != 2) return false;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  return *reinterpret_cast<volatile uint32_t*>(p.ws_header + 5) == 0;
+}
+// A P (dS) beyond fp16 is infinite, and its product with any row makes every column of a sum infinite or NaN: one column of a row
+// of sums tells whether the row has to be formed again, and what the first turn stored of it tells the second.
+__device__ __forceinline__ void note_not_finite(const KParams& p, uint32_t sum) {
+  if ((sum & 0x7fffffffu) >= 0x7f800000u) p.ws_header[5] = 1;
+}
+__device__ __forceinline__ bool stored_finite(const void* half) {
+  return (*static_cast<const uint16_t*>(half) & 0x7c00u) != 0x7c00u;
+}
+
 // Zeroes `pieces` 16-byte pieces from shared-memory address `first` on, in each of `boxes` regions `box_bytes` apart
 // (the rows of a V tile behind a sequence end); called by the 128 threads of a P/O group, `tid` = 0..127.
 __device__ __noinline__ void zero_v_rows(uint32_t first, int pieces, int tid, int boxes, int box_bytes) {
