@@ -607,6 +607,10 @@ int hstu_paged_8bit_fwd(const HstuPaged8Args* args, void* workspace, uint64_t wo
     const UnpackedPages unpacked = {pages, table};
     return jagged_fwd_impl(&pl.fwd, workspace, pl.fwd_bytes, stream_v, &p, &unpacked);
   }
+  // The kernels that take the scale behind the sums are those with a window (scale_behind): fp16 calls without one get one that holds
+  // every key.  (Pages of 24 rows, 4 heads of 64 / 128, us with the scale in P / behind: 64 users of 1000 - 4000 rows, 64 new 272 / 329,
+  // 443 / 438; 512 of 50 - 1000, 300 new 487 / 503, 878 / 871; 4 of 14000 - 20000, 1000 new 544 / 628, 637 / 717.)
+  if (pl.fwd.dtype == HSTU_DTYPE_FP16 && !p.window) set_window(&p, kMostWindow, 0);
   const cudaError_t e = hstu::launch_paged_gather(p, a->kv_cache, b->k, b->v, base + pl.fwd_bytes, base + pl.fwd_bytes + pl.stage_bytes,
                                                   pl.capacity, a->num_pages, a->num_page_ids, pl.fwd.dtype, stream);
   if (e != cudaSuccess) return fail(HSTU_E_CUDA, "gather launch: %s", cudaGetErrorString(e));

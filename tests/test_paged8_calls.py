@@ -1,0 +1,59 @@
+"""hstu_paged_8bit and hstu_cache_append: calls that the tests of values (tests/test_paged8.py) do not make."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+import ops_rec_b200 as ops_rec
+from oracle import hstu_window_oracle as WO
+from ops_rec_b200 import cabi
+from tests.test_paged8 import BF16, E4M3, FP16, FP32, INT8, MANY, TABLE, make, meta, on_gpu
+
+append_op = ops_rec.ascendc.attention.hstu_cache_append
+paged_op = ops_rec.ascendc.attention.hstu_paged_8bit
+
+
+def products(args, window, sink):
+    """(outputs in 64 bits, the sum of the squares of the products P v behind each)."""
+    off, off_k, po = (args[n].tolist() for n in ("seq_offset", "seq_offset_k", "page_offsets"))
+    out, square = (torch.zeros(args["q"].shape, dtype=torch.float64, device="cuda") for _ in range(2))
+    ratio = args["q"].shape[1] // args["k"].shape[1]
+    value = args["kv_cache"].double().unflatten(2, (args["kv_scale"].shape[2], -1)) * args["kv_scale"].double()[:, :, :, None, :, None]
+    value = value.flatten(2, 3)
+    for b in range(len(off) - 1):
+        t = int(args["num_target"][b]) if "num_target" in args else 0
+        n, rows = off_k[b + 1] - off_k[b], slice(off[b], off[b + 1])
+        mine = value[args["page_ids"][po[b]:po[b + 1]]].transpose(0, 1).flatten(1, 2)[:, :n - t]
+        k, v = (torch.cat((mine[w], args[x][off[b + 1] - t:off[b + 1]].double())).transpose(0, 1).repeat_interleave(ratio, 0)
+                for w, x in ((0, "k"), (1, "v")))
+        see = WO.window_mask(off[b + 1] - off[b], n, t, args.get("target_group_size", 0), window, sink, "cuda")
+        x = args["alpha"] * args["q"][rows].double().transpose(0, 1) @ k.transpose(1, 2)
+        p = torch.where(see, x * torch.sigmoid(x) * args["silu_scale"], 0.0)
+        out[rows], square[rows] = (p @ v).transpose(0, 1), (p ** 2 @ v ** 2).transpose(0, 1)
+    return out, square
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("users,new,targets,group,d,page", [
+    (4, 1, None, 1, 64, 64), (4, 20, 5, 1, 128, 64), (MANY, 40, None, 1, 64, 64),          # in place; unpacked
+    (4, 20, 5, 1, 64, 24), (4, 20, 9, 5, 128, 32), (4, 300, None, 1, 64, 32), (4, 7, 3, 1, 320, 16), (4, 9, 5, 2, 48, 20),   # staged
+])
+@pytest.mark.parametrize("window,sink", [(0, 0), (70, 4)])
+def test_half_precision_keeps_its_bits_under_a_small_scale(users, new, targets, group, d, page, window, sink):
+    """fp16 with a scale of 1 / 4096, whichever kernel a call goes to: P of the usual sizes times it would be below the type's normal
+    range.  A value rounded once is u x / sqrt(3) off at most in the mean square (u: half a step), so an output y = sum(P v) of
+    rounded P that is rounded itself u / sqrt(3) sqrt(sum((P v)^2) + y^2), and 2^-25 / sqrt(3) where it is subnormal; a tenth on top
+    for the sample and for what 32 bits add.  (The cache's values are numbers of 8 bits times powers of two: exact in fp16.)"""
+    rng = np.random.default_rng(61)
+    cached = rng.integers(new, 500, users) if users > 4 else np.array([new + 200, new, 640, new + 31])
+    args = make(cached, np.full(users, new), None if targets is None else np.full(users, targets), 4, 2, d, FP16, INT8, page, 4, seed=62)
+    args = on_gpu(args | dict(silu_scale=1 / 4096, v=args["v"] * 8, kv_scale=args["kv_scale"] * 8))
+    args["kv_scale"][:, 0] /= 8
+    if targets is not None:
+        args["target_group_size"] = group
+    out, st = cabi.hstu_paged_8bit_forward(**args, window=window, num_sink=sink, return_status=True)
+    want, square = products(args, window, sink)
+    off = (out.double() - want).square().mean().sqrt()
+    most = 1.1 * ((2.0 ** -22 * (square + want ** 2).mean() + 2.0 ** -50) / 3).sqrt()
+    assert st == 0 and off <= most, (off / most).item()
