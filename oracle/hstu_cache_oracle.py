@@ -66,8 +66,11 @@ def append(k, v, kv_cache, kv_scale, seq_offset, page_offsets, page_ids, last_pa
 
 def paged(q, k, v, kv_cache, kv_scale, max_seq_len, max_seq_len_k=0, silu_scale=0.0, seq_offset=None, seq_offset_k=None,
           page_offsets=None, page_ids=None, last_page_len=None, num_target=None, target_group_size=0, alpha=1.0, window=0,
-          num_sink=0, tanh=True):
-    """(value in 64 bits, tolerance)."""
+          num_sink=0, tanh=None):
+    """(value in 64 bits, tolerance).  tanh: whether SiLU may come from tanh.approx, by default where the framework's kernels take
+    that form - bf16, heads of 64 and 128."""
+    if tanh is None:
+        tanh = q.dtype == torch.bfloat16 and q.shape[2] in (64, 128)
     off, off_k, po, ids = (t.tolist() for t in (seq_offset, seq_offset_k, page_offsets, page_ids))
     page, per_page = kv_cache.shape[2], kv_scale.shape[2]
     out, tol = (torch.zeros(q.shape, dtype=torch.float64, device=q.device) for _ in range(2))

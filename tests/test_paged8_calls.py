@@ -57,3 +57,13 @@ def test_half_precision_keeps_its_bits_under_a_small_scale(users, new, targets, 
     off = (out.double() - want).square().mean().sqrt()
     most = 1.1 * ((2.0 ** -22 * (square + want ** 2).mean() + 2.0 ** -50) / 3).sqrt()
     assert st == 0 and off <= most, (off / most).item()
+
+
+def test_tolerance_follows_the_form_of_silu():
+    """CPU: the 2^-12 |x| of tanh.approx is allowed where a kernel takes that form - bf16, heads of 64 and 128 - and nowhere else."""
+    from oracle import hstu_cache_oracle as CO
+    for dtype, d, tanh in ((BF16, 64, True), (BF16, 128, True), (BF16, 96, False), (BF16, 256, False), (FP16, 64, False), (FP32, 64, False)):
+        args = make([40], [3], [2], 2, 1, d, dtype, E4M3, 32, 16, seed=63)
+        tight, loose = (CO.paged(**args, tanh=form)[1] for form in (False, True))
+        got = CO.paged(**args)[1]
+        assert (tight < loose).any() and torch.equal(got, loose if tanh else tight), (dtype, d)
