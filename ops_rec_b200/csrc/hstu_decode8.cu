@@ -34,7 +34,6 @@ namespace {
 constexpr int kDecWarps = 4, kDecThreads = 32 * kDecWarps;
 constexpr int kDecKeys = 16;      // keys of a tile
 constexpr int kPair = 2;          // tiles a warp works on at a time: their chains of dependent steps overlap
-constexpr int kDecMostTiles = 128;   // of a CTA
 
 template <int D> struct DecCfg {
   static constexpr int kRows = 8;                               // rows of a CTA
@@ -43,15 +42,15 @@ template <int D> struct DecCfg {
   static constexpr int kStage = kPair * 2 * kTile;
   static constexpr int kRing = kStages * kStage;
   static constexpr int kScales = kDecWarps * kStages * kPair * 2 * kDecKeys * 4;
-  static constexpr int kSmem = kDecWarps * kRing + kScales;
+  static constexpr int kSmem = kDecWarps * kRing + kScales;   // and 16 bytes per tile
   static_assert(kDecWarps * kRing >= kDecWarps * kRows * D * 4, "the rings hold the warps' partial outputs at the end");
 };
 
 struct DecParams {
   KParams f;
   uint32_t* counters;   // [batch * hk], of CTAs that have left their sums
-  float* partial;       // [batch * hk][splits][rows][D]
-  int splits, tiles, rows;   // CTAs along the keys, tiles of a CTA, rows of a partial sum
+  float* partial;       // [slots][hk][rows][D]
+  int splits, tiles, by_pages, rows;   // see Split; rows of a partial sum
   int block_shift;      // log2 of a scale's block, 4 at most (a tile has one scale from there on)
   // ceil(2^32 / n): x / n is the upper half of the product, exactly, while x n < 2^32 (a warp with 20 tiles to do feels a
   // handful of divisions)
@@ -65,14 +64,14 @@ __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
 template <int D, typename T, typename H, bool kWin, bool kTanh>
-__global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecParams d) {
+__global__ void __launch_bounds__(kDecThreads, D == 64 ? 5 : 3) hstu_decode8_kernel(const DecParams d) {
   using C = DecCfg<D>;
   using Mask = MaskOf<kWin>;
   constexpr bool kFine = std::is_same<T, __half>::value;
   const KParams& p = d.f;
   extern __shared__ __align__(128) uint8_t ring_of_all[];
-  __shared__ long long s_row[kDecMostTiles];     // where the tile's keys start in the cache, -1: no such page
-  __shared__ long long s_scale[kDecMostTiles];   // where its scales start
+  long long* const s_row = reinterpret_cast<long long*>(ring_of_all + C::kSmem);   // where a tile's keys start in the cache, -1: no such page
+  long long* const s_scale = s_row + d.tiles;                                      // where its scales start
   __shared__ int s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int b = over(blockIdx.x, d.by_hk), hk = blockIdx.x - b * p.hk, split = blockIdx.y;
@@ -88,6 +87,10 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   // CTAs that share the keys, evenly, in whole rounds of the four warps' pairs
   int active = 1;
   while (active * d.tiles < tiles.n) ++active;
+  if (active > 1) {
+    active = min(active, most_partials(p, d.by_pages, b, d.splits, d.tiles));
+    tiles.n = min(tiles.n, active * d.tiles);   // (more keys than pages: flagged)
+  }
   constexpr int kRound = kDecWarps * kPair;
   const int each = active == 1 ? d.tiles : (tiles.n + active * kRound - 1) / (active * kRound) * kRound;
   const int t0 = split * each, t1 = min(tiles.n, t0 + each);
@@ -312,6 +315,8 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
   }
   __syncthreads();
   const long long group = blockIdx.x;
+  const long long first = active > 1 ? first_partial(p, d.by_pages, b, d.splits, d.tiles) : 0;
+  auto partial_of = [&](int n) { return d.partial + ((first + n) * p.hk + hk) * d.rows * D; };
   auto store = [&](int r, int col, float4 v) {
     if (col >= p.dqk) return;
     const int i_row = over(r, d.by_ratio);
@@ -327,7 +332,7 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
       v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
     }
     if (active == 1) store(r, col, v);
-    else *reinterpret_cast<float4*>(d.partial + ((group * d.splits + split) * d.rows + r) * D + col) = v;
+    else *reinterpret_cast<float4*>(partial_of(split) + r * D + col) = v;
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the counters are cleared (and this grid ends after that one)
   if (active == 1) return;
@@ -342,7 +347,7 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int n = 0; n < active; ++n) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(d.partial + ((group * d.splits + n) * d.rows + r) * D + col));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(partial_of(n) + r * D + col));
       v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
     }
     store(r, col, v);
@@ -351,52 +356,28 @@ __global__ void __launch_bounds__(kDecThreads) hstu_decode8_kernel(const DecPara
 
 int tile_width(const KParams& p) { return p.dqk <= 64 ? 64 : 128; }
 
-// How a call is split: tiles of a CTA, CTAs along the keys.
-struct DecPlan {
-  int tiles, splits, rows;
-};
-DecPlan plan(const KParams& p) {
-  DecPlan d;
-  d.rows = p.maxq * p.gqa_ratio;
-  long long most = (p.maxk + kDecKeys - 1) / kDecKeys;   // tiles of the longest sequence
-  long long all = p.num_page_ids * p.page_size / kDecKeys;   // and of all of them together, at most
-  if (all < most) most = all;
-  if (p.window) {
-    const long long seen = (static_cast<long long>(p.window) + p.maxq) / kDecKeys + 2 + (p.sink + kDecKeys - 1) / kDecKeys;
-    if (seen < most) most = seen;
-    if (seen * p.batch < all) all = seen * p.batch;
-  }
-  // Some six CTAs per SM (three fit): fewer, and sequences of different lengths do not even out; more, and set-up and partial
-  // sums - a thousand instructions a warp, where a tile takes 300 - are what the SMs do.  Attention alone, us, at 4 / 6 / 8 /
-  // 12: 128 users of 200 - 2048 rows and 8 heads 64 / 66 / 70 / 75, 4 users of 14000 - 20000 44 / 39 / 45 / 50.
-  long long tiles = all * p.hk / (6ll * 148);
-  // Of a bound that is far above the lengths most CTAs find nothing to do: at most some 32 per SM (1000 users of 60 - 128 rows,
-  // one head, max_seq_len_k 128 / 20480: 14 / 21 us; without it 14 / 169).
-  const long long busy = most * p.batch * p.hk / (32ll * 148);
-  if (tiles < busy) tiles = busy;
-  tiles = tiles < 8 ? 8 : tiles > kDecMostTiles ? kDecMostTiles : tiles;
-  constexpr int kRound = kDecWarps * kPair;
-  d.tiles = static_cast<int>((tiles + kRound - 1) / kRound * kRound);
-  d.splits = static_cast<int>((most + d.tiles - 1) / d.tiles);
-  if (d.splits < 1) d.splits = 1;
-  return d;
-}
+// Some six CTAs per SM (three fit): fewer, and sequences of different lengths do not even out; more, and set-up and partial
+// sums - a thousand instructions a warp, where a tile takes 300 - are what the SMs do.  Attention alone, us, at 4 / 6 / 8 / 12: 128
+// users of 200 - 2048 rows and 8 heads 64 / 66 / 70 / 75, 4 users of 14000 - 20000 44 / 39 / 45 / 50.  With a loose bound of the
+// lengths (1000 users of 60 - 128 rows, max_seq_len_k 128 / 20480): one head 14.6 / 18.7 us, 8 heads 70 / 86.
+Split plan(const KParams& p) { return split_keys(p, 8, kDecWarps * kPair, 6 * 148, 1); }
 uint64_t counters_bytes(const KParams& p) {
   return (static_cast<uint64_t>(p.batch) * p.hk * 4 + 255) & ~static_cast<uint64_t>(255);
 }
 
 template <int D, typename T, typename H>
-cudaError_t launch_dec(const DecParams& d, const DecPlan& pl, cudaStream_t stream) {
+cudaError_t launch_dec(const DecParams& d, const Split& pl, cudaStream_t stream) {
   using C = DecCfg<D>;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   auto kern = kBf16 && tanh_silu(d.f) ? (d.f.window ? hstu_decode8_kernel<D, T, H, true, kBf16> : hstu_decode8_kernel<D, T, H, false, kBf16>)
                                       : (d.f.window ? hstu_decode8_kernel<D, T, H, true, false> : hstu_decode8_kernel<D, T, H, false, false>);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  const int smem = C::kSmem + 16 * pl.tiles;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(d.f.batch) * d.f.hk, pl.splits, 1);
   cfg.blockDim = dim3(kDecThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -417,13 +398,11 @@ bool decode8_supported(const KParams& p, int dtype) {
 }
 
 uint64_t decode8_workspace(const KParams& p) {
-  const DecPlan d = plan(p);
-  const uint64_t partial = d.splits > 1 ? static_cast<uint64_t>(p.batch) * p.hk * d.splits * d.rows * tile_width(p) * 4 : 0;
-  return kWsHeaderBytes + counters_bytes(p) + partial;
+  return kWsHeaderBytes + counters_bytes(p) + static_cast<uint64_t>(plan(p).slots) * p.hk * p.maxq * p.gqa_ratio * tile_width(p) * 4;
 }
 
 cudaError_t launch_decode8(const KParams& p, int dtype, void* workspace, cudaStream_t stream) {
-  const DecPlan pl = plan(p);
+  const Split pl = plan(p);
   DecParams d;
   d.f = p;
   d.f.ws_header = static_cast<uint32_t*>(workspace);
@@ -432,7 +411,8 @@ cudaError_t launch_decode8(const KParams& p, int dtype, void* workspace, cudaStr
   d.partial = reinterpret_cast<float*>(base + counters_bytes(p));
   d.splits = pl.splits;
   d.tiles = pl.tiles;
-  d.rows = pl.rows;
+  d.by_pages = pl.by_pages;
+  d.rows = p.maxq * p.gqa_ratio;
   // (at most 2^20 heads of sequences by 16, 8 rows by 8, 20480 keys by a page of any size)
   d.by_hk = inverse_of(p.hk);
   d.by_ratio = inverse_of(p.gqa_ratio);

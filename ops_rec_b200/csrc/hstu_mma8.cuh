@@ -112,6 +112,55 @@ template <int kThreads> __device__ __forceinline__ void report_sequence(const KP
   }
 }
 
+// Where the CTAs that share a sequence's keys leave their partial sums, and how many of them may: in slots of one CTA per key head
+// and block of rows.  Either every sequence has `splits` slots, or - many sequences, few of them long - sequence b has the slots
+// [2 f(b), 2 f(b + 1)) with f(b) = the tiles in front of its pages / tiles of a CTA, rounded down: whoever needs n > 1 CTAs has
+// pages of more than n - 1 times a CTA's tiles, so f grows by n - 1 at least.
+__device__ __forceinline__ long long tiles_before(const KParams& p, int b, int tiles) {
+  const long long pg = load_index(p.page_offsets, p.index_bytes, b);
+  return min(max(pg, 0ll), p.num_page_ids) * (p.page_size / 16) / tiles;
+}
+__device__ __forceinline__ long long first_partial(const KParams& p, bool by_pages, int b, int splits, int tiles) {
+  return by_pages ? 2 * tiles_before(p, b, tiles) : static_cast<long long>(b) * splits;
+}
+__device__ __forceinline__ int most_partials(const KParams& p, bool by_pages, int b, int splits, int tiles) {
+  return by_pages ? static_cast<int>(min(max(2 * (tiles_before(p, b + 1, tiles) - tiles_before(p, b, tiles)), 1ll), static_cast<long long>(splits))) : splits;
+}
+
+// How a call is split: tiles of 16 keys of a CTA, CTAs along the keys of a sequence, slots of partial sums.
+struct Split {
+  int tiles, splits, by_pages;
+  long long slots;
+};
+// least: of a CTA's tiles; ctas: of the whole GPU, that fill it evenly; blocks: of rows.
+inline Split split_keys(const KParams& p, int least, int step, long long ctas, int blocks) {
+  long long most = (p.maxk + 15) / 16;                              // tiles of the longest sequence
+  const long long pages = p.num_page_ids * (p.page_size / 16);      // and of all of them together, at most
+  long long all = pages;
+  if (all < most) most = all;
+  if (p.window) {
+    const long long seen = (static_cast<long long>(p.window) + p.maxq) / 16 + 2 + (p.sink + 15) / 16;
+    if (seen < most) most = seen;
+    if (seen * p.batch < all) all = seen * p.batch;
+  }
+  const long long heads = static_cast<long long>(p.hk) * blocks;
+  long long tiles = all * heads / ctas;
+  // Where the bound of the lengths is far above most of them, most CTAs find nothing to do, which costs as much as two tiles: at
+  // most some 32 per SM and one for 8 tiles that there are, beside the one that each problem has.
+  const long long busy = most * p.batch * heads / (32ll * 148 + all * heads / 8);
+  if (tiles < busy) tiles = busy;
+  if (tiles < least) tiles = least;
+  if (tiles > most) tiles = most > least ? most : least;
+  Split s;
+  s.tiles = static_cast<int>((tiles + step - 1) / step * step);
+  s.splits = static_cast<int>((most + s.tiles - 1) / s.tiles);
+  if (s.splits < 1) s.splits = 1;
+  const long long by_pages = 2 * (pages / s.tiles) + 2, each = static_cast<long long>(p.batch) * s.splits;
+  s.by_pages = by_pages < each ? 1 : 0;
+  s.slots = s.splits > 1 ? (s.by_pages ? by_pages : each) : 0;
+  return s;
+}
+
 // Eight query rows as the B operands of S^T = K.Q^T: a bf16 row is divided by a power of two (its largest element to [1, 2)).
 // Returns alpha times that power.  w: this thread's pairs of one row; the four threads of a lane group hold the rest of it.
 template <typename T, int kPairs> __device__ __forceinline__ float to_fp16_row(uint32_t (&w)[kPairs], float alpha) {

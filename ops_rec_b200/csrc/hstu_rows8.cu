@@ -14,6 +14,8 @@
 //        on pairs of scores (tanh on two halves at once is no faster, and 1 + tanh from halves is 2^-12 off where it is small)
 // Targets see the cached keys as a row right behind the history would; what they see of each other - their own group, up to
 // themselves - is added at the end in 32 bits (groups of up to four; with one target per group a row's own key and value).
+#include <algorithm>
+
 #include "hstu_mma8.cuh"
 
 namespace hstu {
@@ -23,7 +25,6 @@ namespace {
 constexpr int kRwKeys = 16;        // keys of a tile
 constexpr int kRwStage = 32;       // keys of a stage: two tiles
 constexpr int kRwRows = 64;        // of a CTA
-constexpr int kRwMostTiles = 128;  // of a CTA
 constexpr int kRwMostGroup = 4;    // targets of a group
 constexpr int kRwMostRows = 256;   // of a sequence and key head
 
@@ -35,14 +36,14 @@ template <int D> struct RwCfg {
   static constexpr int kDepth = 4;                     // stages of the ring of raw numbers
   static constexpr int kRaw = kRwStage * D * 2;        // bytes of a stage: K and V
   static constexpr int kBuffers = 4 * kTile > kOut ? 4 * kTile : kOut;
-  static constexpr int kSmem = kBuffers + kDepth * (kRaw + 2 * kRwStage * 4);
+  static constexpr int kSmem = kBuffers + kDepth * (kRaw + 2 * kRwStage * 4);   // and 16 bytes per tile
 };
 
 struct RwParams {
   KParams f;
   uint32_t* counters;   // [batch * hk * row blocks], of CTAs that have left their sums
-  float* partial;       // [batch * hk * row blocks][splits][rows][D]
-  int splits, tiles, rows;
+  float* partial;       // [slots][hk][row blocks][rows][D]
+  int splits, tiles, by_pages, rows;   // see Split; rows of a partial sum
   int block_shift;      // log2 of a scale's block, 4 at most
   uint32_t by_hk, by_ratio, by_page, by_block, by_group;   // over()
 };
@@ -70,8 +71,8 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
   constexpr bool kFine = std::is_same<T, __half>::value;
   const KParams& p = d.f;
   extern __shared__ __align__(256) uint8_t smem[];   // [2][K, V][32][D] halves; at the end the output
-  __shared__ long long s_row[kRwMostTiles];          // where the tile's keys start in the cache, -1: no such page
-  __shared__ long long s_scale[kRwMostTiles];        // and its scales
+  long long* const s_row = reinterpret_cast<long long*>(smem + C::kSmem);   // where the tile's keys start in the cache, -1: no such page
+  long long* const s_scale = s_row + d.tiles;                               // and its scales
   __shared__ float s_factor[2][2][kRwStage];         // scales of a stage's keys and values
   __shared__ float s_own[kRwRows][kRwMostGroup];     // SiLU of a target's scores with its group
   __shared__ int s_last;
@@ -98,6 +99,10 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
   // CTAs that share this block's keys, evenly, in whole stages
   int active = 1;
   while (active * d.tiles < tiles.n) ++active;
+  if (active > 1) {
+    active = min(active, most_partials(p, d.by_pages, b, d.splits, d.tiles));
+    tiles.n = min(tiles.n, active * d.tiles);   // (more keys than pages: flagged)
+  }
   const int each = active == 1 ? d.tiles : (tiles.n + 2 * active - 1) / (2 * active) * 2;
   const int t0 = split * each, nt = min(tiles.n - t0, each);   // first tile, number of tiles
   if (rows <= 0 || split >= active) {   // uniform over the CTA
@@ -366,6 +371,8 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
   }
   __syncthreads();
   const long long group = static_cast<long long>(blockIdx.x) * gridDim.z + blockIdx.z;
+  const long long first = active > 1 ? first_partial(p, d.by_pages, b, d.splits, d.tiles) : 0;
+  auto partial_of = [&](int n) { return d.partial + (((first + n) * p.hk + hk) * gridDim.z + blockIdx.z) * d.rows * D; };
   auto store = [&](int r, int col, float4 v) {
     if (col >= p.dqk) return;
     const int row = r_first + r, i_row = over(row, d.by_ratio);
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
       const int i = i0 + f * kRwThreads, r = i / (D / 4), col = i % (D / 4) * 4;
       if (i >= rows * (D / 4)) continue;
       if (active == 1) store(r, col, v[f]);
-      else *reinterpret_cast<float4*>(d.partial + ((group * d.splits + split) * d.rows + r) * D + col) = v[f];
+      else *reinterpret_cast<float4*>(partial_of(split) + r * D + col) = v[f];
     }
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the counters are cleared (and this grid ends after that one)
@@ -424,7 +431,7 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int n = 0; n < active; ++n) {
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(d.partial + ((group * d.splits + n) * d.rows + r) * D + col));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(partial_of(n) + r * D + col));
       v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
     }
     store(r, col, v);
@@ -433,51 +440,28 @@ __global__ void __launch_bounds__(RwCfg<D>::kThreads) hstu_rows8_kernel(const Rw
 
 int tile_width(const KParams& p) { return p.dqk <= 64 ? 64 : 128; }
 
-// How a call is split: tiles of a CTA, CTAs along the keys, blocks of rows.
-struct RwPlan {
-  int tiles, splits, row_blocks, rows;
-};
-RwPlan plan(const KParams& p) {
-  RwPlan d;
-  const int rows = p.maxq * p.gqa_ratio;
-  d.row_blocks = (rows + kRwRows - 1) / kRwRows;
-  d.rows = rows < kRwRows ? rows : kRwRows;
-  long long most = (p.maxk + kRwKeys - 1) / kRwKeys;         // tiles of the longest sequence
-  long long all = p.num_page_ids * p.page_size / kRwKeys;    // and of all of them together, at most
-  if (all < most) most = all;
-  if (p.window) {
-    const long long seen = (static_cast<long long>(p.window) + p.maxq) / kRwKeys + 2 + (p.sink + kRwKeys - 1) / kRwKeys;
-    if (seen < most) most = seen;
-    if (seen * p.batch < all) all = seen * p.batch;
-  }
-  // some eight CTAs per SM, of at least 16 tiles: less is mostly set-up
-  long long tiles = all * p.hk * d.row_blocks / (8ll * 148);
-  // Of a bound that is far above the lengths most CTAs find nothing to do: at most some 32 per SM (1000 users of 60 - 128 rows,
-  // one head, 9 rows and 20 targets, max_seq_len_k 148 / 20480: 35 / 45 us; without it 35 / 166).
-  const long long busy = most * p.batch * p.hk * d.row_blocks / (32ll * 148);
-  if (tiles < busy) tiles = busy;
-  tiles = tiles < 16 ? 16 : tiles > kRwMostTiles ? kRwMostTiles : tiles;
-  d.tiles = static_cast<int>((tiles + 1) / 2 * 2);
-  d.splits = static_cast<int>((most + d.tiles - 1) / d.tiles);
-  if (d.splits < 1) d.splits = 1;
-  return d;
-}
-uint64_t counters_bytes(const KParams& p, const RwPlan& d) {
-  return (static_cast<uint64_t>(p.batch) * p.hk * d.row_blocks * 4 + 255) & ~static_cast<uint64_t>(255);
+int rows_of(const KParams& p) { return p.maxq * p.gqa_ratio; }
+int row_blocks(const KParams& p) { return (rows_of(p) + kRwRows - 1) / kRwRows; }
+// Some eight CTAs per SM, of at least 16 tiles: less is mostly set-up.  (A loose bound of the lengths - 1000 users of 60 - 128 rows, one
+// head, 9 rows and 20 targets, max_seq_len_k 148 / 20480: 35 / 39 us.)
+Split plan(const KParams& p) { return split_keys(p, 16, 2, 8 * 148, row_blocks(p)); }
+uint64_t counters_bytes(const KParams& p) {
+  return (static_cast<uint64_t>(p.batch) * p.hk * row_blocks(p) * 4 + 255) & ~static_cast<uint64_t>(255);
 }
 
 template <int D, typename T, typename H>
-cudaError_t launch_rows(const RwParams& d, const RwPlan& pl, cudaStream_t stream) {
+cudaError_t launch_rows(const RwParams& d, const Split& pl, cudaStream_t stream) {
   using C = RwCfg<D>;
   constexpr bool kBf16 = !std::is_same<T, __half>::value;
   auto kern = kBf16 && tanh_silu(d.f) ? (d.f.window ? hstu_rows8_kernel<D, T, H, true, kBf16> : hstu_rows8_kernel<D, T, H, false, kBf16>)
                                       : (d.f.window ? hstu_rows8_kernel<D, T, H, true, false> : hstu_rows8_kernel<D, T, H, false, false>);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  const int smem = C::kSmem + 16 * pl.tiles;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(d.f.batch) * d.f.hk, pl.splits, pl.row_blocks);
+  cfg.gridDim = dim3(static_cast<unsigned>(d.f.batch) * d.f.hk, pl.splits, row_blocks(d.f));
   cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -500,22 +484,22 @@ bool rows8_supported(const KParams& p, int dtype) {
 }
 
 uint64_t rows8_workspace(const KParams& p) {
-  const RwPlan d = plan(p);
-  const uint64_t partial = d.splits > 1 ? static_cast<uint64_t>(p.batch) * p.hk * d.row_blocks * d.splits * d.rows * tile_width(p) * 4 : 0;
-  return kWsHeaderBytes + counters_bytes(p, d) + partial;
+  const uint64_t slot = static_cast<uint64_t>(p.hk) * row_blocks(p) * std::min(rows_of(p), kRwRows) * tile_width(p) * 4;
+  return kWsHeaderBytes + counters_bytes(p) + plan(p).slots * slot;
 }
 
 cudaError_t launch_rows8(const KParams& p, int dtype, void* workspace, cudaStream_t stream) {
-  const RwPlan pl = plan(p);
+  const Split pl = plan(p);
   RwParams d;
   d.f = p;
   d.f.ws_header = static_cast<uint32_t*>(workspace);
   char* base = static_cast<char*>(workspace) + kWsHeaderBytes;
   d.counters = reinterpret_cast<uint32_t*>(base);
-  d.partial = reinterpret_cast<float*>(base + counters_bytes(p, pl));
+  d.partial = reinterpret_cast<float*>(base + counters_bytes(p));
   d.splits = pl.splits;
   d.tiles = pl.tiles;
-  d.rows = pl.rows;
+  d.by_pages = pl.by_pages;
+  d.rows = std::min(rows_of(p), kRwRows);
   // (at most 2^20 heads of sequences by 16, 256 rows by 16, 20480 keys by a page of any size, 256 targets by 4)
   d.by_hk = inverse_of(p.hk);
   d.by_ratio = inverse_of(p.gqa_ratio);
@@ -524,7 +508,7 @@ cudaError_t launch_rows8(const KParams& p, int dtype, void* workspace, cudaStrea
   d.by_group = inverse_of(p.group > 0 ? p.group : 1);
   d.block_shift = 4;
   while (d.block_shift > 0 && (1 << d.block_shift) > p.scale_block) --d.block_shift;
-  const long long n = pl.splits > 1 ? static_cast<long long>(p.batch) * p.hk * pl.row_blocks : 0;
+  const long long n = pl.splits > 1 ? static_cast<long long>(p.batch) * p.hk * row_blocks(p) : 0;
   clear_kernel<<<static_cast<unsigned>(n / 256 + 1), 256, 0, stream>>>(d.f.ws_header, d.counters, n);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || p.total_q == 0) return e;

@@ -67,3 +67,68 @@ def test_tolerance_follows_the_form_of_silu():
         tight, loose = (CO.paged(**args, tanh=form)[1] for form in (False, True))
         got = CO.paged(**args)[1]
         assert (tight < loose).any() and torch.equal(got, loose if tanh else tight), (dtype, d)
+
+
+def workspace_size(batch, rows, hq, hk, d, max_seq_len_k, pages, page=32, window=0, dtype=0):
+    """What a call of `rows` query rows of each user asks for (addresses that are not read)."""
+    lib, at, n = cabi.load(), 0x7F0000000000, C.c_uint64()
+    base = cabi.HstuJaggedArgs()
+    base.struct_bytes, base.dtype, base.q, base.k, base.v, base.out = C.sizeof(base), dtype, at, at, at, at
+    base.seq_offset_q, base.seq_offset_k, base.index_bytes, base.batch = at, at, 8, batch
+    base.total_q = base.total_k = batch * rows
+    base.heads_q, base.heads_k, base.dim_qk, base.dim_v = hq, hk, d, d
+    base.max_seq_len_q, base.max_seq_len_k, base.alpha = rows, max_seq_len_k, 1.0
+    p = cabi.HstuPagedArgs(C.sizeof(cabi.HstuPagedArgs), page, base, at, at, at, at, None, pages, pages)
+    a = cabi.HstuPaged8Args(C.sizeof(cabi.HstuPaged8Args), 0, 16, window, 0, 0, at, p)
+    cabi.check(lib.hstu_paged_8bit_fwd_get_workspace_size(C.byref(a), C.byref(n)))
+    return n.value
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 80, 200])
+@pytest.mark.parametrize("users,pages", [(4096, 16), (2048, 16), (300, 200), (4700, 2), (65535, 1), (1, 640), (40, 10)])
+@pytest.mark.parametrize("max_seq_len_k", [512, 2128, 20480])
+@pytest.mark.parametrize("window", [0, 1000])
+def test_workspace_follows_what_can_be_split(rows, users, pages, max_seq_len_k, window):
+    """Partial sums are of some 1200 CTAs' shares of the pages (8 of each of 148 SMs), twice that at most, and one share more per
+    head - whatever the bound of the lengths: of 64 rows of 128 numbers in 32 bits, 32 KB each; and a counter per problem."""
+    size = workspace_size(users, rows, 8, 8, 128, max_seq_len_k, users * pages, window=window)
+    blocks = (rows + 63) // 64
+    assert size <= (2 * 8 * 148 + 2 * 8 * blocks) * 64 * 128 * 4 + 4 * users * 8 * blocks + 4096
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new,targets,hq", [(1, None, 16), (9, None, 16), (3, 4, 16)])
+@pytest.mark.parametrize("dtype,held", [(BF16, E4M3), (FP16, INT8)])
+@pytest.mark.parametrize("window,sink", [(0, 0), (9000, 70)])
+def test_a_few_long_histories_among_many(new, targets, hq, dtype, held, window, sink):
+    """CTAs of more than 200 tiles, several for some of the users, whose partial sums lie in slots that go by their pages."""
+    rng = np.random.default_rng(64)
+    cached = np.maximum(rng.integers(1, 100, 600), new)
+    cached[[0, 77, 300, 301, 599]] = 20000, 15001, 8192, 20001, 12345
+    args = make(cached, np.full(600, new), None if targets is None else np.full(600, targets), hq, hq, 32, dtype, held, 64, 32, seed=65)
+    from tests.test_paged8 import check_paged
+    a = check_paged(args, window, sink)
+    cu = on_gpu(args | dict(max_seq_len_k=20480))
+    for _ in range(3):
+        out = cabi.hstu_paged_8bit_forward(**cu, window=window, num_sink=sink, workspace_fill=0xFF)
+        assert torch.equal(out, cabi.hstu_paged_8bit_forward(**cu, window=window, num_sink=sink))
+    assert (out.double() - a.double()).abs().max() <= 2.0 ** -7 * a.double().abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 9])
+def test_pages_that_do_not_hold_a_long_history_are_flagged(new):
+    """A table with fewer pages than the lengths say, where CTAs share a history and their slots go by the pages."""
+    cached = np.full(600, 40)
+    cached[[3, 500]] = 20000, 16000
+    args = make(cached, np.full(600, new), None, 16, 16, 32, page=64, block=32, seed=66)
+    good, st = cabi.hstu_paged_8bit_forward(**on_gpu(args), return_status=True)
+    assert st == 0
+    po = args["page_offsets"].clone()
+    po[501:] -= 200                                  # user 500 lacks 200 pages; the users behind it read what is not theirs
+    out, st = cabi.hstu_paged_8bit_forward(**on_gpu(args | dict(page_offsets=po)), return_status=True)
+    assert st & cabi.ST_BAD_PAGES and torch.equal(out[:500 * new], good[:500 * new])
+    po = args["page_offsets"].clone()
+    po[4:] = torch.where(po[4:] > po[3] + 2, po[3] + 2, po[4:])
+    out, st = cabi.hstu_paged_8bit_forward(**on_gpu(args | dict(page_offsets=po)), return_status=True)
+    assert st & cabi.ST_BAD_PAGES and torch.equal(out[:3 * new], good[:3 * new])
