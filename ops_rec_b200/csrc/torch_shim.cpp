@@ -997,6 +997,38 @@ at::Tensor hstu_paged_8bit_meta(const at::Tensor& q, const at::Tensor& k, const 
   return meta_out(q, v);
 }
 
+// A cache has no graph, so the attention over it has no gradients: a backward pass through it says so instead of leaving them out.
+struct HstuPaged8Function : public torch::autograd::Function<HstuPaged8Function> {
+  static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& kv_cache, const at::Tensor& kv_scale, int64_t max_seq_len, int64_t max_seq_len_k,
+                            double silu_scale, const OptTensor& seq_offset, const OptTensor& seq_offset_k,
+                            const OptTensor& page_offsets, const OptTensor& page_ids, const OptTensor& last_page_len,
+                            const OptTensor& num_target, OptInt group, OptDouble alpha, int64_t window, int64_t num_sink,
+                            bool deterministic) {
+    at::AutoDispatchBelowAutograd guard;
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("ops_rec::hstu_paged_8bit", "").typed<decltype(hstu_paged_8bit)>();
+    return op.call(q, k, v, kv_cache, kv_scale, max_seq_len, max_seq_len_k, silu_scale, seq_offset, seq_offset_k, page_offsets,
+                   page_ids, last_page_len, num_target, group, alpha, window, num_sink, deterministic);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "hstu_paged_8bit has no gradients: train with hstu_window or hstu_jagged");
+  }
+};
+
+at::Tensor hstu_paged_8bit_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& kv_cache,
+                                    const at::Tensor& kv_scale, int64_t max_seq_len, int64_t max_seq_len_k, double silu_scale,
+                                    const OptTensor& seq_offset, const OptTensor& seq_offset_k, const OptTensor& page_offsets,
+                                    const OptTensor& page_ids, const OptTensor& last_page_len, const OptTensor& num_target,
+                                    OptInt group, OptDouble alpha, int64_t window, int64_t num_sink, bool deterministic) {
+  const bool wanted = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || kv_scale.requires_grad());
+  if (wanted)
+    return HstuPaged8Function::apply(q, k, v, kv_cache, kv_scale, max_seq_len, max_seq_len_k, silu_scale, seq_offset, seq_offset_k,
+                                     page_offsets, page_ids, last_page_len, num_target, group, alpha, window, num_sink, deterministic);
+  return HstuPaged8Function::forward(nullptr, q, k, v, kv_cache, kv_scale, max_seq_len, max_seq_len_k, silu_scale, seq_offset,
+                                     seq_offset_k, page_offsets, page_ids, last_page_len, num_target, group, alpha, window, num_sink,
+                                     deterministic);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(ops_rec, m) {
@@ -1064,6 +1096,7 @@ TORCH_LIBRARY_IMPL(ops_rec, Autograd, m) {
   m.impl("hstu_jagged.equal", TORCH_FN(hstu_jagged_equal_autograd));
   m.impl("hstu_jagged.delta", TORCH_FN(hstu_jagged_delta_autograd));
   m.impl("hstu_window", TORCH_FN(hstu_window_autograd));
+  m.impl("hstu_paged_8bit", TORCH_FN(hstu_paged_8bit_autograd));
 }
 
 TORCH_LIBRARY_IMPL(ops_rec, Meta, m) {

@@ -132,3 +132,35 @@ def test_pages_that_do_not_hold_a_long_history_are_flagged(new):
     po[4:] = torch.where(po[4:] > po[3] + 2, po[3] + 2, po[4:])
     out, st = cabi.hstu_paged_8bit_forward(**on_gpu(args | dict(page_offsets=po)), return_status=True)
     assert st & cabi.ST_BAD_PAGES and torch.equal(out[:3 * new], good[:3 * new])
+
+
+def _meta_call(**grads):
+    i = lambda n: meta(n, dtype=torch.int64)   # noqa: E731
+    t = dict(q=meta(10, 4, 64), k=meta(10, 2, 64), v=meta(10, 2, 64), kv_cache=meta(6, 2, 32, 2, 64, dtype=E4M3), kv_scale=meta(6, 2, 2, 2, dtype=FP32))
+    for n in grads:
+        t[n].requires_grad_()
+    return t, paged_op(**t, max_seq_len=8, max_seq_len_k=32, seq_offset=i(3), seq_offset_k=i(3), page_offsets=i(3), page_ids=i(6),
+                       last_page_len=i(2))
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "kv_scale"])
+def test_paged_refuses_a_backward_pass(name):
+    """The output of queries that require gradients can be had; gradients through it cannot, and are not left out in silence."""
+    t, out = _meta_call(**{name: True})
+    assert out.requires_grad
+    with pytest.raises(RuntimeError, match="hstu_paged_8bit has no gradients"):
+        out.sum().backward()
+    with torch.no_grad():
+        assert not _meta_call(**{name: True})[1].requires_grad
+    assert not _meta_call()[1].requires_grad
+
+
+@pytest.mark.gpu
+def test_paged_of_queries_that_require_gradients():
+    args = on_gpu(make([60, 45], [1, 3], None, seed=67))
+    want = paged_op(**{n: args[n] for n in ("q", *TABLE)}, **{n: args[n] for n in ("max_seq_len", "max_seq_len_k", "seq_offset_k", "alpha")})
+    args["q"].requires_grad_()
+    out = paged_op(**{n: args[n] for n in ("q", *TABLE)}, **{n: args[n] for n in ("max_seq_len", "max_seq_len_k", "seq_offset_k", "alpha")})
+    assert torch.equal(out, want)
+    with pytest.raises(RuntimeError, match="has no gradients"):
+        (out.float().sum() + args["q"].float().sum()).backward()
