@@ -869,7 +869,7 @@ void check_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& kv
   check_held(kv_cache, kv_scale, k);
   // (they are written where they lie)
   TORCH_CHECK(kv_cache.is_contiguous() && kv_scale.is_contiguous(), "kv_cache and kv_scale must be contiguous");
-  TORCH_CHECK(!(k.requires_grad() || v.requires_grad()) || !at::GradMode::is_enabled(),
+  TORCH_CHECK(!(k.requires_grad() || v.requires_grad() || kv_cache.requires_grad() || kv_scale.requires_grad()) || !at::GradMode::is_enabled(),
               "hstu_cache_append: a cache has no gradients (call it under torch.no_grad())");
 }
 
@@ -997,6 +997,20 @@ at::Tensor hstu_paged_8bit_meta(const at::Tensor& q, const at::Tensor& k, const 
   return meta_out(q, v);
 }
 
+// What is written in place counts up its version, as with any operator: a graph that saved the cache or its scales finds out.
+// (Tensors of inference mode have none.)
+void hstu_cache_append_in_place(const at::Tensor& k, const at::Tensor& v, at::Tensor& kv_cache, at::Tensor& kv_scale,
+                                const at::Tensor& seq_offset, const at::Tensor& page_offsets, const at::Tensor& page_ids,
+                                const at::Tensor& last_page_len, const OptTensor& num_target) {
+  {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("ops_rec::hstu_cache_append", "").typed<decltype(hstu_cache_append_op)>();
+    op.call(k, v, kv_cache, kv_scale, seq_offset, page_offsets, page_ids, last_page_len, num_target);
+  }
+  for (at::Tensor* t : {&kv_cache, &kv_scale})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // A cache has no graph, so the attention over it has no gradients: a backward pass through it says so instead of leaving them out.
 struct HstuPaged8Function : public torch::autograd::Function<HstuPaged8Function> {
   static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -1097,6 +1111,10 @@ TORCH_LIBRARY_IMPL(ops_rec, Autograd, m) {
   m.impl("hstu_jagged.delta", TORCH_FN(hstu_jagged_delta_autograd));
   m.impl("hstu_window", TORCH_FN(hstu_window_autograd));
   m.impl("hstu_paged_8bit", TORCH_FN(hstu_paged_8bit_autograd));
+}
+
+TORCH_LIBRARY_IMPL(ops_rec, ADInplaceOrView, m) {
+  m.impl("hstu_cache_append", TORCH_FN(hstu_cache_append_in_place));
 }
 
 TORCH_LIBRARY_IMPL(ops_rec, Meta, m) {

@@ -164,3 +164,30 @@ def test_paged_of_queries_that_require_gradients():
     assert torch.equal(out, want)
     with pytest.raises(RuntimeError, match="has no gradients"):
         (out.float().sum() + args["q"].float().sum()).backward()
+
+
+def _meta_append(**change):
+    i = lambda n: meta(n, dtype=torch.int64)   # noqa: E731
+    t = dict(k=meta(10, 2, 64), v=meta(10, 2, 64), kv_cache=meta(6, 2, 32, 2, 64, dtype=E4M3), kv_scale=meta(6, 2, 2, 2, dtype=FP32),
+             seq_offset=i(3), page_offsets=i(3), page_ids=i(6), last_page_len=i(2)) | change
+    append_op(**t)
+    return t
+
+
+def test_append_counts_up_the_versions_of_what_it_writes():
+    t = _meta_append()
+    assert [t[n]._version for n in ("kv_cache", "kv_scale", "k", "v", "page_ids")] == [1, 1, 0, 0, 0]
+    with torch.no_grad():
+        append_op(**t)
+    assert t["kv_cache"]._version == 2 and t["kv_scale"]._version == 2
+    # a graph that saved the scales finds out
+    leaf = meta(6, 2, 2, 2, dtype=FP32).requires_grad_()
+    product = leaf * t["kv_scale"]
+    append_op(**t)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        t = _meta_append()
+    _meta_append(kv_cache=t["kv_cache"], kv_scale=t["kv_scale"])   # (tensors of inference mode have no version)
+    with pytest.raises(RuntimeError, match="no gradients"):
+        _meta_append(kv_scale=meta(6, 2, 2, 2, dtype=FP32).requires_grad_())
