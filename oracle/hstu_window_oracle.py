@@ -59,7 +59,7 @@ def attention(q, k, v, see, alpha, scale, dtype, grad=None, tanh=False, staged=F
         xerr = xerr + (u + f32) * abs(alpha) * (q.abs() @ kk.abs().transpose(1, 2)) + tiny * abs(alpha) * q.abs().sum(2, keepdim=True)
     sg = torch.sigmoid(x)
     approx = x.abs() * 2.0 ** -12 if tanh else (x * sg).abs() * 2.0 ** -20
-    perr = torch.where(see, scale * (1.1 * (xerr + approx) + (u + 4 * f32) * (x * sg).abs()) + step, 0.0)
+    perr = torch.where(see, abs(scale) * (1.1 * (xerr + approx) + (u + 4 * f32) * (x * sg).abs()) + step, 0.0)
     p = torch.where(see, x * sg * scale, 0.0)
     out = p @ vv
     n = k.shape[1] + 4

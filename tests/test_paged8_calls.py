@@ -191,3 +191,48 @@ def test_append_counts_up_the_versions_of_what_it_writes():
     _meta_append(kv_cache=t["kv_cache"], kv_scale=t["kv_scale"])   # (tensors of inference mode have no version)
     with pytest.raises(RuntimeError, match="no gradients"):
         _meta_append(kv_scale=meta(6, 2, 2, 2, dtype=FP32).requires_grad_())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("users,new", [(4, 1), (4, 20), (MANY, 40)])
+@pytest.mark.parametrize("window,sink", [(60, 3), (1000, 0)])
+def test_a_model_is_served_with_the_scale_it_was_trained_with(dtype, users, new, window, sink):
+    """The last rows of hstu_window over whole sequences, with its scale of 1 / max_seq_len, are those of hstu_paged_8bit over the same
+    keys and values - what the cache holds, exact in 16 bits - if that scale is passed: 0 would mean 1 / (the longest query here)."""
+    from oracle import hstu_cache_oracle as CO
+    rng = np.random.default_rng(68)
+    cached = rng.integers(new, 500, users)
+    args = on_gpu(make(cached, np.full(users, new), None, 4, 2, 64, dtype, INT8, 64, 4, seed=69))
+    value = (args["kv_cache"].float().unflatten(2, (-1, 4)) * args["kv_scale"][:, :, :, None, :, None]).flatten(2, 3)
+    po = args["page_offsets"].tolist()
+    k, v = (torch.cat([value[args["page_ids"][po[b]:po[b + 1]], w].flatten(0, 1)[:n] for b, n in enumerate(cached.tolist())]).to(dtype)
+            for w in (0, 1))
+    off = args["seq_offset_k"]
+    q = torch.randn(int(off[-1]), 4, 64, device="cuda").to(dtype)
+    last = torch.cat([torch.arange(int(e) - new, int(e)) for e in off[1:]]).cuda()
+    q[last] = args["q"]
+    trained = ops_rec.ascendc.attention.hstu_window(q, k, v, window, sink, 512, 0, 0.0, off, None, None, 0, args["alpha"])[last]
+    served = paged_op(**{n: t for n, t in args.items()}, silu_scale=1 / 512, window=window, num_sink=sink)
+    _, tol = CO.paged(**args, silu_scale=1 / 512, window=window, num_sink=sink)
+    assert ((trained.double() - served.double()).abs() <= 2 * tol + 1e-7).all()
+    if new > 1:
+        other = paged_op(**args, window=window, num_sink=sink)   # (1 / new)
+        assert (other.double() - served.double() * 512 / new).abs().max() <= 2.0 ** -6 * other.double().abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [3.0, -0.7, 1.0, 2.0 ** -14])
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_scales_of_the_call(scale, dtype):
+    """Above 1, below 0 and small, on every path and of hstu_window."""
+    from tests.test_paged8 import check_paged
+    for users, new, targets, d, page in ((3, 1, None, 64, 32), (3, 20, 5, 64, 32), (MANY, 40, 3, 64, 64), (3, 20, 5, 64, 24), (3, 5, None, 160, 16)):
+        rng = np.random.default_rng(70)
+        cached = rng.integers(new, 200, users)
+        args = make(cached, np.full(users, new), None if targets is None else np.full(users, targets), 4, 2, d, dtype, INT8, page, 8, seed=71)
+        for window in (0, 50):
+            check_paged(args | dict(silu_scale=scale), window, 2, label=(users, new, d, page))
+    from tests import test_window as W
+    args, grad = W.make([300, 77], 2, 2, 64, dtype=dtype, seed=72)
+    W.check(args | dict(silu_scale=scale), grad, 50, 2)
