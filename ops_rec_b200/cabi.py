@@ -350,6 +350,31 @@ def hstu_jagged_backward(grad, q, k, v, mask=None, attn_bias=None, mask_type=0, 
     return dq, dk, dv, dbias
 
 
+def _check_rows(q, k, v):
+    if not (q.dtype == k.dtype == v.dtype):
+        raise HstuError(-2, f"q, k and v must have the same dtype, but are {q.dtype}, {k.dtype} and {v.dtype}")
+    if k.dim() != 3 or v.dim() != 3 or k.shape[:2] != v.shape[:2] or k.shape[2] != q.shape[2]:
+        raise HstuError(-2, "k and v must agree in tokens and heads, q and k in the head dim")
+
+
+def _indices(seq_offset, **others):
+    """The index tensors of a call as the kernels read them: seq_offset's integers, contiguous, as many as the batch asks for."""
+    import torch
+    if seq_offset.dtype not in (torch.int32, torch.int64):
+        raise HstuError(-2, "seq_offset must be int32 or int64")
+    batch = seq_offset.numel() - 1
+    for name, n in (("seq_offset_k", batch + 1), ("page_offsets", batch + 1), ("last_page_len", batch), ("num_target", batch)):
+        t = others.get(name)
+        if t is not None and (t.numel() < n or "offset" in name and t.numel() != n):
+            raise HstuError(-2, f"{name} must have {n} entries for a batch of {batch}, but has {t.numel()}")
+    return [seq_offset.contiguous()] + [t.to(seq_offset.dtype).contiguous() if t is not None else None for t in others.values()]
+
+
+def _int32(n):
+    """A window or a number of sinks: beyond any sequence is beyond any sequence."""
+    return max(min(int(n), 0x7fffffff), -1)
+
+
 def hstu_window_forward(q, k, v, window, num_sink=0, max_seq_len=0, max_seq_len_k=0, silu_scale=0.0, seq_offset=None,
                         seq_offset_k=None, num_target=None, target_group_size=0, alpha=1.0, *, flags=0, return_status=False):
     """ops_rec::hstu_window through hstu_window_fwd on CUDA tensors; with return_status it synchronises and returns the
@@ -357,6 +382,8 @@ def hstu_window_forward(q, k, v, window, num_sink=0, max_seq_len=0, max_seq_len_
     import torch
     if q.dim() != 3:
         raise HstuError(-2, "The q should be 3D in jagged layout")
+    _check_rows(q, k, v)
+    seq_offset, seq_offset_k, num_target = _indices(seq_offset, seq_offset_k=seq_offset_k, num_target=num_target)
     if not q.is_cuda:
         raise HstuError(-2, "tensors must live on a CUDA device; there is no CPU implementation")
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
@@ -364,7 +391,7 @@ def hstu_window_forward(q, k, v, window, num_sink=0, max_seq_len=0, max_seq_len_
     fwd, keep = make_args(q, k, v, out, seq_offset, seq_offset_k=seq_offset_k, max_seq_len=max_seq_len,
                           max_seq_len_k=max_seq_len_k or None, silu_scale=silu_scale, num_target=num_target,
                           target_group_size=target_group_size, alpha=alpha, flags=flags)
-    a = HstuWindowArgs(C.sizeof(HstuWindowArgs), int(window), int(num_sink), 0, fwd)
+    a = HstuWindowArgs(C.sizeof(HstuWindowArgs), _int32(window), _int32(num_sink), 0, fwd)
     n = C.c_uint64(0)
     check(load().hstu_window_fwd_get_workspace_size(C.byref(a), C.byref(n)))
     ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
@@ -385,6 +412,12 @@ def hstu_window_backward(grad, q, k, v, window, num_sink=0, max_seq_len=0, max_s
     import torch
     if q.dim() != 3:
         raise HstuError(-2, "The q should be 3D in jagged layout")
+    _check_rows(q, k, v)
+    if grad.dtype != q.dtype or tuple(grad.shape) != (q.shape[0], q.shape[1], v.shape[2]):
+        raise HstuError(-2, "grad must be [total_q, heads_q, dim_v] of q's dtype")
+    if grad.device != q.device:
+        raise ValueError(f"grad is on {grad.device} but q is on {q.device}")
+    seq_offset, seq_offset_k, num_target = _indices(seq_offset, seq_offset_k=seq_offset_k, num_target=num_target)
     if not q.is_cuda:
         raise HstuError(-2, "tensors must live on a CUDA device; there is no CPU implementation")
     grad, q, k, v = grad.contiguous(), q.contiguous(), k.contiguous(), v.contiguous()
@@ -393,7 +426,7 @@ def hstu_window_backward(grad, q, k, v, window, num_sink=0, max_seq_len=0, max_s
                           max_seq_len_k=max_seq_len_k or None, silu_scale=silu_scale, num_target=num_target,
                           target_group_size=target_group_size, alpha=alpha, flags=flags)
     b = HstuJaggedBwdArgs(C.sizeof(HstuJaggedBwdArgs), 0, fwd, grad.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None)
-    a = HstuWindowBwdArgs(C.sizeof(HstuWindowBwdArgs), int(window), int(num_sink), 0, b)
+    a = HstuWindowBwdArgs(C.sizeof(HstuWindowBwdArgs), _int32(window), _int32(num_sink), 0, b)
     n = C.c_uint64(0)
     check(load().hstu_window_bwd_get_workspace_size(C.byref(a), C.byref(n)))
     ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
@@ -485,13 +518,14 @@ def hstu_cache_append(k, v, kv_cache, kv_scale, seq_offset, page_offsets, page_i
     import torch
     if k.dim() != 3 or v.shape != k.shape:
         raise HstuError(-2, "k and v must be [tokens, heads_k, dim] and of one shape")
+    _check_rows(k, k, v)
+    idx = _indices(seq_offset, num_target=num_target, page_offsets=page_offsets, page_ids=page_ids, last_page_len=last_page_len)
     if not k.is_cuda:
         raise HstuError(-2, "tensors must live on a CUDA device; there is no CPU implementation")
     for t in (v, kv_cache, kv_scale, seq_offset, page_offsets, page_ids, last_page_len, num_target):
         if t is not None and t.device != k.device:
             raise ValueError(f"a tensor is on {t.device} but k is on {k.device}")
-    k, v, it = k.contiguous(), v.contiguous(), seq_offset.dtype
-    idx = [t.to(it).contiguous() if t is not None else None for t in (seq_offset, num_target, page_offsets, page_ids, last_page_len)]
+    k, v = k.contiguous(), v.contiguous()
     status = torch.zeros(1, dtype=torch.int32, device=k.device) if return_status else None
     ptr = lambda t: t.data_ptr() if t is not None else None   # noqa: E731
     a = HstuCacheAppendArgs(C.sizeof(HstuCacheAppendArgs), _dtype_code(k.dtype), _held_code(kv_cache), kv_cache.shape[2],
@@ -511,22 +545,26 @@ def hstu_paged_8bit_forward(q, k, v, kv_cache, kv_scale, max_seq_len=0, max_seq_
     import torch
     if q.dim() != 3:
         raise HstuError(-2, "The q should be 3D in jagged layout")
+    _check_rows(q, k, v)
+    if k.shape[0] != q.shape[0]:
+        raise HstuError(-2, "k and v hold the same tokens as q (only their target rows are read)")
+    seq_offset, seq_offset_k, page_offsets, page_ids, last_page_len, num_target = conv = _indices(
+        seq_offset, seq_offset_k=seq_offset_k, page_offsets=page_offsets, page_ids=page_ids, last_page_len=last_page_len,
+        num_target=num_target)
     if not q.is_cuda:
         raise HstuError(-2, "tensors must live on a CUDA device; there is no CPU implementation")
     block = _check_held(kv_cache, kv_scale, k.shape[1], k.shape[2])
     for t in (kv_cache, kv_scale, page_offsets, page_ids, last_page_len):
         if t.device != q.device:
             raise ValueError(f"a page-table tensor is on {t.device} but q is on {q.device}")
-    q, k, v, it = q.contiguous(), k.contiguous(), v.contiguous(), seq_offset.dtype
-    seq_offset_k, page_offsets, page_ids, last_page_len = conv = [
-        t.to(it).contiguous() for t in (seq_offset_k, page_offsets, page_ids, last_page_len)]
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     out = torch.empty(q.shape[0], q.shape[1], v.shape[2], dtype=q.dtype, device=q.device)
     base, keep = make_args(q, k, v, out, seq_offset, seq_offset_k=seq_offset_k, max_seq_len=max_seq_len,
                            max_seq_len_k=max_seq_len_k or None, silu_scale=silu_scale, num_target=num_target,
                            target_group_size=target_group_size, alpha=alpha, flags=flags)
     p = HstuPagedArgs(C.sizeof(HstuPagedArgs), kv_cache.shape[2], base, kv_cache.data_ptr(), page_offsets.data_ptr(),
                       page_ids.data_ptr(), last_page_len.data_ptr(), None, kv_cache.shape[0], page_ids.numel())
-    a = HstuPaged8Args(C.sizeof(HstuPaged8Args), _held_code(kv_cache), block, int(window), int(num_sink), 0, kv_scale.data_ptr(), p)
+    a = HstuPaged8Args(C.sizeof(HstuPaged8Args), _held_code(kv_cache), block, _int32(window), _int32(num_sink), 0, kv_scale.data_ptr(), p)
     n = C.c_uint64(0)
     check(load().hstu_paged_8bit_fwd_get_workspace_size(C.byref(a), C.byref(n)))
     # (workspace_fill: tests fill the workspace with a byte pattern first - nothing the call reads may be uninitialised)
