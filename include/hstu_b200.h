@@ -221,7 +221,9 @@ HSTU_API int hstu_jagged_bwd(const HstuJaggedBwdArgs* args, void* workspace, uin
  * to itself.  A row that sees nothing (len_q > len_k) gives zeros.  Arithmetic and traffic follow the visible tiles, not
  * len^2.
  *   fwd        the jagged arguments, with mask_type HSTU_MASK_TRIL and without mask, attn_bias and num_context
- *   window     >= 1, the row's own key among them; window >= max_seq_len_k is the jagged operator
+ *   window     >= 1, the row's own key among them; window >= max_seq_len_k gives the jagged operator's values (from half of the
+ *              sequence on hstu_jagged_fwd can be the faster call: long 16-bit sequences have a kernel there that knows no windows)
+ * fp16: results are finite wherever the jagged operator's are, though P and dS are formed without the scale, for their bits.
  *   num_sink   >= 0 */
 typedef struct HstuWindowArgs {
   uint32_t struct_bytes;  /* sizeof(HstuWindowArgs) */

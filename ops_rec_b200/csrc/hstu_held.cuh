@@ -1,5 +1,5 @@
-// The 8-bit forms a paged cache holds its rows in, for the kernels that write and read one (hstu_append.cu, hstu_paged.cu,
-// hstu_paged8.cu): value = number * scale, one fp32 scale per block of tokens and head.
+// The 8-bit forms a paged cache holds its rows in, for the kernels that write and read one (hstu_append.cu; hstu_decode8.cu,
+// hstu_rows8.cu and hstu_paged.cu through hstu_mma8.cuh): value = number * scale, one fp32 scale per block of tokens and head.
 #pragma once
 
 #include <cuda_bf16.h>

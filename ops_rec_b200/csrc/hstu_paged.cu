@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kGatherThreads) hstu_paged_gather_kernel(const
 // hstu_paged_8bit, calls that the kernel for short sequences then reads in place: the pages of the table, slot by slot, in the
 // call's type - a cache of its own whose page i is slot i, with the table of its pages.  Rows nobody reads (behind a sequence's
 // last one, and a whole tile of 64 keys away from what a window or its sinks show) stay unwritten.  HBM-bound: one byte in, two
-// out (10 600 pages of 128 rows, 4 heads of 64, 80 % full: 1.5 GB, 244 us, 6.2 TB/s; in pieces of 16 numbers, whose stores do not
+// out (9760 pages of 128 rows, 4 heads of 64, 78 % full: 1.5 GB, 244 us, 6.2 TB/s; in pieces of 16 numbers, whose stores do not
 // fill lines, 263); the pre-pass runs beside it (15 us of 600 of such a call).
 constexpr int kUnpackThreads = 256;
 
