@@ -214,7 +214,7 @@ hstu_bwd_tc_kernel(const BwdParams bp, const __grid_constant__ CUtensorMap tm_a1
   BwdBars* bars = reinterpret_cast<BwdBars*>(base_ptr + (2 + kRing1 + kRing2) * kTileBytes + (staged ? 2 * kTileM * 128 : 0));
   const BwdWaiter w{&bars->abort_flag, p.ws_header};
   constexpr bool kTurns = kWin && std::is_same<T, __half>::value;   // (see KParams)
-  if (kTurns && second_turn_idle(p)) return;
+  if (kTurns && second_turn_idle<kDKV>(p)) return;
 
   // The two passes do not depend on each other, only on the pre-pass before them.  The dK/dV pass is launched with
   // programmatic stream serialization behind the dQ pass, which lets it go at once: its CTAs take the SMs as the dQ

@@ -63,6 +63,7 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
+// (CTAs an SM: what 96 and 168 registers allow; without the bound some instantiations take 118 and 134, four of the one kind)
 template <int D, typename T, typename H, bool kWin, bool kTanh>
 __global__ void __launch_bounds__(kDecThreads, D == 64 ? 5 : 3) hstu_decode8_kernel(const DecParams d) {
   using C = DecCfg<D>;

@@ -148,7 +148,7 @@ hstu_short_kernel(const KParams p, const __grid_constant__ CUtensorMap tm_q, con
   const int halves_qk = C::kHalves == 1 ? 1 : (p.dqk + 63) >> 6;
   const int halves_v = C::kHalves == 1 ? 1 : (p.dv + 63) >> 6;
   constexpr bool kTurns = std::is_same<T, __half>::value && !kBias;   // (see KParams)
-  if (kTurns && second_turn_idle(p)) return;
+  if (kTurns && second_turn_idle<true>(p)) return;
 
   if (threadIdx.x == 0) {
     ptx::prefetch_tensormap(&tm_q);

@@ -125,10 +125,12 @@ __device__ __forceinline__ uint32_t visible_bits(const WinBounds& rb, int j0) {
          (low_bits(rb.hi3 + 1 - j0) & ~low_bits(rb.lo3 - j0));
 }
 
-// KParams::turn.  The start of a kernel that has two, for every thread of the grid: the first lets the second go, which takes
-// SMs as they become free, waits for the first one's mark and results, and leaves (true) if there is none.
-__device__ __forceinline__ bool second_turn_idle(const KParams& p) {
-  if (p.turn == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+// KParams::turn.  The start of a kernel that has two, for every thread of the grid: the second takes SMs as they become free, waits
+// for the first one's mark and results, and leaves (true) if there is none.  kRelease: the grid behind this one is that second
+// turn, and the first lets it go at once.  (Not the backward's dQ pass: the dK/dV pass behind it reads the pre-pass's lists
+// without a wait of its own, so it must not start before the dQ pass has waited for them.)
+template <bool kRelease> __device__ __forceinline__ bool second_turn_idle(const KParams& p) {
+  if (kRelease && p.turn == 1) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (p.turn != 2) return false;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   return *reinterpret_cast<volatile uint32_t*>(p.ws_header + 5) == 0;
