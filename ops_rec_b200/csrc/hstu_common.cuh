@@ -95,8 +95,8 @@ struct KParams {
   // Where P and dS are formed without the scale (out_scale; fp16 on the tensor cores), they may be beyond fp16 although the scaled
   // ones are not.  Such a call takes two turns: 1 notes in the header that sums came out infinite or NaN; 2 ends at once when none
   // did, and otherwise forms them again with the scale inside P and dS and stores those the first turn left infinite or NaN.  0:
-  // one turn.  (16 sequences of 1024 - 4096 rows, fp16, window 512: forward and backward 856 -> 863 us; 8 of 20 - 200, forward
-  // 14.5 -> 15.1.)
+  // one turn.  (fp16: 16 sequences of 1024 - 4096 rows, window 512, forward and backward 852 -> 860 us; 8 of 20 - 200, forward
+  // 14.4 -> 15.9.)
   int turn;
 };
 
